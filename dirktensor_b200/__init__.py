@@ -29,4 +29,17 @@ from .attention import (  # noqa: F401
     rope_theta,
 )
 
+_SERVING = ("KVCache", "TokenLogProbs", "cache_attention_forward", "prefix_attention_forward", "token_log_probs",
+            "token_log_probs_backward")
+
+
+def __getattr__(name):
+    """The serving operators, which work on torch tensors only and import it when first used."""
+    if name in _SERVING:
+        from . import serving
+
+        return getattr(serving, name)
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+
+
 lib()

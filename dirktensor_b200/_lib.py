@@ -72,6 +72,19 @@ class dt_model_weights(ctypes.Structure):
     ]
 
 
+class dt_kv_cache(ctypes.Structure):
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("num_pages", ctypes.c_int),
+        ("page_size", ctypes.c_int),
+        ("kv_heads", ctypes.c_int),
+        ("format", ctypes.c_int),
+    ]
+
+
 _lib = None
 
 _P = ctypes.c_void_p
@@ -135,6 +148,14 @@ SIGNATURES = {
     "dt_attn_create_sharded": (_I, [ctypes.POINTER(dt_attn_weights), _P, _I, ctypes.POINTER(_P)]),
     "dt_attn_forward_sharded": (_I, [_P, _P, _I, _I, _P, _I, _P, _P]),
     "dt_attn_forward_sharded_host": (_I, [_P, _P, _I, _I, _P, _I, _P]),
+    "dt_kv_cache_append": (_I, [_P, _P, _LL, _LL, _P, _LL, _LL, _I, _P, _LL, _I, _P, _P, _I, _I, _P]),
+    "dt_kv_cache_read": (_I, [_P, _P, _P, _I, _P, _LL, _I, _P, _P, _I, _I, _P]),
+    "dt_cache_attn_fwd": (_I, [_P, _P, _LL, _LL, _I, _P, _P, _P, _P, _LL, _I, _P, _P, _I, _I, _I, _F, _P]),
+    "dt_prefix_attn_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I]),
+    "dt_prefix_attn_fwd": (_I, [_P, _P, _LL, _LL, _I, _P, _P, _P, _P, _I, _P, _LL, _I, _P, _P, _I, _I, _I, _F, _P, _SZ,
+                                _P]),
+    "dt_token_log_probs": (_I, [_P, _I, _LL, _I, _I, _P, _I, _I, _P, _P, _P, _P, _P, _P]),
+    "dt_token_log_probs_bwd": (_I, [_P, _I, _LL, _I, _I, _P, _I, _P, _P, _P, _P, _P, _LL, _P]),
     "dt_attn_create_sharded_from_npy": (_I, [ctypes.c_char_p, ctypes.c_uint, _P, _I, ctypes.POINTER(_P)]),
 }
 

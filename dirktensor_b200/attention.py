@@ -448,6 +448,20 @@ class OlmoModel:
         check(lib().dt_model_forward_host(self._h, ids.ctypes.data, B, T, logits.ctypes.data))
         return logits
 
+    def log_probs(self, ids, top: int = 0):
+        """Scores of a prompt's own tokens: ``TokenLogProbs`` of ids [B, T] (CUDA tensor), where
+        log_prob[b, t] is that of ids[b, t + 1] after ids[b, : t + 1] (0 in the last column, which
+        has no next token), and entropy and the ``top`` alternatives are those of the same
+        distribution.  -log_prob is the loss of each label of CrossEntropyLoss.cpp:8-43."""
+        from .serving import token_log_probs
+
+        torch = _torch()
+        if not (_is_torch(ids) and ids.is_cuda and ids.dim() == 2):
+            raise ValueError("ids must be a CUDA tensor [B, T]")
+        targets = torch.full(ids.shape, -100, dtype=torch.int32, device=ids.device)
+        targets[:, :-1] = ids[:, 1:]
+        return token_log_probs(self.forward(ids), targets, top=top)
+
     __call__ = forward
 
     def close(self):

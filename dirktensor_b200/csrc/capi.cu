@@ -19,11 +19,14 @@
 #include <vector>
 
 #include "../../include/dirktensor_b200.h"
+#include "cache_attn.cuh"
 #include "dt_common.cuh"
 #include "flash_bwd.cuh"
 #include "flash_fwd.cuh"
 #include "gemm.cuh"
 #include "gemm2sm.cuh"
+#include "kv_cache.cuh"
+#include "logprobs.cuh"
 #include "model.cuh"
 #include "prologue.cuh"
 
@@ -2540,3 +2543,5 @@ int dt_model_forward_host(dt_model* m, const uint32_t* tokens, int B, int T, flo
 }
 
 }  // extern "C"
+
+#include "serving.cuh"

@@ -1,0 +1,307 @@
+"""Serving operators over the C ABI: a paged K/V cache of 8-bit codes, the attention of new
+tokens that reads it (alone, or behind a prefix that a batch shares), and log probabilities of
+given tokens with their gradient.
+
+Arguments are CUDA torch tensors; calls run on the current stream of the tensors' device, do not
+synchronise, and raise ``ValueError`` for arguments they cannot take and ``DTError`` for
+what the library refuses.  The reference has no counterpart: it recomputes every prefix, and its
+CrossEntropyLoss.cpp:8-43 reduces the loss to one number.
+"""
+from __future__ import annotations
+
+import ctypes
+from contextlib import nullcontext
+from typing import NamedTuple, Optional
+
+import torch
+
+from ._lib import check, dt_kv_cache, lib
+from .attention import FlashAttentionResult, head_dim, n_heads
+
+_CODES = {"int8": (torch.int8, 0), "e4m3": (torch.float8_e4m3fn, 1)}
+_FORMAT_OF = {torch.int8: 0, torch.float8_e4m3fn: 1}
+_VALUES = (torch.bfloat16, torch.float32)
+
+
+def _on(device: torch.device):
+    """The library works on the current device: makes it the tensors' own."""
+    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _stream(device: torch.device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _values(name: str, t, device, heads: Optional[int] = None):
+    """[B, T, heads, 128] of bf16 or fp32 whose rows start on 16-byte boundaries."""
+    if not (isinstance(t, torch.Tensor) and t.device == device and t.dtype in _VALUES and t.dim() == 4
+            and t.shape[3] == head_dim):
+        raise ValueError(f"{name} must be a bfloat16 or float32 tensor [B, T, heads, {head_dim}] on {device}")
+    if heads is not None and t.shape[2] != heads:
+        raise ValueError(f"{name} must have {heads} heads")
+    s = t.stride()
+    if (t.numel() and (s[3] != 1 or (t.shape[2] > 1 and s[2] != head_dim) or (s[0] | s[1]) % (16 // t.element_size())
+                       or s[0] < 0 or s[1] < 0 or t.data_ptr() & 15)):
+        raise ValueError(f"{name}: heads must be {head_dim} apart, and rows must start on 16-byte boundaries")
+    return s
+
+
+def _ints(name: str, t, device, n: Optional[int]):
+    if t is None:
+        return None
+    if not (isinstance(t, torch.Tensor) and t.device == device and t.dtype == torch.int32 and t.dim() == 1
+            and (n is None or t.shape[0] == n) and (t.shape[0] < 2 or t.stride(0) == 1)):
+        raise ValueError(f"{name} must be a contiguous int32 tensor{'' if n is None else f' of {n} entries'} on {device}")
+    return t.data_ptr()
+
+
+def _table(t, device, B: int):
+    if not (isinstance(t, torch.Tensor) and t.device == device and t.dtype == torch.int32 and t.dim() == 2
+            and t.shape[0] == B):
+        raise ValueError(f"page_table must be an int32 tensor [{B}, pages] on {device}")
+    n = t.shape[1]
+    if (n > 1 and t.stride(1) != 1) or (B > 1 and t.stride(0) < n):
+        raise ValueError("page_table rows must be contiguous and must not overlap")
+    return t.data_ptr(), max(t.stride(0), n), n
+
+
+class KVCache:
+    """A pool of pages that holds K and V of past tokens as 8-bit codes, one fp32 scale per row of
+    128 values: ``k``, ``v`` [num_pages, kv_heads, page_size, 128] (``torch.int8`` or
+    ``torch.float8_e4m3fn``), ``k_scale``, ``v_scale`` [num_pages, kv_heads, page_size].
+
+    The caller hands out pages: ``page_table`` [B, pages] (int32) names, for each sequence, the
+    page of its first ``page_size`` tokens, then of the next, and so on.  Entries that no token
+    reaches yet may be anything; a page id outside the pool is skipped, not followed.
+    """
+
+    def __init__(self, num_pages: int, page_size: int = 64, kv_heads: int = n_heads, format: str = "int8",
+                 device: int = 0):
+        if format not in _CODES:
+            raise ValueError(f"format must be one of {sorted(_CODES)}")
+        dev = torch.device("cuda", device) if isinstance(device, int) else torch.device(device)
+        shape = (int(num_pages), int(kv_heads), int(page_size))
+        codes = [torch.zeros(shape + (head_dim,), dtype=torch.int8, device=dev).view(_CODES[format][0])
+                 for _ in range(2)]
+        self._take(*codes, *(torch.zeros(shape, dtype=torch.float32, device=dev) for _ in range(2)))
+
+    @classmethod
+    def from_tensors(cls, k, v, k_scale, v_scale) -> "KVCache":
+        """A cache over the caller's own arrays, in the layout above."""
+        self = cls.__new__(cls)
+        self._take(k, v, k_scale, v_scale)
+        return self
+
+    def _take(self, k, v, k_scale, v_scale):
+        if not (isinstance(k, torch.Tensor) and k.is_cuda and k.dtype in _FORMAT_OF and k.dim() == 4
+                and k.shape[3] == head_dim):
+            raise ValueError(f"k must be an int8 or float8_e4m3fn CUDA tensor [pages, heads, page_size, {head_dim}]")
+        for name, t, shape, dtype in (("k", k, k.shape, k.dtype), ("v", v, k.shape, k.dtype),
+                                      ("k_scale", k_scale, k.shape[:3], torch.float32),
+                                      ("v_scale", v_scale, k.shape[:3], torch.float32)):
+            if not (isinstance(t, torch.Tensor) and t.device == k.device and t.dtype == dtype and t.shape == shape
+                    and t.is_contiguous()):
+                raise ValueError(f"{name} must be a contiguous {dtype} tensor {list(shape)} on {k.device}")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.num_pages, self.kv_heads, self.page_size = k.shape[:3]
+        if self.page_size not in (16, 32, 64, 128, 256):
+            raise ValueError("page_size must be 16, 32, 64, 128 or 256")
+        self.device = k.device
+        self._c = dt_kv_cache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), self.num_pages,
+                              self.page_size, self.kv_heads, _FORMAT_OF[k.dtype])
+        self._ref = ctypes.byref(self._c)
+
+    @property
+    def format(self) -> str:
+        return "int8" if self.k.dtype == torch.int8 else "e4m3"
+
+    def append(self, k, v, page_table, start=None, lens=None) -> None:
+        """Quantises k, v [B, T, kv_heads, 128] (bf16 or fp32) into the cache: token t < lens[b]
+        of sequence b at position start[b] + t.  start, lens: int32 [B] tensors (default 0 and
+        T).  Tokens without a valid page are skipped; where the page table gives two tokens of
+        the call one slot, the one of the highest (sequence, position) is kept."""
+        ks, vs = _values("k", k, self.device, self.kv_heads), _values("v", v, self.device, self.kv_heads)
+        if k.shape != v.shape or k.dtype != v.dtype:
+            raise ValueError("k and v differ in shape or type")
+        B, T = k.shape[:2]
+        table, stride, n = _table(page_table, self.device, B)
+        with _on(self.device):
+            check(lib().dt_kv_cache_append(self._ref, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
+                                           int(k.dtype == torch.float32), table, stride, n,
+                                           _ints("start", start, self.device, B), _ints("lens", lens, self.device, B),
+                                           B, T, _stream(self.device)))
+
+    def read(self, page_table, start, T: int, lens=None, dtype=torch.bfloat16):
+        """The values of positions start[b] .. start[b] + T - 1 as k, v [B, T, kv_heads, 128] of
+        ``dtype`` (bf16 or fp32).  Rows t >= lens[b] and positions without a valid page are zeros."""
+        if dtype not in _VALUES:
+            raise ValueError("dtype must be bfloat16 or float32")
+        B = page_table.shape[0]
+        table, stride, n = _table(page_table, self.device, B)
+        k = torch.empty((B, int(T), self.kv_heads, head_dim), dtype=dtype, device=self.device)
+        v = torch.empty_like(k)
+        with _on(self.device):
+            check(lib().dt_kv_cache_read(self._ref, k.data_ptr(), v.data_ptr(), int(dtype == torch.float32), table,
+                                         stride, n, _ints("start", start, self.device, B),
+                                         _ints("lens", lens, self.device, B), B, int(T), _stream(self.device)))
+        return k, v
+
+
+def _outputs(q, out, return_stats):
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif not (out.device == q.device and out.dtype == q.dtype and out.shape == q.shape and out.is_contiguous()):
+        raise ValueError("out must be a contiguous tensor of q's shape and type")
+    if not return_stats:
+        return out, None, None
+    return out, *(torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) for _ in range(2))
+
+
+def cache_attention_forward(q, cache: KVCache, page_table, seq_lens, scale: float, q_lens=None, out=None,
+                            return_stats: bool = False):
+    """Attention of new tokens over the cache; flash_attention_forward's form for single tokens.
+
+    q: [B, T, heads, 128] bf16 or fp32, heads a multiple of the cache's.  seq_lens (int32 [B])
+    counts each sequence's tokens in the cache, the queries' own included: query t sees the keys
+    j < seq_lens[b] - q_lens[b] + t + 1.  q_lens (int32 [B], default T): rows past it are padding
+    and come back as zeros, as do rows that see no key.  Returns the output [B, T, heads, 128]
+    of q's type, or with return_stats a ``FlashAttentionResult`` with softmax_m and softmax_l.
+    """
+    s = _values("q", q, cache.device)
+    B, T, H = q.shape[:3]
+    table, stride, n = _table(page_table, cache.device, B)
+    lens = _ints("seq_lens", seq_lens, cache.device, B)
+    o, m, l = _outputs(q, out, return_stats)
+    with _on(cache.device):
+        check(lib().dt_cache_attn_fwd(cache._ref, q.data_ptr(), s[0], s[1], int(q.dtype == torch.float32), o.data_ptr(),
+                                      m.data_ptr() if return_stats else None, l.data_ptr() if return_stats else None,
+                                      table, stride, n, lens, _ints("q_lens", q_lens, cache.device, B), B, T, H,
+                                      float(scale), _stream(cache.device)))
+    return FlashAttentionResult(o, m, l) if return_stats else o
+
+
+def prefix_attention_forward(q, cache: KVCache, prefix_pages, prefix_len: int, page_table, seq_lens, scale: float,
+                             q_lens=None, out=None, return_stats: bool = False):
+    """cache_attention_forward for a batch whose sequences share their first ``prefix_len`` tokens,
+    kept once in the pages ``prefix_pages`` (int32): the prefix is read once for the whole batch.
+    page_table and seq_lens describe what follows the prefix in each sequence; both may be None when
+    nothing does.
+    """
+    s = _values("q", q, cache.device)
+    B, T, H = q.shape[:3]
+    prefix_len = int(prefix_len)
+    pages = _ints("prefix_pages", prefix_pages, cache.device, None)
+    if prefix_len < 0 or prefix_len > (0 if prefix_pages is None else prefix_pages.shape[0] * cache.page_size):
+        raise ValueError("prefix_len must be >= 0 and within prefix_pages")
+    if (page_table is None) != (seq_lens is None):
+        raise ValueError("page_table and seq_lens come together")
+    table, stride, n = (None, 0, 0) if page_table is None else _table(page_table, cache.device, B)
+    lens = _ints("seq_lens", seq_lens, cache.device, B)
+    o, m, l = _outputs(q, out, return_stats)
+    L = lib()
+    nbytes = L.dt_prefix_attn_workspace_bytes(B, T, H, cache.kv_heads, prefix_len)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=cache.device) if nbytes else None
+    with _on(cache.device):
+        check(L.dt_prefix_attn_fwd(cache._ref, q.data_ptr(), s[0], s[1], int(q.dtype == torch.float32), o.data_ptr(),
+                                   m.data_ptr() if return_stats else None, l.data_ptr() if return_stats else None,
+                                   pages, prefix_len, table, stride, n, lens,
+                                   _ints("q_lens", q_lens, cache.device, B), B, T, H, float(scale),
+                                   ws.data_ptr() if nbytes else None, nbytes, _stream(cache.device)))
+    return FlashAttentionResult(o, m, l) if return_stats else o
+
+
+class TokenLogProbs(NamedTuple):
+    log_prob: object       # [...] log probability of each target (None without targets)
+    entropy: object        # [...] of each row's distribution, in nats
+    lse: object            # [...] log of the sum of exponentials
+    top_ids: object        # [..., top] int32, most likely first (None for top = 0)
+    top_log_probs: object  # [..., top]
+
+
+def _rows(name, t):
+    """(row count, row stride) of a tensor [..., V] whose rows are contiguous and evenly spaced."""
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in _VALUES and t.dim() >= 1 and t.shape[-1] >= 1):
+        raise ValueError(f"{name} must be a bfloat16 or float32 CUDA tensor [..., vocabulary]")
+    V = t.shape[-1]
+    if t.is_contiguous():
+        return t.numel() // V, V
+    n, ld = 1, None
+    if V == 1 or t.stride(-1) == 1:
+        for size, stride in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+            if size == 1:
+                continue
+            if ld is None:
+                ld = stride
+            elif stride != n * ld:
+                break
+            n *= size
+        else:
+            if (ld or V) >= V:
+                return n, ld or V
+    raise ValueError(f"{name}: rows must be contiguous and evenly spaced")
+
+
+def _targets(targets, shape, device):
+    if targets is None:
+        return None, 0
+    if not (isinstance(targets, torch.Tensor) and targets.device == device and targets.shape == shape
+            and targets.dtype in (torch.int32, torch.int64) and targets.is_contiguous()):
+        raise ValueError(f"targets must be a contiguous int32 or int64 tensor {list(shape)} on {device}")
+    return targets.data_ptr(), int(targets.dtype == torch.int64)
+
+
+def token_log_probs(logits, targets=None, top: int = 0) -> TokenLogProbs:
+    """Log probabilities of given tokens, with each distribution's entropy and its ``top`` (0..32)
+    most likely tokens.
+
+    logits: [..., V] fp32 or bf16 (rows may be spaced apart); targets: int32 or int64 [...].
+    A target outside 0..V-1, such as an ignored label's -100, gives 0.  Ties among the
+    alternatives go to the lower id.  Logits of -inf have probability 0.
+    """
+    n, ld = _rows("logits", logits)
+    V, shape, dev = logits.shape[-1], logits.shape[:-1], logits.device
+    t, t64 = _targets(targets, shape, dev)
+    top = int(top)
+    if not 0 <= top <= min(32, V):
+        raise ValueError("top must be 0..32 and at most the vocabulary")
+    lp = torch.empty(shape, dtype=torch.float32, device=dev) if targets is not None else None
+    ent, lse = torch.empty(shape, dtype=torch.float32, device=dev), torch.empty(shape, dtype=torch.float32, device=dev)
+    ids = tlp = None
+    if top:
+        ids = torch.empty(shape + (top,), dtype=torch.int32, device=dev)
+        tlp = torch.empty(shape + (top,), dtype=torch.float32, device=dev)
+    with _on(dev):
+        check(lib().dt_token_log_probs(logits.data_ptr(), int(logits.dtype == torch.float32), ld, n, V, t, t64, top,
+                                       lp.data_ptr() if t else None, ent.data_ptr(), lse.data_ptr(),
+                                       ids.data_ptr() if top else None, tlp.data_ptr() if top else None, _stream(dev)))
+    return TokenLogProbs(lp, ent, lse, ids, tlp)
+
+
+def token_log_probs_backward(logits, targets, lse, entropy, d_log_prob, d_entropy=None, out=None):
+    """Gradient of token_log_probs with respect to the logits, of their shape and type, from its
+    lse and entropy and the upstream gradients (fp32; d_log_prob or d_entropy may be None).
+    ``out`` may be the logits themselves."""
+    n, ld = _rows("logits", logits)
+    V, shape, dev = logits.shape[-1], logits.shape[:-1], logits.device
+    t, t64 = _targets(targets, shape, dev)
+    if d_log_prob is not None and targets is None:
+        raise ValueError("d_log_prob needs targets")
+    if d_entropy is not None and entropy is None:
+        raise ValueError("d_entropy needs entropy")
+    for name, x in (("lse", lse), ("entropy", entropy), ("d_log_prob", d_log_prob), ("d_entropy", d_entropy)):
+        if x is None and name != "lse":
+            continue
+        if not (isinstance(x, torch.Tensor) and x.device == dev and x.dtype == torch.float32 and x.shape == shape
+                and x.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous float32 tensor {list(shape)} on {dev}")
+    if out is None:
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+    elif out.device != dev or out.dtype != logits.dtype or out.shape != logits.shape:
+        raise ValueError("out must have the logits' shape and type")
+    dn, dld = _rows("out", out)
+    ptr = lambda x: None if x is None else x.data_ptr()  # noqa: E731
+    with _on(dev):
+        check(lib().dt_token_log_probs_bwd(logits.data_ptr(), int(logits.dtype == torch.float32), ld, n, V, t, t64,
+                                           lse.data_ptr(), ptr(entropy), ptr(d_log_prob), ptr(d_entropy),
+                                           out.data_ptr(), dld, _stream(dev)))
+    return out

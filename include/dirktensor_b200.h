@@ -363,6 +363,111 @@ int dt_qk_norm_rope_shard(const float* q, const float* k, const float* v, long l
  * computed like compute_rope_buffers (OlmoAttention.cpp:18-36). */
 int dt_rope_tables(float* sin_out, float* cos_out, int max_seq, int head_dim, float theta);
 
+/* ---- serving: the quantised K/V cache --------------------------------------
+ * No counterpart in the reference, which recomputes every prefix.  K and V of
+ * past tokens are kept as 8-bit codes with one fp32 scale per row of 128
+ * values (one token, one head), in pages of page_size tokens:
+ *   k, v              [num_pages, kv_heads, page_size, 128] one byte per value
+ *   k_scale, v_scale  [num_pages, kv_heads, page_size] fp32
+ * The caller owns the arrays (device, 16-byte aligned) and hands out pages: a
+ * page table holds, for each sequence, the page of its tokens 0..page_size-1,
+ * then of the next page_size tokens, and so on.
+ *   scale = amax / Q, code = round(x * Q / amax) (nearest, ties to even),
+ *   amax = max |x| of the row, Q = 127 (int8) or 448 (e4m3)
+ * so a value reads back within scale / 2 (int8; one fp32 rounding more).  Rows
+ * with amax < 2^-100 are stored as zeros; a row with an infinity or a NaN gets
+ * the scale NaN and reads back as NaN.  num_pages * kv_heads * page_size must
+ * be below 2^31; page_size is 16, 32, 64, 128 or 256. */
+enum dt_kv_format { DT_KV_INT8 = 0, DT_KV_E4M3 = 1 };
+typedef struct dt_kv_cache {
+    void* k;
+    void* v;
+    float* k_scale;
+    float* v_scale;
+    int num_pages;
+    int page_size;
+    int kv_heads;
+    int format; /* enum dt_kv_format */
+} dt_kv_cache;
+
+/* Quantises new tokens into the cache as it writes them.  Token t < lens[b] of
+ * sequence b goes to position start[b] + t; rows t >= lens[b] are not read and
+ * nothing is written for them.  k, v: fp32 (src_f32 = 1) or bf16 device arrays
+ * [B, T, kv_heads, 128], heads 128 elements apart, tokens and sequences at the
+ * given strides (in elements; multiples of 16 bytes).  page_table: device
+ * int[B, max_pages], rows page_table_stride apart.  start, lens: device int[B]
+ * or NULL (0, and T).  A token whose position is negative or past the table,
+ * or whose page id is not in 0..num_pages-1, is skipped.  Where one call maps
+ * several tokens to one slot, the one of the highest (b, position) is kept.
+ * Asynchronous on `stream`. */
+int dt_kv_cache_append(const dt_kv_cache* cache, const void* k, long long k_batch_stride, long long k_token_stride,
+                       const void* v, long long v_batch_stride, long long v_token_stride, int src_f32,
+                       const int* page_table, long long page_table_stride, int max_pages, const int* start,
+                       const int* lens, int B, int T, void* stream);
+/* Reads the values of positions start[b] .. start[b] + T - 1 back into dense
+ * k, v [B, T, kv_heads, 128], fp32 (dst_f32 = 1) or bf16: code * scale, rounded
+ * once.  Rows t >= lens[b], and rows whose position has no valid page, are
+ * written as zeros. */
+int dt_kv_cache_read(const dt_kv_cache* cache, void* k, void* v, int dst_f32, const int* page_table,
+                     long long page_table_stride, int max_pages, const int* start, const int* lens, int B, int T,
+                     void* stream);
+
+/* Attention of new tokens over the cache (the single-token counterpart of
+ * dt_flash_fwd): o = softmax(scale * q k^T) v, where query t of sequence b sees
+ * the keys j < seq_lens[b] - q_lens[b] + t + 1, i.e. seq_lens counts the
+ * sequence's tokens in the cache, the call's own included, and the queries are
+ * the last q_lens[b] of them.  q: bf16 or fp32 (q_f32 = 1) [B, T, heads, 128]
+ * at the given strides (in elements); o: dense [B, T, heads, 128] of q's type;
+ * softmax_m, softmax_l [B, T, heads] as dt_flash_fwd writes them, or NULL.
+ * heads is a multiple of the cache's kv_heads: query head h reads K/V head
+ * h / (heads / kv_heads).  q_lens: device int[B] or NULL (T).  Rows
+ * t >= q_lens[b] and rows that see no key are written as zeros (m = l = 0).
+ * Lengths past the page table are cut to it; keys on a page whose id is not in
+ * 0..num_pages-1 are not seen.  Codes are exact in the products, which are
+ * summed in fp32.  Asynchronous on `stream`. */
+int dt_cache_attn_fwd(const dt_kv_cache* cache, const void* q, long long q_batch_stride, long long q_token_stride,
+                      int q_f32, void* o, float* softmax_m, float* softmax_l, const int* page_table,
+                      long long page_table_stride, int max_pages, const int* seq_lens, const int* q_lens, int B, int T,
+                      int heads, float scale, void* stream);
+/* The same for a batch whose sequences share their first prefix_len tokens:
+ * every query that is not padding sees all keys of the prefix (prefix_pages:
+ * device int[ceil(prefix_len / page_size)]) and then its own sequence's keys
+ * as above, whose positions, page_table and seq_lens count from the prefix's
+ * end.  The prefix is read once for the whole batch, not once per sequence.
+ * max_pages may be 0 (no keys of their own).  workspace: at least
+ * dt_prefix_attn_workspace_bytes, 16-byte aligned (NULL when that is 0); calls
+ * that may overlap on the GPU need one each. */
+size_t dt_prefix_attn_workspace_bytes(int B, int T, int heads, int kv_heads, int prefix_len);
+int dt_prefix_attn_fwd(const dt_kv_cache* cache, const void* q, long long q_batch_stride, long long q_token_stride,
+                       int q_f32, void* o, float* softmax_m, float* softmax_l, const int* prefix_pages, int prefix_len,
+                       const int* page_table, long long page_table_stride, int max_pages, const int* seq_lens,
+                       const int* q_lens, int B, int T, int heads, float scale, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/* ---- scoring: log probabilities of given tokens ----------------------------
+ * For each of N rows of V logits (fp32 or bf16, rows ld elements apart):
+ *   log_prob = x[target] - lse, lse = log sum exp x, entropy = -sum p log p,
+ * and the `top` (0..32) most likely tokens, by logit and then by lower id, with
+ * their log probabilities ([N, top]).  Sums are fp32.  The unreduced loss of
+ * CrossEntropyLoss.cpp:8-43 is -log_prob.  A target outside 0..V-1 (such as
+ * the -100 of an ignored label) gives log_prob 0.  Logits of -inf have
+ * probability 0; a row of nothing else gets lse = log_prob = -inf and entropy
+ * 0; a row with a NaN or +inf gets NaN (its alternatives still ordered, NaN
+ * last).  targets: int32 or int64 [N], may be NULL with log_prob; log_prob,
+ * entropy and lse may each be NULL. */
+int dt_token_log_probs(const void* logits, int logits_f32, long long ld, int N, int V, const void* targets,
+                       int targets_int64, int top, float* log_prob, float* entropy, float* lse, int* top_ids,
+                       float* top_log_probs, void* stream);
+/* Gradient of the above with respect to the logits, of their type, rows d_ld
+ * apart, from lse and entropy as written there and the upstream gradients
+ * d_log_prob and d_entropy (fp32 [N]; either may be NULL for zero):
+ *   d_logits[j] = d_log_prob (1[j = target] - p_j) - d_entropy p_j (log p_j + entropy)
+ * Rows whose lse is -inf get zeros; d_log_prob of an ignored target is not
+ * used.  d_logits may be the logits' own memory (with d_ld = ld). */
+int dt_token_log_probs_bwd(const void* logits, int logits_f32, long long ld, int N, int V, const void* targets,
+                           int targets_int64, const float* lse, const float* entropy, const float* d_log_prob,
+                           const float* d_entropy, void* d_logits, long long d_ld, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
