@@ -249,6 +249,8 @@ int current_device(int* dev) {
     return DT_OK;
 }
 
+int serving_attrs();  // serving.cuh
+
 // Called with g_mu held.
 int ensure_attrs(int dev) {
     DevState& s = g_dev[dev];
@@ -271,6 +273,7 @@ int ensure_attrs(int dev) {
                                  cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kGemmNarrowSmem));
     DT_CUDA(cudaFuncSetAttribute(dt::gemm2::gemm_bf16_tn_2sm_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  (int)kGemm2Smem));
+    DT_TRY(serving_attrs());
     s.attrs = true;
     return DT_OK;
 }

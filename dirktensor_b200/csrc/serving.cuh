@@ -115,6 +115,44 @@ int dt_kv_cache_read(const dt_kv_cache* cache, void* k, void* v, int dst_f32, co
 
 namespace {
 
+// Launches the split kernel with `split` CTAs (a cluster) per work item.
+int launch_split(void (*kernel)(dt::cache_attn::Params), dt::cache_attn::Params& p, int dev, cudaStream_t st) {
+    namespace ca = dt::cache_attn;
+    const long long items = (long long)p.B * p.c.heads * ((p.T * p.group + ca::kRows - 1) / ca::kRows);
+    const long long tiles = ((long long)p.max_pages << p.c.page_shift) / ca::kTile;
+    const int sms = g_dev[dev].num_sms;
+    int split = 1;
+    while (split < ca::kMaxSplit && items * split < 4 * sms && tiles > (long long)split * ca::kWarps) split *= 2;
+    p.split = split;
+    if (items * split > 0x7fffffffll) return fail(DT_ERR_INVALID_ARGUMENT, "B * kv_heads * query rows is too large");
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = DT_PDL;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)split;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(items * split));
+    cfg.blockDim = dim3(ca::kThreads);
+    cfg.dynamicSmemBytes = sizeof(ca::Smem);
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    DT_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
+    return DT_OK;
+}
+
+// Per-device attributes of the kernels below (called with g_mu held, from ensure_attrs).
+int serving_attrs() {
+    using dt::cache_attn::split_kernel;
+    for (auto* k : {split_kernel<0, false>, split_kernel<0, true>, split_kernel<1, false>, split_kernel<1, true>}) {
+        DT_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(dt::cache_attn::Smem)));
+        DT_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    }
+    return DT_OK;
+}
+
 int cache_attn(const dt_kv_cache* cache, const void* q, long long q_batch_stride, long long q_token_stride, int q_f32,
                void* o, float* m, float* l, const int* prefix_pages, int prefix_len, const int* page_table,
                long long page_table_stride, int max_pages, const int* seq_lens, const int* q_lens, int B, int T,
@@ -153,6 +191,13 @@ int cache_attn(const dt_kv_cache* cache, const void* q, long long q_batch_stride
     int dev;
     DT_TRY(prepare_device(&dev));
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    if (prefix_len == 0) {
+        if (cache->format == DT_KV_INT8)
+            return q_f32 ? launch_split(dt::cache_attn::split_kernel<0, true>, p, dev, st)
+                         : launch_split(dt::cache_attn::split_kernel<0, false>, p, dev, st);
+        return q_f32 ? launch_split(dt::cache_attn::split_kernel<1, true>, p, dev, st)
+                     : launch_split(dt::cache_attn::split_kernel<1, false>, p, dev, st);
+    }
     const dim3 grid((unsigned)(((long long)B * T * heads + 3) / 4)), block(128);
     if (cache->format == DT_KV_INT8)
         return q_f32 ? launch_pdl(dt::cache_attn::row_kernel<0, true>, grid, block, 0, st, p)

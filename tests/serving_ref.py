@@ -31,12 +31,13 @@ def pages_of(gen, pages, B, per_row, device):
 
 
 def keys_of(cache, pages, head, n):
-    """K and V rows 0 .. n - 1 of one head along a list of pages, and which of them exist."""
+    """K and V rows 0 .. n - 1 of one head along a list of pages, V's scales and |codes|, and which rows exist."""
     ok = (pages >= 0) & (pages < cache.num_pages)
     at = torch.where(ok, pages, torch.zeros_like(pages)).long()
     k = values(cache.k.view(torch.int8)[at, head].view(cache.k.dtype), cache.k_scale[at, head]).reshape(-1, D)[:n]
     v = values(cache.v.view(torch.int8)[at, head].view(cache.v.dtype), cache.v_scale[at, head]).reshape(-1, D)[:n]
-    return k, v, ok.repeat_interleave(cache.page_size)[:n]
+    codes = cache.v.view(torch.int8)[at, head].view(cache.v.dtype).float().double().reshape(-1, D)[:n].abs()
+    return k, v, cache.v_scale[at, head].double().reshape(-1)[:n], codes, ok.repeat_interleave(cache.page_size)[:n]
 
 
 def attention(q, cache, table, seq_lens, scale, q_lens=None, prefix_pages=None, prefix_len=0, p_half=0.0):
@@ -66,15 +67,13 @@ def attention(q, cache, table, seq_lens, scale, q_lens=None, prefix_pages=None, 
                 parts.append(keys_of(cache, table[b], h // group, own))
             for t in range(n_q):
                 last = 0 if table is None else max(0, min(int(seq_lens[b]) - n_q + t + 1, cap))
-                k, v = [], []
-                for i, (pk, pv, ok) in enumerate(parts):
+                seen = []
+                for i, part in enumerate(parts):
                     n = prefix_len if prefix_len and i == 0 else last
-                    keep = ok[:n]
-                    k.append(pk[:n][keep])
-                    v.append(pv[:n][keep])
-                if not k or sum(len(x) for x in k) == 0:
+                    seen.append([x[:n][part[-1][:n]] for x in part[:-1]])
+                if sum(len(x[0]) for x in seen) == 0:
                     continue
-                k, v = torch.cat(k), torch.cat(v)
+                k, v, vs, codes = (torch.cat(x) for x in zip(*seen))
                 s = k @ qd[b, t, h] * scale
                 d = float((132 * 2 * EPS32 * (k.abs() @ qd[b, t, h].abs()) * abs(scale)).max())
                 m[b, t, h] = s.max()
@@ -84,6 +83,9 @@ def attention(q, cache, table, seq_lens, scale, q_lens=None, prefix_pages=None, 
                 o[b, t, h] = p @ v
                 rel = 2 * d + 8 * EPS32 * (1 + float((p * (s.max() - s)).sum())) + 2 * len(k) * EPS32 + p_half
                 o_tol[b, t, h] = HALF[q.dtype] * o[b, t, h].abs() + 2 * rel * (p @ v.abs())
+                # The second product takes p * v_scale as two fp16 numbers, scaled so that a row's largest is at
+                # least 2^8: each is off by at most half of fp16's smallest step, 2^-25, so by 2^-33 of the largest.
+                o_tol[b, t, h] += 2.0 ** -33 * float((p * vs).max()) * codes.sum(0)
                 m_tol[b, t, h] = d + EPS32 * abs(float(s.max()))
                 l_tol[b, t, h] = (2 * d + 8 * EPS32 * (1 + float((p * (s.max() - s)).sum())) + 2 * len(k) * EPS32) * w.sum()
     return o, m, l, o_tol, m_tol, l_tol

@@ -221,7 +221,7 @@ def attention_case(dt, cuda, seed, fmt, dtype, B, T, heads, group, page, lens, p
 
 
 def poison(c, table, seq_lens, prefix_pages=None, prefix_len=0):
-    """NaN scales wherever no key of any sequence lies: what is masked must not reach an output."""
+    """NaN scales and codes wherever no key of any sequence lies: what is masked must not reach an output."""
     seen = torch.zeros(c.k_scale.shape, dtype=torch.bool, device=c.device)
     spans = [(table[b], min(int(seq_lens[b]), table.shape[1] * c.page_size)) for b in range(len(seq_lens))] if table is not None else []
     if prefix_len:
@@ -233,6 +233,8 @@ def poison(c, table, seq_lens, prefix_pages=None, prefix_len=0):
                 seen[p, :, j % c.page_size] = True
     for t in (c.k_scale, c.v_scale):
         t[~seen] = math.nan
+    for t in (c.k, c.v):
+        t.view(torch.int8)[~seen] = 0x7f  # e4m3's NaN
 
 
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
