@@ -150,7 +150,8 @@ SIGNATURES = {
     "dt_attn_forward_sharded_host": (_I, [_P, _P, _I, _I, _P, _I, _P]),
     "dt_kv_cache_append": (_I, [_P, _P, _LL, _LL, _P, _LL, _LL, _I, _P, _LL, _I, _P, _P, _I, _I, _P]),
     "dt_kv_cache_read": (_I, [_P, _P, _P, _I, _P, _LL, _I, _P, _P, _I, _I, _P]),
-    "dt_cache_attn_fwd": (_I, [_P, _P, _LL, _LL, _I, _P, _P, _P, _P, _LL, _I, _P, _P, _I, _I, _I, _F, _P]),
+    "dt_cache_attn_workspace_bytes": (_SZ, [_I] * 7),
+    "dt_cache_attn_fwd": (_I, [_P, _P, _LL, _LL, _I, _P, _P, _P, _P, _LL, _I, _P, _P, _I, _I, _I, _F, _P, _SZ, _P]),
     "dt_prefix_attn_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I]),
     "dt_prefix_attn_fwd": (_I, [_P, _P, _LL, _LL, _I, _P, _P, _P, _P, _I, _P, _LL, _I, _P, _P, _I, _I, _I, _F, _P, _SZ,
                                 _P]),

@@ -115,27 +115,55 @@ int dt_kv_cache_read(const dt_kv_cache* cache, void* k, void* v, int dst_f32, co
 
 namespace {
 
-// Launches the split kernel with `split` CTAs (a cluster) per work item.
-int launch_split(void (*kernel)(dt::cache_attn::Params), dt::cache_attn::Params& p, int dev, cudaStream_t st) {
+constexpr int kPlanSms = 148;  // B200; the plan is made without a device, for the workspace size
+
+// How the split kernel's work is cut: see the rules at plan_split.
+struct SplitPlan {
+    bool wide;       // 16 query rows per CTA
+    long long items; // (sequence, K/V head, rows) that a cluster or a group of CTAs takes
+    int split;       // CTAs per item
+    bool parts;      // joined through the workspace
+};
+
+#ifndef DT_ATTN_FORCE_SPLIT
+#define DT_ATTN_FORCE_SPLIT 0
+#endif
+SplitPlan plan_split(int B, int T, int heads, int kv_heads, int q_f32, int page_size, int max_pages) {
     namespace ca = dt::cache_attn;
-    const long long items = (long long)p.B * p.c.heads * ((p.T * p.group + ca::kRows - 1) / ca::kRows);
-    const long long tiles = ((long long)p.max_pages << p.c.page_shift) / ca::kTile;
-    const int sms = g_dev[dev].num_sms;
-    int split = 1;
-    while (split < ca::kMaxSplit && items * split < 4 * sms && tiles > (long long)split * ca::kWarps) split *= 2;
-    p.split = split;
-    if (items * split > 0x7fffffffll) return fail(DT_ERR_INVALID_ARGUMENT, "B * kv_heads * query rows is too large");
+    SplitPlan s{};
+    const int rows = T * (heads / kv_heads);
+    s.wide = !q_f32 && rows > 8;
+    s.items = (long long)B * kv_heads * ((rows + (s.wide ? 15 : 7)) / (s.wide ? 16 : 8));
+    const long long tiles = ((long long)max_pages * page_size + ca::kTile - 1) / ca::kTile;
+    const long long slots = 3 * kPlanSms;
+    s.split = 1;
+    while (s.split < ca::kMaxCluster && s.items * s.split * 2 <= slots && tiles > (long long)s.split * ca::kWarps) s.split *= 2;
+    if (s.split == ca::kMaxCluster && s.items * s.split * 2 <= slots && tiles > 4ll * s.split * ca::kWarps) {
+        s.parts = true;
+        s.split = (int)std::min(slots / s.items, tiles / (2 * ca::kWarps));
+    }
+    if (DT_ATTN_FORCE_SPLIT) s.split = DT_ATTN_FORCE_SPLIT, s.parts = false;
+    return s;
+}
+
+size_t parts_bytes(long long parts, int B, int T, int heads) {
+    const size_t rows = (size_t)B * T * heads;
+    return align256(parts * rows * 16) + align256(parts * rows * dt::cache_attn::kD * 4);
+}
+
+int launch_split(void (*kernel)(dt::cache_attn::Params), const dt::cache_attn::Params& p, long long items,
+                 cudaStream_t st) {
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = DT_PDL;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = (unsigned)split;
+    attr[1].val.clusterDim.x = p.part_o ? 1u : (unsigned)p.split;
     attr[1].val.clusterDim.y = 1;
     attr[1].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(items * split));
-    cfg.blockDim = dim3(ca::kThreads);
-    cfg.dynamicSmemBytes = sizeof(ca::Smem);
+    cfg.gridDim = dim3((unsigned)(items * p.split));
+    cfg.blockDim = dim3(dt::cache_attn::kThreads);
+    cfg.dynamicSmemBytes = sizeof(dt::cache_attn::Smem);
     cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
@@ -143,20 +171,37 @@ int launch_split(void (*kernel)(dt::cache_attn::Params), dt::cache_attn::Params&
     return DT_OK;
 }
 
+int launch_join(const dt::cache_attn::Params& p, int q_f32, cudaStream_t st) {
+    const dim3 grid((unsigned)(((long long)p.B * p.T * p.heads + 3) / 4)), block(128);
+    return q_f32 ? launch_pdl(dt::cache_attn::join_kernel<true>, grid, block, 0, st, p)
+                 : launch_pdl(dt::cache_attn::join_kernel<false>, grid, block, 0, st, p);
+}
+
+template <int kFmt>
+void (*split_kernel_of(bool f32, bool wide))(dt::cache_attn::Params) {
+    namespace ca = dt::cache_attn;
+    return f32 ? ca::split_kernel<kFmt, true, false> : wide ? ca::split_kernel<kFmt, false, true> : ca::split_kernel<kFmt, false, false>;
+}
+
 // Per-device attributes of the kernels below (called with g_mu held, from ensure_attrs).
 int serving_attrs() {
-    using dt::cache_attn::split_kernel;
-    for (auto* k : {split_kernel<0, false>, split_kernel<0, true>, split_kernel<1, false>, split_kernel<1, true>}) {
+    for (int i = 0; i < 6; ++i) {
+        auto* k = i & 1 ? split_kernel_of<1>(i >= 4, i >= 2) : split_kernel_of<0>(i >= 4, i >= 2);
         DT_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(dt::cache_attn::Smem)));
-        DT_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     }
     return DT_OK;
+}
+
+void set_parts(dt::cache_attn::Params& p, int parts, void* workspace) {
+    p.n_parts = parts;
+    p.part_s = static_cast<float4*>(workspace);
+    p.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + align256((size_t)parts * p.B * p.T * p.heads * 16));
 }
 
 int cache_attn(const dt_kv_cache* cache, const void* q, long long q_batch_stride, long long q_token_stride, int q_f32,
                void* o, float* m, float* l, const int* prefix_pages, int prefix_len, const int* page_table,
                long long page_table_stride, int max_pages, const int* seq_lens, const int* q_lens, int B, int T,
-               int heads, float scale, void* stream) {
+               int heads, float scale, void* workspace, size_t workspace_bytes, void* stream) {
     dt::cache_attn::Params p{};
     DT_TRY(check_cache(cache, &p.c));
     if (B < 0 || T < 0 || heads < 0) return fail(DT_ERR_INVALID_ARGUMENT, "B, T and heads must be >= 0");
@@ -188,15 +233,23 @@ int cache_attn(const dt_kv_cache* cache, const void* q, long long q_batch_stride
     p.heads = heads;
     p.group = heads / cache->kv_heads;
     p.scale = scale;
+    const size_t need = prefix_len > 0 ? dt_prefix_attn_workspace_bytes(B, T, heads, cache->kv_heads, prefix_len)
+                                       : dt_cache_attn_workspace_bytes(B, T, heads, cache->kv_heads, q_f32,
+                                                                       cache->page_size, max_pages);
+    if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+        return fail(DT_ERR_INVALID_ARGUMENT, "workspace must be >= %zu bytes and 16-byte aligned", need);
     int dev;
     DT_TRY(prepare_device(&dev));
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     if (prefix_len == 0) {
-        if (cache->format == DT_KV_INT8)
-            return q_f32 ? launch_split(dt::cache_attn::split_kernel<0, true>, p, dev, st)
-                         : launch_split(dt::cache_attn::split_kernel<0, false>, p, dev, st);
-        return q_f32 ? launch_split(dt::cache_attn::split_kernel<1, true>, p, dev, st)
-                     : launch_split(dt::cache_attn::split_kernel<1, false>, p, dev, st);
+        const SplitPlan plan = plan_split(B, T, heads, cache->kv_heads, q_f32, cache->page_size, max_pages);
+        if (plan.items * plan.split > 0x7fffffffll)
+            return fail(DT_ERR_INVALID_ARGUMENT, "B * kv_heads * query rows is too large");
+        p.split = plan.split;
+        if (plan.parts) set_parts(p, plan.split, workspace);
+        DT_TRY(launch_split(cache->format == DT_KV_INT8 ? split_kernel_of<0>(q_f32, plan.wide) : split_kernel_of<1>(q_f32, plan.wide),
+                            p, plan.items, st));
+        return plan.parts ? launch_join(p, q_f32, st) : DT_OK;
     }
     const dim3 grid((unsigned)(((long long)B * T * heads + 3) / 4)), block(128);
     if (cache->format == DT_KV_INT8)
@@ -213,10 +266,18 @@ extern "C" {
 int dt_cache_attn_fwd(const dt_kv_cache* cache, const void* q, long long q_batch_stride, long long q_token_stride,
                       int q_f32, void* o, float* softmax_m, float* softmax_l, const int* page_table,
                       long long page_table_stride, int max_pages, const int* seq_lens, const int* q_lens, int B, int T,
-                      int heads, float scale, void* stream) {
+                      int heads, float scale, void* workspace, size_t workspace_bytes, void* stream) {
     t_last_error.clear();
     return cache_attn(cache, q, q_batch_stride, q_token_stride, q_f32, o, softmax_m, softmax_l, nullptr, 0, page_table,
-                      page_table_stride, max_pages, seq_lens, q_lens, B, T, heads, scale, stream);
+                      page_table_stride, max_pages, seq_lens, q_lens, B, T, heads, scale, workspace, workspace_bytes,
+                      stream);
+}
+
+size_t dt_cache_attn_workspace_bytes(int B, int T, int heads, int kv_heads, int q_f32, int page_size, int max_pages) {
+    if (B <= 0 || T <= 0 || kv_heads <= 0 || heads < kv_heads || page_size <= 0 || max_pages <= 0) return 0;
+    if ((long long)B * T * heads > 0x7fffffffll) return 0;
+    const SplitPlan plan = plan_split(B, T, heads, kv_heads, q_f32, page_size, max_pages);
+    return plan.parts ? parts_bytes(plan.split, B, T, heads) : 0;
 }
 
 size_t dt_prefix_attn_workspace_bytes(int B, int T, int heads, int kv_heads, int prefix_len) {
@@ -232,7 +293,7 @@ int dt_prefix_attn_fwd(const dt_kv_cache* cache, const void* q, long long q_batc
     t_last_error.clear();
     return cache_attn(cache, q, q_batch_stride, q_token_stride, q_f32, o, softmax_m, softmax_l, prefix_pages,
                       prefix_len, page_table, page_table_stride, max_pages, seq_lens, q_lens, B, T, heads, scale,
-                      stream);
+                      workspace, workspace_bytes, stream);
 }
 
 int dt_token_log_probs(const void* logits, int logits_f32, long long ld, int N, int V, const void* targets,

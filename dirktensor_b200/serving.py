@@ -172,11 +172,14 @@ def cache_attention_forward(q, cache: KVCache, page_table, seq_lens, scale: floa
     table, stride, n = _table(page_table, cache.device, B)
     lens = _ints("seq_lens", seq_lens, cache.device, B)
     o, m, l = _outputs(q, out, return_stats)
+    f32, L = int(q.dtype == torch.float32), lib()
+    nbytes = L.dt_cache_attn_workspace_bytes(B, T, H, cache.kv_heads, f32, cache.page_size, n)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=cache.device) if nbytes else None
     with _on(cache.device):
-        check(lib().dt_cache_attn_fwd(cache._ref, q.data_ptr(), s[0], s[1], int(q.dtype == torch.float32), o.data_ptr(),
-                                      m.data_ptr() if return_stats else None, l.data_ptr() if return_stats else None,
-                                      table, stride, n, lens, _ints("q_lens", q_lens, cache.device, B), B, T, H,
-                                      float(scale), _stream(cache.device)))
+        check(L.dt_cache_attn_fwd(cache._ref, q.data_ptr(), s[0], s[1], f32, o.data_ptr(),
+                                  m.data_ptr() if return_stats else None, l.data_ptr() if return_stats else None,
+                                  table, stride, n, lens, _ints("q_lens", q_lens, cache.device, B), B, T, H,
+                                  float(scale), ws.data_ptr() if nbytes else None, nbytes, _stream(cache.device)))
     return FlashAttentionResult(o, m, l) if return_stats else o
 
 

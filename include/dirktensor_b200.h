@@ -424,11 +424,14 @@ int dt_kv_cache_read(const dt_kv_cache* cache, void* k, void* v, int dst_f32, co
  * t >= q_lens[b] and rows that see no key are written as zeros (m = l = 0).
  * Lengths past the page table are cut to it; keys on a page whose id is not in
  * 0..num_pages-1 are not seen.  Codes are exact in the products, which are
- * summed in fp32.  Asynchronous on `stream`. */
+ * summed in fp32.  workspace: at least dt_cache_attn_workspace_bytes (which
+ * may be 0: then NULL), 16-byte aligned; calls that may overlap on the GPU
+ * need one each.  Asynchronous on `stream`. */
+size_t dt_cache_attn_workspace_bytes(int B, int T, int heads, int kv_heads, int q_f32, int page_size, int max_pages);
 int dt_cache_attn_fwd(const dt_kv_cache* cache, const void* q, long long q_batch_stride, long long q_token_stride,
                       int q_f32, void* o, float* softmax_m, float* softmax_l, const int* page_table,
                       long long page_table_stride, int max_pages, const int* seq_lens, const int* q_lens, int B, int T,
-                      int heads, float scale, void* stream);
+                      int heads, float scale, void* workspace, size_t workspace_bytes, void* stream);
 /* The same for a batch whose sequences share their first prefix_len tokens:
  * every query that is not padding sees all keys of the prefix (prefix_pages:
  * device int[ceil(prefix_len / page_size)]) and then its own sequence's keys

@@ -47,10 +47,12 @@ def attention(q, cache, table, seq_lens, scale, q_lens=None, prefix_pages=None, 
     d = (128 + 4) * 2 * EPS32 * sum |q k| (twice, since the tensor cores may cut instead of round).
     A weight is then off by a factor of about 1 +- (2 d + 8 EPS32 (1 + |s - m|)), the sums of n
     weights by n * 2 * EPS32 more; p_half is half a step of the type that the weights are rounded to
-    for the second product.
+    for the second product (fp16, 2^-11, in any case where more than 8 bf16 queries share a K/V head).
     """
     B, T, H, _ = q.shape
     group = H // cache.kv_heads
+    if q.dtype == torch.bfloat16 and T * group > 8:
+        p_half = max(p_half, 2.0 ** -11)
     qd = q.double()
     o = torch.zeros((B, T, H, D), dtype=torch.float64, device=q.device)
     m, l = torch.zeros((B, T, H), dtype=torch.float64, device=q.device), torch.zeros((B, T, H), dtype=torch.float64, device=q.device)

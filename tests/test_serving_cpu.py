@@ -31,7 +31,7 @@ def test_cache_descriptor_is_checked(bad, word):
     L = _lib.lib()
     calls = [lambda c: append(c),
              lambda c: L.dt_kv_cache_read(c, FAKE, FAKE, 0, FAKE, 4, 4, None, None, 1, 1, None),
-             lambda c: L.dt_cache_attn_fwd(c, FAKE, 512, 512, 0, FAKE, None, None, FAKE, 4, 4, FAKE, None, 1, 1, 4, 0.1, None),
+             lambda c: L.dt_cache_attn_fwd(c, FAKE, 512, 512, 0, FAKE, None, None, FAKE, 4, 4, FAKE, None, 1, 1, 4, 0.1, FAKE, 1 << 30, None),
              lambda c: L.dt_prefix_attn_fwd(c, FAKE, 512, 512, 0, FAKE, None, None, FAKE, 64, FAKE, 4, 4, FAKE, None, 1,
                                             1, 4, 0.1, FAKE, 1 << 30, None)]
     for call in calls:
@@ -58,7 +58,7 @@ def test_attention_refusals():
     L = _lib.lib()
 
     def attn(c=None, q=FAKE, qb=512, o=FAKE, table=FAKE, n=4, lens=FAKE, B=1, T=1, H=4):
-        return L.dt_cache_attn_fwd(c or cache(), q, qb, 512, 0, o, None, None, table, 4, n, lens, None, B, T, H, 0.1, None)
+        return L.dt_cache_attn_fwd(c or cache(), q, qb, 512, 0, o, None, None, table, 4, n, lens, None, B, T, H, 0.1, FAKE, 1 << 30, None)
 
     assert attn(H=6) == 1 and b"multiple of kv_heads" in L.dt_last_error()
     assert attn(q=None) == 1 and attn(q=FAKE + 8) == 1 and attn(qb=510) == 1
