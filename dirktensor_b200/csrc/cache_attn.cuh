@@ -32,13 +32,17 @@ struct Params {
     int prefix_len;
     int B, T, heads, group;      // heads = kv heads * group
     float scale;
-    int split;                   // CTAs per work item: a cluster, or, with `parts`, on their own
-    // Partial results in the workspace (null: none), one per query row and CTA of its item:
-    // o relative to 2^m, and (m, l, largest score), for the join kernel.
-    float* part_o;               // [n_parts][B * T * heads][128]
-    float4* part_s;              // [n_parts][B * T * heads]
-    int n_parts;                 // of them, `split` are this kernel's, from first_part on
-    int first_part;
+    int split;                   // CTAs of a cluster per work item (split_kernel)
+    int by_length;               // split_kernel takes the longest sequences first
+    // Workspace of stream_kernel and join_kernel: partial sums of the CTAs and, of the prefix
+    // kernel, of the shared keys.  Sums are relative to 2^m; statistics are (m, l, largest score, -).
+    int shares;                  // CTAs of stream_kernel (0: not launched, no keys but the prefix's)
+    int* starts;                 // [B + 1] first tile of each sequence, were each of one item
+    float* part_o;               // [shares + items][rows of an item][128]
+    float4* part_s;              // [shares + items][rows of an item]
+    int n_shared;                // parts of the prefix
+    float* shared_o;             // [n_shared][B * T * heads][128]
+    float4* shared_s;            // [n_shared][B * T * heads]
 };
 
 // One warp per query row, lane l holding dims 4l .. 4l + 3, keys one after another.
@@ -107,31 +111,45 @@ __global__ void __launch_bounds__(128) row_kernel(const Params p) {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kSub = 16;      // keys of an MMA step: the smallest page, so these share a page
-constexpr int kTile = 32;     // keys per warp and step
-constexpr int kStages = 2;    // tiles of a warp: one in use, one in flight
+constexpr int kSub = 16;       // keys of an MMA step: the smallest page, so these share a page
+constexpr int kTile = 32;      // keys per warp and step
+constexpr int kStages = 3;     // pieces (K or V of a tile) of a warp: one in use, two in flight
 constexpr int kMaxCluster = 8;
-constexpr float kGrow = 8.f;  // the running maximum moves when a score passes it by this much (log2)
+constexpr float kGrow = 8.f;   // the running maximum moves when a score passes it by this much (log2)
 constexpr float kLog2e = 1.4426950408889634f;
 
-// One tile of one warp.  Every lane copies the 16-byte pieces that it will read itself, at
-// [piece][lane], so that reads have no bank conflicts and K and V need no exchange; the scales
-// are read by all lanes.
+// K or V of one tile of one warp.  Every lane copies the 16-byte pieces that it will read itself,
+// at [piece][lane], so that reads have no bank conflicts and need no exchange; the scales are read
+// by all lanes.
 struct Stage {
-    uint4 k[8][32];
-    uint4 v[8][32];
-    float4 scales[16];  // K's of the tile's keys, four by four, then V's
+    uint4 d[8][32];
+    float scale[kTile];
 };
 
 struct Smem {
-    Stage ring[kWarps][kStages];  // afterwards each warp's rows, [rows][kD] fp32, at its first stage
-    float m[kWarps][16];          // running maxima that the warps' sums refer to (log2 units)
+    Stage ring[kWarps][kStages];    // afterwards each warp's rows, [rows][kD] fp32, from its start
+    float m[kWarps][16];            // running maxima that the warps' sums refer to (log2 units)
     float l[kWarps][16];
-    float mx[kWarps][16];         // largest score
-    float om[16], ol[16], omx[16];  // the CTA's own, for the cluster; its rows are at ring[0][1]
+    float mx[kWarps][16];           // largest score
+    float om[16], ol[16], omx[16];  // the CTA's own, for the cluster
+    // and its rows, behind the warps': eight at the end of each of the first two rings
+    __device__ __forceinline__ float* joined(int row) {
+        return reinterpret_cast<float*>(&ring[row >> 3][0]) + 16 * kD + (row & 7) * kD;
+    }
 };
-static_assert(sizeof(Stage) >= 16 * kD * 4, "16 rows fit into a stage");
-static_assert(3 * (sizeof(Smem) + 1024) <= 227 * 1024, "three CTAs per SM");
+static_assert(kStages * sizeof(Stage) >= 24 * kD * 4, "16 rows of a warp and 8 of the CTA fit into a ring");
+static_assert(4 * (sizeof(Smem) + 1024) <= 227 * 1024, "four CTAs per SM");
+
+// Query rows that a warp takes.  An MMA has eight columns for them; each lane has the scores of
+// columns 2t and 2t + 1, so up to four queries sit in the even columns, at half the softmax work.
+enum : int { kFew = 0, kEight = 1, kWide = 2 };  // 4, 8, or 16 in two sets of columns
+constexpr int rows_of(int form) { return form == kFew ? 4 : form == kEight ? 8 : 16; }
+
+#ifndef DT_ATTN_WIDE_CTAS
+#define DT_ATTN_WIDE_CTAS 3
+#endif
+// CTAs per SM: four where 128 registers a thread suffice.
+constexpr int ctas_per_sm(bool f32, int form) { return form == kWide ? DT_ATTN_WIDE_CTAS : f32 ? 3 : 4; }
 
 __device__ __forceinline__ void cp16(void* dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
@@ -190,13 +208,23 @@ __device__ __forceinline__ void split_pair(float a, float b, uint32_t& hi, uint3
     lo = half_pair(a - f.x, b - f.y);
 }
 
-__device__ __forceinline__ float quad_max(float x) {
-    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-    return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+// The transpose of an 8 x 8 matrix of 16-bit values, row g's columns 2t, 2t + 1 in lane 4g + t.
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
-__device__ __forceinline__ float quad_sum(float x) {
-    x += __shfl_xor_sync(0xffffffffu, x, 1);
-    return x + __shfl_xor_sync(0xffffffffu, x, 2);
+
+// Over the eight lanes of one t.
+__device__ __forceinline__ float column_max(float x) {
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+    return x;
+}
+__device__ __forceinline__ float column_sum(float x) {
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    return x;
 }
 
 // 2^e for e in [-126, 127]
@@ -234,133 +262,151 @@ __device__ __forceinline__ void store_row(const Params& p, long long row, int la
     }
 }
 
-// Split attention over the cache.  `split` CTAs take 8 or 16 query rows of one sequence and K/V
-// head; their warps take the sequence's 32-key tiles in turn, keep their own running softmax, and
-// are joined in shared memory, then over the CTAs' cluster or, where more CTAs than a cluster
-// holds share few rows, through the workspace by join_kernel.
+// A warp's attention of 8 or 16 query rows of one sequence and K/V head over 32-key tiles
+// tile0, tile0 + step, ... below tile1, with its own running softmax.
 //
-// Both products run on the tensor cores as m16n8k16 with the queries as the 16 rows.  8 rows:
-// MMA rows 0-7 are fp16(q), rows 8-15 the rest q - fp16(q), so that fp32 queries lose nothing (bf16
-// queries fit the first part; each row is scaled by a power of two into fp16's range first), and
-// the weights p * v_scale are split the same way for the second product.  16 rows (kWide: bf16
-// queries, more than 8 of them per K/V head, whose keys would be read twice otherwise): the weights
-// are rounded to fp16 once, at 2^-11 well below the bf16 result's own 2^-8.  Codes are exact in fp16.
+// Both products run on the tensor cores as m16n8k16 with the queries as the 8 columns:
+//   S^T (16 keys x 8 queries) = K (16 keys x 16 dims) Q^T,  O^T (16 dims x 8 queries) = V^T (16 dims x 16 keys) P^T
+// so that no row of an MMA is idle however few queries there are.  Codes are exact in fp16.  Queries
+// are scaled row by row by a power of two into fp16's range, where bf16 values are exact; fp32 ones
+// go in as fp16(q) and q - fp16(q), and so do their weights p * v_scale.  The weights of bf16 queries
+// are rounded to fp16 once, at 2^-11 well below the result's own 2^-8.  More than 8 bf16 queries of
+// a K/V head take two sets of columns (kWide), so that the keys are read and converted once.
 //
-// The k and n indices of an MMA may be permuted freely if both operands agree, which saves every
-// exchange.  Lane 4g + t holds, of each 16-key half of a tile,
-//   K: keys 4 (g / 2) + 2 i + g % 2 (i = 0, 1: column g of 8-key block i), dims 16 (4 hf + t) ..+15;
-//   S: query g, keys 4t .. 4t + 3 (columns 2t, 2t + 1 of block 0, then of block 1);
-//   V: keys 4t .. 4t + 3, dims 16 g ..+15.
-template <int kFmt, bool kF32, bool kWide>
-__global__ void __launch_bounds__(kThreads, 3) split_kernel(const Params p) {
-    static_assert(!(kF32 && kWide), "fp32 queries take both halves of the MMA rows");
-    pdl_enter();
-    constexpr int kSets = kWide ? 2 : 1;  // query rows per lane: g, and g + 8
-    constexpr int kRows = 8 * kSets;
-    extern __shared__ __align__(16) uint8_t smem_raw[];
-    Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int g = lane >> 2, t = lane & 3;
-    const int rank = (int)(blockIdx.x % (unsigned)p.split);
-    const int item = (int)(blockIdx.x / (unsigned)p.split);
-    const int per_head = (p.T * p.group + kRows - 1) / kRows;
-    const int hk = item / per_head % p.c.heads;
-    const int b = item / per_head / p.c.heads;
-    const int row0 = item % per_head * kRows;
-
-    // this lane's query rows, and how many keys they and the CTA's rows see
-    const int q_len = p.q_lens ? min(p.q_lens[b], p.T) : p.T;
-    const long long cap = (long long)p.max_pages << p.c.page_shift;
-    const long long base = p.max_pages > 0 ? (long long)p.seq_lens[b] - q_len + 1 : 0;  // (lengths may be null then)
-    int lim[kSets], keys = 0;
+// The k indices of an MMA may be permuted freely if both operands agree, and its rows if the result is
+// read accordingly, which saves every exchange but the transpose of P.  Lane 4g + t holds, of
+// each 16-key half of a tile,
+//   K: keys g and g + 8, dims 16 (4 hf + t) ..+15;      S, P: keys g and g + 8, queries 2t and 2t + 1;
+//   V: keys 2t, 2t + 1, 2t + 8, 2t + 9, dims 16 g ..+15;  O: dims 16 g ..+15, queries 2t and 2t + 1.
+template <int kForm>
+struct State {
+    static constexpr int kSets = kForm == kWide ? 2 : 1, kCols = kForm == kFew ? 1 : 2;
+    float acc[kSets][8][4];  // of step j: dims 16g + 2j (0, 1) and 16g + 2j + 1 (2, 3), queries 2t (0, 2) and 2t + 1 (1, 3)
+    float m[kSets][kCols];       // running maxima that the sums refer to (log2 units; -inf: no key seen)
+    float l[kSets][kCols];       // this lane's share of the sums of p
+    float mx[kSets][kCols];      // this lane's largest scores
+    float f[kSets][kCols];       // acc holds sums of p * v_scale * f: f keeps them in fp16's range
+    // dim 16g + d of query 2t + c
+    __device__ __forceinline__ float sum(int z, int c, int d) const { return acc[z][d >> 1][2 * (d & 1) + c]; }
+    __device__ __forceinline__ void rescale(int z, int c, float a) {
 #pragma unroll
-    for (int z = 0; z < kSets; ++z) {
-        const int r = row0 + g + 8 * z;
-        const int tq = r / p.group;
-        lim[z] = tq < q_len && p.max_pages > 0 ? (int)max(0ll, min(base + tq, cap)) : 0;
-        if (r >= p.T * p.group) lim[z] = 0x7fffffff;  // (an MMA row that no query fills: nothing to mask, and never stored)
-        else keys = max(keys, lim[z]);
+        for (int j = 0; j < 8; ++j) acc[z][j][c] *= a, acc[z][j][2 + c] *= a;
     }
-#pragma unroll
-    for (int o = 4; o < 32; o <<= 1) keys = max(keys, __shfl_xor_sync(0xffffffffu, keys, o));
-    const int tiles = (keys + kTile - 1) / kTile;
-    const int step = p.split * kWarps;
-    const int first = rank * kWarps + warp;
+};
 
-    // Pages of a tile's two halves (-1 where there is none), looked up a step ahead.
-    const int* table = p.table + (long long)b * p.table_stride;
-    const int shift = p.c.page_shift;
-    auto page_at = [&](int tile, int half) {
-        const int key = tile * kTile + half * kSub;
-        return tile < tiles && key < keys ? __ldg(table + (key >> shift)) : -1;
-    };
-    Stage* ring = sm.ring[warp];
-    const int in_page = (1 << shift) - 1;
-    const uint8_t* k_lane = p.c.k + (4 * (g >> 1) + (g & 1)) * kD + t * 16;
-    const uint8_t* v_lane = p.c.v + (4 * t) * kD + g * 16;
-    // (lanes 0-7 copy K's scales, 8-15 V's: four keys each, the first half of the tile first)
-    const float* s_lane = (lane < 8 ? p.c.ks : p.c.vs) + 4 * (lane & 3);
-    // Starts the copies of a tile's halves whose pages exist; returns which.
-    auto issue = [&](int tile, int page0, int page1, int slot) {
-        Stage& st = ring[slot];
-        uint32_t ok = 0;
-#pragma unroll
-        for (int a = 0; a < 2; ++a) {
-            const int page = a ? page1 : page0;
-            if (page >= 0 && page < p.c.pages) {
-                ok |= 1u << a;
-                const int off = (tile * kTile + a * kSub) & in_page;
-                const long long row = (((long long)page * p.c.heads + hk) << shift) + off;
-                const uint8_t* k = k_lane + row * kD;
-                const uint8_t* v = v_lane + row * kD;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) cp16(&st.k[4 * a + i][lane], k + (i >> 1) * 2 * kD + (i & 1) * 64);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) cp16(&st.v[4 * a + i][lane], v + i * kD);
-                if (lane < 16 && ((lane >> 2) & 1) == a) cp16(&st.scales[lane], s_lane + row);
-            }
-        }
-        cp_commit();
-        return ok;
-    };
+template <int kFmt, bool kF32, int kForm>
+__device__ __forceinline__ void attend(const Params& p, Stage* ring, int b, int hk, int row0, int tile0, int tile1, int step,
+                                       State<kForm>& st) {
+    static_assert(!(kF32 && kForm == kWide), "fp32 queries have no wide form: twice the registers");
+    constexpr int kSets = kForm == kWide ? 2 : 1, kCols = kForm == kFew ? 1 : 2;
+    constexpr int kParts = kF32 ? 2 : 1;
+    const int lane = threadIdx.x & 31;
+    const int g = lane >> 2, t = lane & 3;
 
-    int pages[2] = {page_at(first, 0), page_at(first, 1)};
-    int ahead[2] = {page_at(first + step, 0), page_at(first + step, 1)};
-    uint32_t have = issue(first, pages[0], pages[1], 0);
-
-    // the query rows, scaled by a power of two to at most 2^14, as fp16 (and what that leaves)
-    uint32_t qa[2][16];     // MMA rows g and g + 8
-    float factor[kSets];    // back from the scaled products to scores in log2 units
+    // the query of column g of each set, asked for first, since nothing else is needed to
+    uint4 raw[kSets][kF32 ? 8 : 4];
 #pragma unroll
     for (int z = 0; z < kSets; ++z) {
-        const int r = row0 + g + 8 * z;
-        const bool in = r < p.T * p.group;
+        const int r = row0 + (kCols == 1 ? g >> 1 : g) + 8 * z;
+        const bool in = r < p.T * p.group && (kCols == 2 || !(g & 1));
         const int tq = in ? r / p.group : 0;
         const int h = hk * p.group + (in ? r % p.group : 0);
-        const long long at = (long long)b * p.q_batch + (long long)tq * p.q_token + (long long)h * kD;
+        const long long at = (long long)b * p.q_batch + (long long)tq * p.q_token + (long long)h * kD + 16 * t;
+        const uint4* src = kF32 ? reinterpret_cast<const uint4*>(static_cast<const float*>(p.q) + at)
+                                : reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.q) + at);
+        constexpr int kPieces = kF32 ? 4 : 2;  // of 16 dims
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i)
+                raw[z][kPieces * hf + i] = in ? __ldg(src + hf * 4 * kPieces + i) : make_uint4(0, 0, 0, 0);
+    }
+    // Pages of a tile's two halves (-1 past the table), looked up ahead: entries past the
+    // sequence's keys may be anything, and are not followed.  From 32 tokens a page on, one serves both.
+    const long long cap = (long long)p.max_pages << p.c.page_shift;
+    const int* table = p.table + (long long)b * p.table_stride;
+    const int shift = p.c.page_shift;
+    auto page_at = [&](int tile, int (&page)[2]) {
+        const int key = tile * kTile;
+        page[0] = key < cap ? __ldg(table + (key >> shift)) : -1;
+        page[1] = page[0];
+        if (shift < 5) page[1] = key + kSub < cap ? __ldg(table + (key >> shift) + 1) : -1;
+    };
+    int pages[3][2];  // of the next tile, the one after it, and the one after that
+#pragma unroll
+    for (int i = 0; i < 3; ++i) page_at(tile0 + i * step, pages[i]);
+
+    // how many keys this lane's queries 2t and 2t + 1, and all of the warp's, see
+    const int q_len = p.q_lens ? min(p.q_lens[b], p.T) : p.T;
+    const long long base = (long long)p.seq_lens[b] - q_len + 1;
+    int lim[kSets][kCols], keys = 0, least = 0x7fffffff;
+#pragma unroll
+    for (int z = 0; z < kSets; ++z)
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) {
+            const int r = row0 + kCols * t + c + 8 * z;
+            const int tq = r / p.group;
+            lim[z][c] = tq < q_len ? (int)max(0ll, min(base + tq, cap)) : 0;
+            if (r >= p.T * p.group) lim[z][c] = 0x7fffffff;  // (a column that no query fills: nothing to mask, and never stored)
+            else keys = max(keys, lim[z][c]);
+            least = min(least, lim[z][c]);
+        }
+    keys = max(keys, __shfl_xor_sync(0xffffffffu, keys, 1));
+    keys = max(keys, __shfl_xor_sync(0xffffffffu, keys, 2));
+    least = min(least, __shfl_xor_sync(0xffffffffu, least, 1));
+    least = min(least, __shfl_xor_sync(0xffffffffu, least, 2));
+    tile1 = min(tile1, (int)(((long long)keys + kTile - 1) / kTile));
+
+    // Which halves of a tile there are to read.
+    auto halves = [&](int tile, const int (&page)[2]) {
+        uint32_t ok = 0;
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+            if (page[a] >= 0 && page[a] < p.c.pages && tile < tile1 && tile * kTile + a * kSub < keys) ok |= 1u << a;
+        return ok;
+    };
+    const int in_page = (1 << shift) - 1;
+    const uint8_t* k_lane = p.c.k + g * kD + t * 16;
+    const uint8_t* v_lane = p.c.v + 2 * t * kD + g * 16;
+    const float* ks_lane = p.c.ks + 4 * (lane & 3);
+    const float* vs_lane = p.c.vs + 4 * (lane & 3);
+    // Starts the copies of K or V of a tile's halves.  (A cache has fewer than 2^31 rows.)
+    auto issue = [&](bool v, int tile, const int (&page)[2], uint32_t ok, int slot) {
+        Stage& into = ring[slot];
+        if (ok) {
+            uint32_t row0 = ((uint32_t)(page[0] * p.c.heads + hk) << shift) + ((tile * kTile) & in_page);
+            uint32_t row1 = ((uint32_t)(page[1] * p.c.heads + hk) << shift) + ((tile * kTile + kSub) & in_page);
+            if (ok == 1u) row1 = row0;  // (the other half again, and hidden)
+            if (ok == 2u) row0 = row1;
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+                const uint8_t* src = (v ? v_lane : k_lane) + (size_t)(a ? row1 : row0) * kD;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    cp16(&into.d[4 * a + i][lane], src + (i >> 1) * 8 * kD + (i & 1) * (v ? kD : 64));
+            }
+            if (lane < 8) cp16(&into.scale[4 * lane], (v ? vs_lane : ks_lane) + (lane < 4 ? row0 : row1));
+        }
+        cp_commit();
+    };
+    uint32_t have = halves(tile0, pages[0]), next = halves(tile0 + step, pages[1]);
+    issue(false, tile0, pages[0], have, 0);
+    issue(true, tile0, pages[0], have, 1);
+    issue(false, tile0 + step, pages[1], next, 2);
+
+    // the queries, scaled by a power of two to at most 2^14, as fp16 (and what that leaves)
+    uint32_t qb[kSets][kParts][16];
+    float factor[kSets][kCols];  // back from the scaled products to scores in log2 units, of queries 2t, 2t + 1
+#pragma unroll
+    for (int z = 0; z < kSets; ++z) {
         float x[32];
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-            const int d0 = 16 * (4 * hf + t);
-            if (kF32) {
-                const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + at + d0);
+        for (int i = 0; i < (kF32 ? 8 : 4); ++i) {
+            const uint32_t w[4] = {raw[z][i].x, raw[z][i].y, raw[z][i].z, raw[z][i].w};
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float4 y = in ? src[i] : make_float4(0.f, 0.f, 0.f, 0.f);
-                    x[16 * hf + 4 * i] = y.x, x[16 * hf + 4 * i + 1] = y.y, x[16 * hf + 4 * i + 2] = y.z, x[16 * hf + 4 * i + 3] = y.w;
-                }
-            } else {
-                const uint4* src = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.q) + at + d0);
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const uint4 y = in ? src[i] : make_uint4(0, 0, 0, 0);
-                    const uint32_t w[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        x[16 * hf + 8 * i + 2 * e] = __uint_as_float(w[e] << 16);
-                        x[16 * hf + 8 * i + 2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
-                    }
-                }
+            for (int e = 0; e < 4; ++e) {
+                if (kF32) x[4 * i + e] = __uint_as_float(w[e]);
+                else x[8 * (i & 3) + 2 * e] = __uint_as_float(w[e] << 16), x[8 * (i & 3) + 2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
             }
         }
         // largest magnitude as an integer: infinities and NaNs order above every finite value
@@ -372,211 +418,233 @@ __global__ void __launch_bounds__(kThreads, 3) split_kernel(const Params p) {
         const bool finite = top < 0x7f800000u;
         const int e = finite ? max(exponent(__uint_as_float(top)), -100) : 0;
         const float mul = finite ? pow2(13 - e) : 0.f;
-        factor[z] = finite ? pow2(e - 13) * p.scale * kLog2e : __uint_as_float(0x7fffffffu);
+        const float back = finite ? pow2(e - 13) * p.scale * kLog2e : __uint_as_float(0x7fffffffu);
+        factor[z][0] = __shfl_sync(0xffffffffu, back, 8 * t);
+        if (kCols == 2) factor[z][kCols - 1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const float a = finite ? x[2 * i] * mul : 0.f, c = finite ? x[2 * i + 1] * mul : 0.f;
-            if (kF32) split_pair(a, c, qa[0][i], qa[1][i]);
-            else qa[z][i] = half_pair(a, c);
-            if (!kF32 && !kWide) qa[1][i] = 0u;
+            if (kF32) split_pair(a, c, qb[z][0][i], qb[z][kParts - 1][i]);
+            else qb[z][0][i] = half_pair(a, c);
         }
     }
 
-    float acc[16][4];
 #pragma unroll
-    for (int j = 0; j < 16; ++j)
+    for (int z = 0; z < kSets; ++z) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
-    float m[kSets], l[kSets], mx[kSets];
-    float f[kSets];  // acc holds sums of p * v_scale * f: f keeps them in fp16's range
+        for (int j = 0; j < 8; ++j)
 #pragma unroll
-    for (int z = 0; z < kSets; ++z) m[z] = mx[z] = -INFINITY, l[z] = 0.f, f[z] = pow2(100);
-    auto rescale = [&](int z, float a) {
+            for (int e = 0; e < 4; ++e) st.acc[z][j][e] = 0.f;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            acc[j][2 * z] *= a, acc[j][2 * z + 1] *= a;
-            if (!kWide) acc[j][2] *= a, acc[j][3] *= a;
-        }
-    };
+        for (int c = 0; c < kCols; ++c) st.m[z][c] = st.mx[z][c] = -INFINITY, st.l[z][c] = 0.f, st.f[z][c] = pow2(100);
+    }
 
-    uint32_t slot = 0;
-    for (int tile = first; tile < tiles; tile += step) {
+    int slot = 0;
+    for (int tile = tile0; tile < tile1; tile += step) {
         const uint32_t now = have;
-        __syncwarp();  // every lane is done with the other slot's scales
-        have = issue(tile + step, ahead[0], ahead[1], slot ^ 1);
-        ahead[0] = page_at(tile + 2 * step, 0);
-        ahead[1] = page_at(tile + 2 * step, 1);
-        cp_wait<1>();
+        // the pages of three tiles ahead are asked for here and first used in the next step
+        int far[2];
+        page_at(tile + 3 * step, far);
+        cp_wait<kStages - 1>();
         __syncwarp();
-        const Stage& st = ring[slot];
-        slot ^= 1;
 
-        // scores: keys 4t .. 4t + 3 of either half (four chains of products side by side)
-        float s[kSets][8], vv[8];
+        // scores [half][key g, key g + 8][query column 2t, 2t + 1]
+        float s[kSets][2][2][kCols];
         {
-            float d[4][4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) d[i][e] = 0.f;
-#pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-                uint32_t w[4][4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(w[i]) = st.k[2 * i + hf][lane];
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint32_t b0, b1;
-                        pairs_of_word<kFmt>(w[i][e], b0, b1);
-                        const int q = 8 * hf + 2 * e;
-                        mma_f16(d[i], qa[0][q], qa[1][q], qa[0][q + 1], qa[1][q + 1], b0, b1);
-                    }
-            }
+            const Stage& k = ring[slot];
 #pragma unroll
             for (int a = 0; a < 2; ++a) {
-                const float4 ks = st.scales[4 * a + t], vs = st.scales[8 + 4 * a + t];
-                const float kk[4] = {ks.x, ks.y, ks.z, ks.w};
-                vv[4 * a] = vs.x, vv[4 * a + 1] = vs.y, vv[4 * a + 2] = vs.z, vv[4 * a + 3] = vs.w;
+                float d[kSets][2][4];  // (two chains of products each)
 #pragma unroll
                 for (int z = 0; z < kSets; ++z)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float* dd = d[2 * a + (i >> 1)];
-                        const float y = kWide ? dd[2 * z + (i & 1)] : (kF32 ? dd[i & 1] + dd[2 + (i & 1)] : dd[i & 1]);
-                        s[z][4 * a + i] = y * (kk[i] * factor[z]);
+                    for (int e = 0; e < 4; ++e) d[z][0][e] = d[z][1][e] = 0.f;
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) {
+                    uint32_t w0[4], w1[4];  // rows g and g + 8
+                    *reinterpret_cast<uint4*>(w0) = k.d[4 * a + hf][lane];
+                    *reinterpret_cast<uint4*>(w1) = k.d[4 * a + 2 + hf][lane];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        uint32_t a0, a1, a2, a3;
+                        pairs_of_word<kFmt>(w0[e], a0, a2);
+                        pairs_of_word<kFmt>(w1[e], a1, a3);
+#pragma unroll
+                        for (int z = 0; z < kSets; ++z)
+#pragma unroll
+                            for (int c = 0; c < kParts; ++c)
+                                mma_f16(d[z][e & 1], a0, a1, a2, a3, qb[z][c][8 * hf + 2 * e], qb[z][c][8 * hf + 2 * e + 1]);
+                    }
+                }
+                const float ks0 = k.scale[kSub * a + g], ks1 = k.scale[kSub * a + g + 8];
+#pragma unroll
+                for (int z = 0; z < kSets; ++z)
+#pragma unroll
+                    for (int c = 0; c < kCols; ++c) {
+                        s[z][a][0][c] = (d[z][0][c] + d[z][1][c]) * (ks0 * factor[z][c]);
+                        s[z][a][1][c] = (d[z][0][2 + c] + d[z][1][2 + c]) * (ks1 * factor[z][c]);
                     }
             }
         }
-        const int key0 = tile * kTile + 4 * t;
-        bool whole = now == 3u;
-#pragma unroll
-        for (int z = 0; z < kSets; ++z) whole &= tile * kTile + kTile <= lim[z];
-        whole = __all_sync(0xffffffffu, whole);
+        __syncwarp();  // every lane is done with this piece
+        issue(true, tile + step, pages[1], next, slot);
+        slot = slot == kStages - 1 ? 0 : slot + 1;
+
+        const int key0 = tile * kTile + g;
+        const bool whole = now == 3u && tile * kTile + kTile <= least;
         if (!whole) {  // hidden keys: past a row's last one, or on a page that does not exist
 #pragma unroll
             for (int z = 0; z < kSets; ++z)
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (key0 + (i >> 2) * kSub + (i & 3) >= lim[z] || !((now >> (i >> 2)) & 1u)) s[z][i] = -INFINITY;
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int c = 0; c < kCols; ++c)
+                        if (key0 + 8 * i >= lim[z][c] || !((now >> (i >> 1)) & 1u)) s[z][i >> 1][i & 1][c] = -INFINITY;
         }
-        float top[kSets];
+        float top[kSets][kCols];
         bool grows = false;
 #pragma unroll
-        for (int z = 0; z < kSets; ++z) {
-            const float* x = s[z];
-            top[z] = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-            mx[z] = fmaxf(mx[z], top[z]);
-            grows |= top[z] > m[z] + kGrow;
-        }
+        for (int z = 0; z < kSets; ++z)
+#pragma unroll
+            for (int c = 0; c < kCols; ++c) {
+                top[z][c] = fmaxf(fmaxf(s[z][0][0][c], s[z][0][1][c]), fmaxf(s[z][1][0][c], s[z][1][1][c]));
+                st.mx[z][c] = fmaxf(st.mx[z][c], top[z][c]);
+                grows |= top[z][c] > st.m[z][c] + kGrow;
+            }
         if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
-            for (int z = 0; z < kSets; ++z) {
-                const float best = quad_max(top[z]);
-                if (best > m[z] + kGrow) {
-                    const float a = m[z] == -INFINITY ? 0.f : ex2_approx(m[z] - best);
-                    m[z] = best;
-                    l[z] *= a;
-                    rescale(z, a);
+            for (int z = 0; z < kSets; ++z)
+#pragma unroll
+                for (int c = 0; c < kCols; ++c) {
+                    const float best = column_max(top[z][c]);
+                    if (best > st.m[z][c] + kGrow) {
+                        if (st.m[z][c] != -INFINITY || st.l[z][c] != 0.f) {  // (else there is nothing to scale yet)
+                            const float a = ex2_approx(st.m[z][c] - best);
+                            st.l[z][c] *= a;
+                            st.rescale(z, c, a);
+                        }
+                        st.m[z][c] = best;
+                    }
                 }
-            }
         }
+        cp_wait<kStages - 1>();
+        __syncwarp();
+        const Stage& vp = ring[slot];
         // weights p and p * v_scale; a hidden key weighs nothing, whatever its scale is
-        float u[kSets][8], utop[kSets];
+        float u[kSets][2][2][kCols];
         grows = false;
 #pragma unroll
-        for (int z = 0; z < kSets; ++z) {
-            const float m_safe = m[z] == -INFINITY ? 0.f : m[z];  // (no key seen yet: every weight is 2^-inf)
+        for (int a = 0; a < 2; ++a)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float w = ex2_approx(s[z][i] - m_safe);
-                l[z] += w;
-                u[z][i] = w * vv[i];
-            }
-            if (!whole) {
+            for (int k = 0; k < 2; ++k) {
+                const float vs = vp.scale[kSub * a + 8 * k + g];
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (s[z][i] == -INFINITY) u[z][i] = 0.f;
+                for (int z = 0; z < kSets; ++z)
+#pragma unroll
+                    for (int c = 0; c < kCols; ++c) {
+                        const float m_safe = st.m[z][c] == -INFINITY ? 0.f : st.m[z][c];  // (no key seen yet: every weight is 2^-inf)
+                        const float w = ex2_approx(s[z][a][k][c] - m_safe);
+                        st.l[z][c] += w;
+                        u[z][a][k][c] = w * vs;
+                        if (!whole && s[z][a][k][c] == -INFINITY) u[z][a][k][c] = 0.f;
+                    }
             }
-            const float* x = u[z];
-            utop[z] = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-            grows |= utop[z] * f[z] > 32768.f;
-        }
+#pragma unroll
+        for (int z = 0; z < kSets; ++z)
+#pragma unroll
+            for (int c = 0; c < kCols; ++c) {
+                top[z][c] = fmaxf(fmaxf(u[z][0][0][c], u[z][0][1][c]), fmaxf(u[z][1][0][c], u[z][1][1][c]));
+                grows |= top[z][c] * st.f[z][c] > 32768.f;
+            }
         if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
-            for (int z = 0; z < kSets; ++z) {
-                const float best = quad_max(utop[z]);
-                if (best * f[z] > 32768.f) {
-                    const float fn = pow2(min(max(8 - exponent(best), -120), 100));
-                    rescale(z, fn / f[z]);  // a power of two
-                    f[z] = fn;
+            for (int z = 0; z < kSets; ++z)
+#pragma unroll
+                for (int c = 0; c < kCols; ++c) {
+                    const float best = column_max(top[z][c]);
+                    if (best * st.f[z][c] > 32768.f) {
+                        const float fn = pow2(min(max(8 - exponent(best), -120), 100));
+                        if (st.f[z][c] != pow2(100)) st.rescale(z, c, fn / st.f[z][c]);  // by a power of two
+                        st.f[z][c] = fn;
+                    }
                 }
-            }
         }
 #pragma unroll
         for (int a = 0; a < 2; ++a) {
-            uint32_t a0, a1, a2, a3;
-            if (kWide) {
-                constexpr int y = kSets - 1;
-                a0 = half_pair(u[0][4 * a] * f[0], u[0][4 * a + 1] * f[0]);
-                a1 = half_pair(u[y][4 * a] * f[y], u[y][4 * a + 1] * f[y]);
-                a2 = half_pair(u[0][4 * a + 2] * f[0], u[0][4 * a + 3] * f[0]);
-                a3 = half_pair(u[y][4 * a + 2] * f[y], u[y][4 * a + 3] * f[y]);
-            } else {
-                split_pair(u[0][4 * a] * f[0], u[0][4 * a + 1] * f[0], a0, a1);
-                split_pair(u[0][4 * a + 2] * f[0], u[0][4 * a + 3] * f[0], a2, a3);
-            }
-            uint4 v[4];
+            uint32_t pb[kSets][kParts][2];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = st.v[4 * a + i][lane];
+            for (int z = 0; z < kSets; ++z)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const float x = u[z][a][k][0] * st.f[z][0], y = kCols == 2 ? u[z][a][k][kCols - 1] * st.f[z][kCols - 1] : 0.f;
+                    if (kF32) {
+                        uint32_t hi, lo;
+                        split_pair(x, y, hi, lo);
+                        pb[z][0][k] = transposed(hi);
+                        pb[z][kParts - 1][k] = transposed(lo);
+                    } else {
+                        pb[z][0][k] = transposed(half_pair(x, y));
+                    }
+                }
+            uint32_t v[4][4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(v[i]) = vp.d[4 * a + i][lane];
             if (!whole) {  // codes of hidden keys may be anything, a NaN too
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (key0 + a * kSub + i >= keys || !((now >> a) & 1u)) v[i] = make_uint4(0, 0, 0, 0);
+                    if (tile * kTile + kSub * a + 2 * t + (i & 1) + 8 * (i >> 1) >= keys || !((now >> a) & 1u))
+                        v[i][0] = v[i][1] = v[i][2] = v[i][3] = 0u;
             }
-            const uint32_t v0[4] = {v[0].x, v[0].y, v[0].z, v[0].w}, v1[4] = {v[1].x, v[1].y, v[1].z, v[1].w};
-            const uint32_t v2[4] = {v[2].x, v[2].y, v[2].z, v[2].w}, v3[4] = {v[3].x, v[3].y, v[3].z, v[3].w};
 #pragma unroll
             for (int e = 0; e < 4; ++e)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    uint32_t b0e, b0o, b1e, b1o;
-                    pairs_across<kFmt>(v0[e], v1[e], i, b0e, b0o);
-                    pairs_across<kFmt>(v2[e], v3[e], i, b1e, b1o);
-                    mma_f16(acc[4 * e + 2 * i], a0, a1, a2, a3, b0e, b1e);
-                    mma_f16(acc[4 * e + 2 * i + 1], a0, a1, a2, a3, b0o, b1o);
+                    uint32_t a0, a1, a2, a3;
+                    pairs_across<kFmt>(v[0][e], v[1][e], i, a0, a1);
+                    pairs_across<kFmt>(v[2][e], v[3][e], i, a2, a3);
+#pragma unroll
+                    for (int z = 0; z < kSets; ++z)
+#pragma unroll
+                        for (int c = 0; c < kParts; ++c) mma_f16(st.acc[z][2 * e + i], a0, a1, a2, a3, pb[z][c][0], pb[z][c][1]);
                 }
         }
+        __syncwarp();  // every lane is done with this piece
+        have = next;
+        next = halves(tile + 2 * step, pages[2]);
+        issue(false, tile + 2 * step, pages[2], next, slot);
+        slot = slot == kStages - 1 ? 0 : slot + 1;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) pages[1][i] = pages[2][i], pages[2][i] = far[i];
     }
     cp_wait<0>();
     __syncwarp();
+}
 
-    // join the warps: every warp's rows in units of 2^-m
+// Joins a CTA's warps: each puts its rows into its ring, then a warp takes a row, four dims a
+// lane, and calls done(row, sums, maximum that they refer to, largest score).
+template <int kForm, typename Done>
+__device__ __forceinline__ void join_warps(Smem& sm, const State<kForm>& st, int rows, Done done) {
+    constexpr int kSets = kForm == kWide ? 2 : 1, kCols = kForm == kFew ? 1 : 2;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int g = lane >> 2, t = lane & 3;
 #pragma unroll
-    for (int z = 0; z < kSets; ++z) {
-        const int row = g + 8 * z;
-        const float lq = quad_sum(l[z]), mq = quad_max(mx[z]);
-        const float inv = 1.f / f[z];
-        // (the 16-byte pieces of a 128-byte span are exchanged by 2t + row: no bank conflicts)
-        float* o = reinterpret_cast<float*>(ring) + row * kD;
+    for (int z = 0; z < kSets; ++z)
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
+        for (int c = 0; c < kCols; ++c) {
+            const int row = 8 * z + kCols * t + c;
+            const float l = column_sum(st.l[z][c]), mx = column_max(st.mx[z][c]);
+            const float inv = 1.f / st.f[z][c];
+            // (a row's 16-byte pieces are exchanged within 128-byte spans: fewer bank conflicts)
+            float* o = reinterpret_cast<float*>(sm.ring[warp]) + row * kD;
 #pragma unroll
-            for (int j = 0; j < 16; j += 4) {
-                const int piece = 8 * t + ((4 * c + (j >> 2)) ^ ((2 * t + g) & 7));
-                float y[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) y[e] = (kWide ? acc[j + e][2 * z + c] : acc[j + e][c] + acc[j + e][c + 2]) * inv;
-                *reinterpret_cast<float4*>(o + 4 * piece) = make_float4(y[0], y[1], y[2], y[3]);
-            }
-        if (t == 0) sm.m[warp][row] = m[z], sm.l[warp][row] = lq, sm.mx[warp][row] = mq;
-    }
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<float4*>(o + 4 * ((4 * g + i) ^ (row & 7))) =
+                    make_float4(st.sum(z, c, 4 * i) * inv, st.sum(z, c, 4 * i + 1) * inv, st.sum(z, c, 4 * i + 2) * inv,
+                                st.sum(z, c, 4 * i + 3) * inv);
+            if (g == 0) sm.m[warp][row] = st.m[z][c], sm.l[warp][row] = l, sm.mx[warp][row] = mx;
+        }
     __syncthreads();
-    const int rows = min(kRows, p.T * p.group - row0);
-    float* mine = reinterpret_cast<float*>(&sm.ring[0][1]);
     for (int row = warp; row < rows; row += kWarps) {  // a warp per row, four dims a lane
-        const int piece = (lane & 24) + ((lane & 7) ^ ((2 * (lane >> 3) + row) & 7));
         float best = -INFINITY, big = -INFINITY;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) best = fmaxf(best, sm.m[w][row]), big = fmaxf(big, sm.mx[w][row]);
@@ -584,19 +652,51 @@ __global__ void __launch_bounds__(kThreads, 3) split_kernel(const Params p) {
 #pragma unroll
         for (int w = 0; w < kWarps; ++w)
             y.add(sm.m[w][row], sm.l[w][row], best,
-                  *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(sm.ring[w]) + row * kD + 4 * piece));
-        if (p.part_o) {
-            const int rr = row0 + row;
-            const long long out = ((long long)b * p.T + rr / p.group) * p.heads + hk * p.group + rr % p.group;
-            const long long at = (long long)(p.first_part + rank) * p.B * p.T * p.heads + out;
-            reinterpret_cast<float4*>(p.part_o + at * kD)[lane] = y.o;
-            if (lane == 0) p.part_s[at] = make_float4(best, y.l, big, 0.f);
-        } else {
-            reinterpret_cast<float4*>(mine + row * kD)[lane] = y.o;
-            if (lane == 0) sm.om[row] = best, sm.ol[row] = y.l, sm.omx[row] = big;
-        }
+                  *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(sm.ring[w]) + row * kD + 4 * (lane ^ (row & 7))));
+        done(row, y, best, big);
     }
-    if (p.part_o) return;
+}
+
+// A cluster of `split` CTAs per work item (8 or 16 query rows of a sequence and K/V head): their
+// warps take the sequence's tiles in turn and are joined in shared memory, then over the cluster.
+// Where there are more CTAs than the GPU holds, those of the longest sequences come first, so
+// that the last to start are the shortest.
+template <int kFmt, bool kF32, int kForm>
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(kF32, kForm)) split_kernel(const Params p) {
+    pdl_enter();
+    constexpr int kRows = rows_of(kForm);
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)(blockIdx.x % (unsigned)p.split);
+    const int item = (int)(blockIdx.x / (unsigned)p.split);
+    const int per_head = (p.T * p.group + kRows - 1) / kRows;
+    const int hk = item / per_head % p.c.heads;
+    const int row0 = item % per_head * kRows;
+    int b = item / per_head / p.c.heads;
+    if (p.by_length) {  // the b-th longest, ties by number: every thread ranks its sequences
+        int* lens = reinterpret_cast<int*>(&sm.ring);
+        for (int i = threadIdx.x; i < p.B; i += kThreads) lens[i] = p.seq_lens[i];
+        __syncthreads();
+        for (int i = threadIdx.x; i < p.B; i += kThreads) {
+            const int mine = lens[i];
+            int rank = 0;
+            for (int j = 0; j < p.B; ++j) rank += lens[j] > mine || (lens[j] == mine && j < i);
+            if (rank == b) sm.om[0] = __int_as_float(i);
+        }
+        __syncthreads();
+        b = __float_as_int(sm.om[0]);
+        __syncthreads();
+    }
+
+    State<kForm> st;
+    attend<kFmt, kF32, kForm>(p, sm.ring[warp], b, hk, row0, rank * kWarps + warp, 0x7fffffff, p.split * kWarps, st);
+
+    const int rows = min(kRows, p.T * p.group - row0);
+    join_warps<kForm>(sm, st, rows, [&](int row, const Joined& y, float best, float big) {
+        reinterpret_cast<float4*>(sm.joined(row))[lane] = y.o;
+        if (lane == 0) sm.om[row] = best, sm.ol[row] = y.l, sm.omx[row] = big;
+    });
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
     if (p.split > 1) cluster.sync();
@@ -608,45 +708,201 @@ __global__ void __launch_bounds__(kThreads, 3) split_kernel(const Params p) {
         const int rr = row0 + row;
         float best = -INFINITY, big = -INFINITY;
         for (int c = 0; c < p.split; ++c) {
-            const Smem* other = p.split > 1 ? cluster.map_shared_rank(&sm, c) : &sm;
+            Smem* other = p.split > 1 ? cluster.map_shared_rank(&sm, c) : &sm;
             best = fmaxf(best, other->om[row]), big = fmaxf(big, other->omx[row]);
         }
         Joined y;
         for (int c = 0; c < p.split; ++c) {
-            const Smem* other = p.split > 1 ? cluster.map_shared_rank(&sm, c) : &sm;
+            Smem* other = p.split > 1 ? cluster.map_shared_rank(&sm, c) : &sm;
             y.add(other->om[row], other->ol[row], best,
-                  reinterpret_cast<const float4*>(reinterpret_cast<const float*>(&other->ring[0][1]) + row * kD)[lane]);
+                  reinterpret_cast<const float4*>(other->joined(row))[lane]);
         }
         store_row<kF32>(p, ((long long)b * p.T + rr / p.group) * p.heads + hk * p.group + rr % p.group, lane, y, best, big);
     }
     if (p.split > 1) cluster.sync();  // no CTA leaves while another reads its shared memory
 }
 
-// Joins the parts of each query row: a warp per row, four dims a lane.
-template <bool kF32>
-__global__ void __launch_bounds__(128) join_kernel(const Params p) {
+// Tiles of sequence b's keys (those of its last query).
+__device__ __forceinline__ int tiles_of(const Params& p, int b) {
+    const int q_len = p.q_lens ? min(p.q_lens[b], p.T) : p.T;
+    const long long keys = min((long long)p.seq_lens[b], (long long)p.max_pages << p.c.page_shift);
+    return q_len > 0 && keys > 0 ? (int)((keys + kTile - 1) / kTile) : 0;
+}
+
+// CTA w of W takes the tiles [w n / W, (w + 1) n / W) of all n tiles of all items in order
+// (sequence, K/V head, rows): every CTA has the same amount of work whatever the lengths are.
+// W <= n, so that none of them has nothing (and leaves a part unwritten that join_kernel reads).
+__device__ __forceinline__ int shares_of(const Params& p, long long n) { return (int)min((long long)p.shares, n); }
+__device__ __forceinline__ long long first_tile(long long n, int w, int W) { return n * w / W; }
+// The CTA that takes tile x.
+__device__ __forceinline__ int share_of(long long n, long long x, int W) { return (int)(((x + 1) * W - 1) / n); }
+
+// One even share of all the work per CTA, for few items of many keys; its warps take the share's tiles
+// in turn.  A share may begin and end inside items: what it has of an item goes to the workspace at
+// slot w + item (which no other pair of CTA and item has, since one of the two grows from pair
+// to pair), and join_kernel adds the parts up.  An item that lies within one share is written at once.
+constexpr int kMaxBatch = 8192;  // the first tiles of so many sequences fit into the ring's memory
+template <int kFmt, bool kF32, int kForm>
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(kF32, kForm)) stream_kernel(const Params p) {
     pdl_enter();
-    const long long rows = (long long)p.B * p.T * p.heads;
-    const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (row >= rows) return;
-    float best = -INFINITY, big = -INFINITY;
-    for (int i = lane; i < p.n_parts; i += 32) {
-        const float4 s = p.part_s[i * rows + row];
-        best = fmaxf(best, s.x), big = fmaxf(big, s.z);
-    }
+    constexpr int kRows = rows_of(kForm);
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
+    static_assert(sizeof(sm.ring) >= (kMaxBatch + 1) * 4, "first tiles of a batch");
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    // starts[b] = tiles of the sequences before b; in the ring's memory until the first tile comes
+    int* starts = reinterpret_cast<int*>(&sm.ring);
+    {
+        __shared__ int totals[kWarps];
+        const int per = (p.B + kThreads - 1) / kThreads;
+        const int b0 = min((int)threadIdx.x * per, p.B), b1 = min(b0 + per, p.B);
+        int sum = 0;
+        for (int b = b0; b < b1; ++b) sum += tiles_of(p, b);
+        int before = sum;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
-        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, before, o);
+            if (lane >= o) before += y;
+        }
+        if (lane == 31) totals[warp] = before;
+        __syncthreads();
+        before -= sum;
+        for (int w = 0; w < warp; ++w) before += totals[w];
+        for (int b = b0; b < b1; ++b) {
+            starts[b] = before;
+            if (blockIdx.x == 0) p.starts[b] = before;
+            before += tiles_of(p, b);
+        }
+        if (threadIdx.x == kThreads - 1) {
+            starts[p.B] = before;
+            if (blockIdx.x == 0) p.starts[p.B] = before;
+        }
+        __syncthreads();
     }
+    const int per_head = (p.T * p.group + kRows - 1) / kRows;
+    const int items = p.c.heads * per_head;  // of one sequence
+    const long long n = (long long)starts[p.B] * items;
+    const int w = blockIdx.x, W = shares_of(p, n);
+    if (w >= W) return;
+    long long x = first_tile(n, w, W);
+    const long long end = first_tile(n, w + 1, W);
+    // the sequence that tile x is of: the last one that starts at or before it
+    int b = 0;
+    for (int up = kMaxBatch / 2; up > 0; up >>= 1)
+        if (b + up < p.B && (long long)starts[b + up] * items <= x) b += up;
+    long long at = (long long)starts[b] * items;
+    while (x < end) {
+        const int tiles = tiles_of(p, b);
+        if (x >= at + (long long)tiles * items) {
+            at += (long long)tiles * items;
+            ++b;
+            continue;
+        }
+        const int i = (int)((x - at) / tiles);
+        const int tile0 = (int)((x - at) % tiles);
+        const int tile1 = (int)min((long long)tiles, tile0 + (end - x));
+        const int hk = i / per_head, row0 = i % per_head * kRows;
+        __syncthreads();  // the ring's memory is free
+        State<kForm> st;
+        attend<kFmt, kF32, kForm>(p, sm.ring[warp], b, hk, row0, tile0 + warp, tile1, kWarps, st);
+        const bool whole = tile0 == 0 && tile1 == tiles && p.n_shared == 0;
+        const long long slot = ((long long)w + (long long)b * items + i) * kRows;
+        join_warps<kForm>(sm, st, min(kRows, p.T * p.group - row0), [&](int row, const Joined& y, float best, float big) {
+            if (whole) {
+                const int r = row0 + row;
+                store_row<kF32>(p, ((long long)b * p.T + r / p.group) * p.heads + hk * p.group + r % p.group, lane, y, best, big);
+            } else {
+                reinterpret_cast<float4*>(p.part_o + (slot + row) * kD)[lane] = y.o;
+                if (lane == 0) p.part_s[slot + row] = make_float4(best, y.l, big, 0.f);
+            }
+        });
+        x += tile1 - tile0;
+    }
+}
+
+// Joins the parts of each query row: a CTA per row, its warps taking eight parts at a time (so
+// that eight rows of 512 bytes are on their way at once), then joined themselves.
+constexpr int kJoinWarps = 4;
+template <bool kF32, int kForm>
+__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const Params p) {
+    pdl_enter();
+    constexpr int kRows = rows_of(kForm);
+    const long long rows = (long long)p.B * p.T * p.heads;
+    const long long row = blockIdx.x;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int h = (int)(row % p.heads), tq = (int)(row / p.heads % p.T), b = (int)(row / p.heads / p.T);
+    const int r = tq * p.group + h % p.group;
+    const int q_len = p.q_lens ? min(p.q_lens[b], p.T) : p.T;
+
+    // the CTAs that had a part of this row's item
+    int parts = 0;
+    long long slot = 0;
+    if (p.shares > 0) {
+        const int per_head = (p.T * p.group + kRows - 1) / kRows;
+        const int items = p.c.heads * per_head;
+        const int i = h / p.group * per_head + r / kRows;
+        const int start = p.starts[b], tiles = p.starts[b + 1] - start;
+        const long long n = (long long)p.starts[p.B] * items;
+        if (tiles > 0) {
+            const long long x = (long long)start * items + (long long)i * tiles;
+            const int W = shares_of(p, n);
+            const int first = share_of(n, x, W);
+            parts = share_of(n, x + tiles - 1, W) - first + 1;
+            if (parts == 1 && p.n_shared == 0) return;  // written by stream_kernel
+            slot = (long long)first + (long long)b * items + i;
+        }
+    }
+    const int shared = tq < q_len ? p.n_shared : 0;
+    const float4* own_s = p.part_s + slot * kRows + r % kRows;
+    const float4* own_o = reinterpret_cast<const float4*>(p.part_o + (slot * kRows + r % kRows) * kD) + lane;
+    const float4* shared_s = p.shared_s + row;
+    const float4* shared_o = reinterpret_cast<const float4*>(p.shared_o + row * kD) + lane;
+    float m = -INFINITY, big = -INFINITY;
     Joined y;
-#pragma unroll 8
-    for (int i = 0; i < p.n_parts; ++i) {
-        const float4 s = p.part_s[i * rows + row];
-        y.add(s.x, s.y, best, reinterpret_cast<const float4*>(p.part_o + (i * rows + row) * kD)[lane]);
+    for (int i0 = 8 * warp; i0 < parts + shared; i0 += 8 * kJoinWarps) {
+        float4 s = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
+        const int mine = i0 + (lane & 7);
+        if (mine < parts) s = own_s[(long long)mine * kRows];
+        else if (mine < parts + shared) s = shared_s[(mine - parts) * rows];
+        float4 o[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (i0 + i < parts) o[i] = own_o[(long long)(i0 + i) * kRows * (kD / 4)];
+            else if (i0 + i < parts + shared) o[i] = shared_o[(i0 + i - parts) * rows * (kD / 4)];
+        }
+        float top = s.x;
+#pragma unroll
+        for (int w = 1; w < 8; w <<= 1) {
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+            s.z = fmaxf(s.z, __shfl_xor_sync(0xffffffffu, s.z, w));
+        }
+        big = fmaxf(big, s.z);
+        if (top > m) {
+            const float a = m == -INFINITY ? 1.f : ex2_approx(m - top);  // (at -inf there may be NaNs, which stay)
+            m = top;
+            y.l *= a;
+            y.o.x *= a, y.o.y *= a, y.o.z *= a, y.o.w *= a;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            y.add(__shfl_sync(0xffffffffu, s.x, i), __shfl_sync(0xffffffffu, s.y, i), m, o[i]);
     }
-    store_row<kF32>(p, row, lane, y, best, big);
+    __shared__ float4 so[kJoinWarps][32];
+    __shared__ float sm[kJoinWarps], sl[kJoinWarps], sx[kJoinWarps];
+    so[warp][lane] = y.o;
+    if (lane == 0) sm[warp] = m, sl[warp] = y.l, sx[warp] = big;
+    __syncthreads();
+    if (warp != 0) return;
+    float best = -INFINITY;
+    big = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) best = fmaxf(best, sm[w]), big = fmaxf(big, sx[w]);
+    Joined all;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) all.add(sm[w], sl[w], best, so[w][lane]);
+    store_row<kF32>(p, row, lane, all, best, big);
 }
 
 }  // namespace cache_attn

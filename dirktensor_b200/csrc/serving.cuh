@@ -117,38 +117,59 @@ namespace {
 
 constexpr int kPlanSms = 148;  // B200; the plan is made without a device, for the workspace size
 
-// How the split kernel's work is cut: see the rules at plan_split.
-struct SplitPlan {
-    bool wide;       // 16 query rows per CTA
-    long long items; // (sequence, K/V head, rows) that a cluster or a group of CTAs takes
-    int split;       // CTAs per item
-    bool parts;      // joined through the workspace
+// How the attention's work is cut.
+struct AttnPlan {
+    int form;         // query rows per item: rows_of(form)
+    long long items;  // (sequence, K/V head, rows)
+    int split;        // CTAs per item (split_kernel), or
+    bool by_length;   // longest sequences first (split_kernel)
+    int shares;       // CTAs of stream_kernel, which join_kernel follows (0: split_kernel)
 };
 
-#ifndef DT_ATTN_FORCE_SPLIT
-#define DT_ATTN_FORCE_SPLIT 0
-#endif
-SplitPlan plan_split(int B, int T, int heads, int kv_heads, int q_f32, int page_size, int max_pages) {
+// split_kernel, with as many CTAs per item as the GPU holds at once, up to a cluster, and no more
+// than there are tiles for; stream_kernel where that leaves most of the GPU idle: few items with
+// many keys.  (8 x 131071 keys: 71 us shared by 444 CTAs, 149 us in 8 clusters of 8.)
+AttnPlan plan_attn(int B, int T, int heads, int kv_heads, int q_f32, int page_size, int max_pages, int prefix_len) {
     namespace ca = dt::cache_attn;
-    SplitPlan s{};
+    AttnPlan s{};
     const int rows = T * (heads / kv_heads);
-    s.wide = !q_f32 && rows > 8;
-    s.items = (long long)B * kv_heads * ((rows + (s.wide ? 15 : 7)) / (s.wide ? 16 : 8));
+    s.form = rows <= 4 ? ca::kFew : q_f32 || rows <= 8 ? ca::kEight : ca::kWide;
+    s.items = (long long)B * kv_heads * ((rows + ca::rows_of(s.form) - 1) / ca::rows_of(s.form));
     const long long tiles = ((long long)max_pages * page_size + ca::kTile - 1) / ca::kTile;
-    const long long slots = 3 * kPlanSms;
-    s.split = 1;
-    while (s.split < ca::kMaxCluster && s.items * s.split * 2 <= slots && tiles > (long long)s.split * ca::kWarps) s.split *= 2;
-    if (s.split == ca::kMaxCluster && s.items * s.split * 2 <= slots && tiles > 4ll * s.split * ca::kWarps) {
-        s.parts = true;
-        s.split = (int)std::min(slots / s.items, tiles / (2 * ca::kWarps));
+    const int slots = ca::ctas_per_sm(q_f32, s.form) * kPlanSms;
+    const bool fits = B <= ca::kMaxBatch && tiles * B < 0x7fffffffll && s.items < 0x7fffffffll - slots;
+    const bool few = s.items * ca::kMaxCluster * 2 < slots && tiles > 4ll * ca::kMaxCluster * ca::kWarps;
+    if (prefix_len > 0 || (fits && few)) {
+        s.shares = fits ? (int)std::min<long long>(slots, (s.items * tiles + ca::kWarps - 1) / ca::kWarps) : -1;
+        return s;
     }
-    if (DT_ATTN_FORCE_SPLIT) s.split = DT_ATTN_FORCE_SPLIT, s.parts = false;
+    s.split = 1;
+    while (s.split < ca::kMaxCluster && s.items * (s.split + 1) <= slots && tiles > (long long)s.split * ca::kWarps) ++s.split;
+    s.by_length = s.items > slots && B <= 256;
     return s;
 }
 
-size_t parts_bytes(long long parts, int B, int T, int heads) {
-    const size_t rows = (size_t)B * T * heads;
-    return align256(parts * rows * 16) + align256(parts * rows * dt::cache_attn::kD * 4);
+// Workspace of a plan: the tile counts, the CTAs' parts, the prefix's parts.
+struct AttnSpace {
+    size_t starts, part_s, part_o, shared_s, shared_o, total;
+};
+AttnSpace attn_space(const AttnPlan& plan, int B, int T, int heads, int n_shared) {
+    AttnSpace w{};
+    const size_t parts = plan.shares > 0 ? ((size_t)plan.shares + plan.items) * dt::cache_attn::rows_of(plan.form) : 0;
+    const size_t shared = (size_t)n_shared * B * T * heads;
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t here = at;
+        at += align256(bytes);
+        return here;
+    };
+    w.starts = take(plan.shares > 0 ? ((size_t)B + 1) * 4 : 0);
+    w.part_s = take(parts * 16);
+    w.part_o = take(parts * dt::cache_attn::kD * 4);
+    w.shared_s = take(shared * 16);
+    w.shared_o = take(shared * dt::cache_attn::kD * 4);
+    w.total = at;
+    return w;
 }
 
 int launch_split(void (*kernel)(dt::cache_attn::Params), const dt::cache_attn::Params& p, long long items,
@@ -157,7 +178,7 @@ int launch_split(void (*kernel)(dt::cache_attn::Params), const dt::cache_attn::P
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = DT_PDL;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = p.part_o ? 1u : (unsigned)p.split;
+    attr[1].val.clusterDim.x = (unsigned)p.split;
     attr[1].val.clusterDim.y = 1;
     attr[1].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg = {};
@@ -171,31 +192,41 @@ int launch_split(void (*kernel)(dt::cache_attn::Params), const dt::cache_attn::P
     return DT_OK;
 }
 
-int launch_join(const dt::cache_attn::Params& p, int q_f32, cudaStream_t st) {
-    const dim3 grid((unsigned)(((long long)p.B * p.T * p.heads + 3) / 4)), block(128);
-    return q_f32 ? launch_pdl(dt::cache_attn::join_kernel<true>, grid, block, 0, st, p)
-                 : launch_pdl(dt::cache_attn::join_kernel<false>, grid, block, 0, st, p);
+typedef void (*AttnKernel)(dt::cache_attn::Params);
+template <int kFmt, bool kF32, int kForm>
+AttnKernel attn_kernel_of(bool stream) {
+    return stream ? dt::cache_attn::stream_kernel<kFmt, kF32, kForm> : dt::cache_attn::split_kernel<kFmt, kF32, kForm>;
+}
+template <int kFmt>
+AttnKernel attn_kernel_of(bool stream, bool f32, int form) {
+    namespace ca = dt::cache_attn;
+    if (f32) return form == ca::kFew ? attn_kernel_of<kFmt, true, ca::kFew>(stream) : attn_kernel_of<kFmt, true, ca::kEight>(stream);
+    return form == ca::kFew     ? attn_kernel_of<kFmt, false, ca::kFew>(stream)
+           : form == ca::kEight ? attn_kernel_of<kFmt, false, ca::kEight>(stream)
+                                : attn_kernel_of<kFmt, false, ca::kWide>(stream);
+}
+AttnKernel attn_kernel_of(bool stream, int format, bool f32, int form) {
+    return format == DT_KV_INT8 ? attn_kernel_of<0>(stream, f32, form) : attn_kernel_of<1>(stream, f32, form);
 }
 
-template <int kFmt>
-void (*split_kernel_of(bool f32, bool wide))(dt::cache_attn::Params) {
+int launch_stream(const dt::cache_attn::Params& p, const AttnPlan& plan, int format, int q_f32, cudaStream_t st) {
     namespace ca = dt::cache_attn;
-    return f32 ? ca::split_kernel<kFmt, true, false> : wide ? ca::split_kernel<kFmt, false, true> : ca::split_kernel<kFmt, false, false>;
+    if (plan.shares > 0)
+        DT_TRY(launch_pdl(attn_kernel_of(true, format, q_f32, plan.form),
+                          dim3((unsigned)plan.shares), dim3(ca::kThreads), sizeof(ca::Smem), st, p));
+    const dim3 grid((unsigned)((long long)p.B * p.T * p.heads)), block(ca::kJoinWarps * 32);
+    AttnKernel join = ca::join_kernel<false, ca::kWide>;
+    if (plan.form == ca::kFew) join = q_f32 ? ca::join_kernel<true, ca::kFew> : ca::join_kernel<false, ca::kFew>;
+    if (plan.form == ca::kEight) join = q_f32 ? ca::join_kernel<true, ca::kEight> : ca::join_kernel<false, ca::kEight>;
+    return launch_pdl(join, grid, block, 0, st, p);
 }
 
 // Per-device attributes of the kernels below (called with g_mu held, from ensure_attrs).
 int serving_attrs() {
-    for (int i = 0; i < 6; ++i) {
-        auto* k = i & 1 ? split_kernel_of<1>(i >= 4, i >= 2) : split_kernel_of<0>(i >= 4, i >= 2);
-        DT_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(dt::cache_attn::Smem)));
-    }
+    for (int i = 0; i < 24; ++i)
+        DT_CUDA(cudaFuncSetAttribute(attn_kernel_of(i & 1, (i >> 1) & 1, (i >> 2) & 1, i / 8),
+                                     cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(dt::cache_attn::Smem)));
     return DT_OK;
-}
-
-void set_parts(dt::cache_attn::Params& p, int parts, void* workspace) {
-    p.n_parts = parts;
-    p.part_s = static_cast<float4*>(workspace);
-    p.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + align256((size_t)parts * p.B * p.T * p.heads * 16));
 }
 
 int cache_attn(const dt_kv_cache* cache, const void* q, long long q_batch_stride, long long q_token_stride, int q_f32,
@@ -209,6 +240,8 @@ int cache_attn(const dt_kv_cache* cache, const void* q, long long q_batch_stride
         return fail(DT_ERR_INVALID_ARGUMENT, "heads (%d) must be a multiple of kv_heads (%d)", heads, cache->kv_heads);
     if (B == 0 || T == 0 || heads == 0) return DT_OK;
     DT_TRY(check_table(page_table, page_table_stride, max_pages, B));
+    if (((long long)max_pages << p.c.page_shift) > (1ll << 30))
+        return fail(DT_ERR_INVALID_ARGUMENT, "max_pages * page_size must be at most 2^30");
     if (!seq_lens && max_pages > 0) return fail(DT_ERR_INVALID_ARGUMENT, "null seq_lens");
     DT_TRY(check_strides("q", q, q_batch_stride, q_token_stride, q_f32 ? 4 : 2));
     if (!o || !aligned16(o)) return fail(DT_ERR_INVALID_ARGUMENT, "o must be non-null and 16-byte aligned");
@@ -233,23 +266,31 @@ int cache_attn(const dt_kv_cache* cache, const void* q, long long q_batch_stride
     p.heads = heads;
     p.group = heads / cache->kv_heads;
     p.scale = scale;
-    const size_t need = prefix_len > 0 ? dt_prefix_attn_workspace_bytes(B, T, heads, cache->kv_heads, prefix_len)
-                                       : dt_cache_attn_workspace_bytes(B, T, heads, cache->kv_heads, q_f32,
-                                                                       cache->page_size, max_pages);
-    if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
-        return fail(DT_ERR_INVALID_ARGUMENT, "workspace must be >= %zu bytes and 16-byte aligned", need);
+    const AttnPlan plan = plan_attn(B, T, heads, cache->kv_heads, q_f32, cache->page_size, max_pages, 0);
+    if (plan.items * std::max(plan.split, 1) > 0x7fffffffll)
+        return fail(DT_ERR_INVALID_ARGUMENT, "B * kv_heads * query rows is too large");
+    const AttnSpace space = attn_space(plan, B, T, heads, 0);
+    if (prefix_len == 0 && space.total > 0 && (!workspace || workspace_bytes < space.total || !aligned16(workspace)))
+        return fail(DT_ERR_INVALID_ARGUMENT, "workspace must be >= %zu bytes and 16-byte aligned", space.total);
     int dev;
     DT_TRY(prepare_device(&dev));
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     if (prefix_len == 0) {
-        const SplitPlan plan = plan_split(B, T, heads, cache->kv_heads, q_f32, cache->page_size, max_pages);
-        if (plan.items * plan.split > 0x7fffffffll)
-            return fail(DT_ERR_INVALID_ARGUMENT, "B * kv_heads * query rows is too large");
+        if (max_pages == 0) {  // no keys: zeros
+            p.shares = 0;
+            return launch_stream(p, AttnPlan{}, cache->format, q_f32, st);
+        }
         p.split = plan.split;
-        if (plan.parts) set_parts(p, plan.split, workspace);
-        DT_TRY(launch_split(cache->format == DT_KV_INT8 ? split_kernel_of<0>(q_f32, plan.wide) : split_kernel_of<1>(q_f32, plan.wide),
-                            p, plan.items, st));
-        return plan.parts ? launch_join(p, q_f32, st) : DT_OK;
+        p.shares = plan.shares;
+        p.by_length = plan.by_length;
+        if (plan.shares > 0) {
+            uint8_t* w = static_cast<uint8_t*>(workspace);
+            p.starts = reinterpret_cast<int*>(w + space.starts);
+            p.part_s = reinterpret_cast<float4*>(w + space.part_s);
+            p.part_o = reinterpret_cast<float*>(w + space.part_o);
+            return launch_stream(p, plan, cache->format, q_f32, st);
+        }
+        return launch_split(attn_kernel_of(false, cache->format, q_f32, plan.form), p, plan.items, st);
     }
     const dim3 grid((unsigned)(((long long)B * T * heads + 3) / 4)), block(128);
     if (cache->format == DT_KV_INT8)
@@ -276,8 +317,7 @@ int dt_cache_attn_fwd(const dt_kv_cache* cache, const void* q, long long q_batch
 size_t dt_cache_attn_workspace_bytes(int B, int T, int heads, int kv_heads, int q_f32, int page_size, int max_pages) {
     if (B <= 0 || T <= 0 || kv_heads <= 0 || heads < kv_heads || page_size <= 0 || max_pages <= 0) return 0;
     if ((long long)B * T * heads > 0x7fffffffll) return 0;
-    const SplitPlan plan = plan_split(B, T, heads, kv_heads, q_f32, page_size, max_pages);
-    return plan.parts ? parts_bytes(plan.split, B, T, heads) : 0;
+    return attn_space(plan_attn(B, T, heads, kv_heads, q_f32, page_size, max_pages, 0), B, T, heads, 0).total;
 }
 
 size_t dt_prefix_attn_workspace_bytes(int B, int T, int heads, int kv_heads, int prefix_len) {

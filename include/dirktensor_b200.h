@@ -424,7 +424,7 @@ int dt_kv_cache_read(const dt_kv_cache* cache, void* k, void* v, int dst_f32, co
  * t >= q_lens[b] and rows that see no key are written as zeros (m = l = 0).
  * Lengths past the page table are cut to it; keys on a page whose id is not in
  * 0..num_pages-1 are not seen.  Codes are exact in the products, which are
- * summed in fp32.  workspace: at least dt_cache_attn_workspace_bytes (which
+ * summed in fp32.  max_pages * page_size is at most 2^30.  workspace: at least dt_cache_attn_workspace_bytes (which
  * may be 0: then NULL), 16-byte aligned; calls that may overlap on the GPU
  * need one each.  Asynchronous on `stream`. */
 size_t dt_cache_attn_workspace_bytes(int B, int T, int heads, int kv_heads, int q_f32, int page_size, int max_pages);

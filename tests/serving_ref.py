@@ -47,11 +47,11 @@ def attention(q, cache, table, seq_lens, scale, q_lens=None, prefix_pages=None, 
     d = (128 + 4) * 2 * EPS32 * sum |q k| (twice, since the tensor cores may cut instead of round).
     A weight is then off by a factor of about 1 +- (2 d + 8 EPS32 (1 + |s - m|)), the sums of n
     weights by n * 2 * EPS32 more; p_half is half a step of the type that the weights are rounded to
-    for the second product (fp16, 2^-11, in any case where more than 8 bf16 queries share a K/V head).
+    for the second product (for bf16 queries at least fp16's, 2^-11).
     """
     B, T, H, _ = q.shape
     group = H // cache.kv_heads
-    if q.dtype == torch.bfloat16 and T * group > 8:
+    if q.dtype == torch.bfloat16:
         p_half = max(p_half, 2.0 ** -11)
     qd = q.double()
     o = torch.zeros((B, T, H, D), dtype=torch.float64, device=q.device)
@@ -85,8 +85,8 @@ def attention(q, cache, table, seq_lens, scale, q_lens=None, prefix_pages=None, 
                 o[b, t, h] = p @ v
                 rel = 2 * d + 8 * EPS32 * (1 + float((p * (s.max() - s)).sum())) + 2 * len(k) * EPS32 + p_half
                 o_tol[b, t, h] = HALF[q.dtype] * o[b, t, h].abs() + 2 * rel * (p @ v.abs())
-                # The second product takes p * v_scale as two fp16 numbers, scaled so that a row's largest is at
-                # least 2^8: each is off by at most half of fp16's smallest step, 2^-25, so by 2^-33 of the largest.
+                # The second product takes p * v_scale as fp16 numbers (fp32 queries: as two), scaled so that a row's largest
+                # is at least 2^8: each is off by at most half of fp16's smallest step, 2^-25, so by 2^-33 of the largest.
                 o_tol[b, t, h] += 2.0 ** -33 * float((p * vs).max()) * codes.sum(0)
                 m_tol[b, t, h] = d + EPS32 * abs(float(s.max()))
                 l_tol[b, t, h] = (2 * d + 8 * EPS32 * (1 + float((p * (s.max() - s)).sum())) + 2 * len(k) * EPS32) * w.sum()
