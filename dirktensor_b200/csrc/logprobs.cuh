@@ -7,17 +7,26 @@
 // s and u are kept together with the running maximum m: when m grows by d, s and u become
 // s e^-d and (u - d s) e^-d, so one pass over the row gives all three.  A logit of -inf (a
 // masked token) adds nothing; a row of nothing else has lse = log_prob = -inf and entropy 0.
-// The alternatives are ordered by logit, ties by the lower token id, NaN after every number.
+// Differences below -200 weigh nothing in fp32 and are cut there, which keeps infinities (and masks of the
+// type's lowest value) out of products with zero.  The alternatives are ordered by logit, ties by
+// the lower token id, NaN after every number.
 //
 //   d_logits_j = d_log_prob (1[j = t] - p_j) - d_entropy p_j (log p_j + entropy)
 #pragma once
+#include <cooperative_groups.h>
+
 #include "dt_common.cuh"
 
 namespace dt {
 namespace logprobs {
 
 constexpr int kThreads = 512;
+constexpr int kWarps = kThreads / 32;
 constexpr int kMaxTop = 32;
+constexpr int kMaxCluster = 8;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLowest = -3.402823466e38f;
+constexpr float kFar = -200.f;  // e^-200 is 0 in fp32: no difference below it counts
 
 struct Params {
     const void* x;       // [N, V], rows ld apart
@@ -31,6 +40,7 @@ struct Params {
     float* lse;          // [N] or null
     int* top_ids;        // [N, top]
     float* top_log_probs;
+    int split;           // CTAs (a cluster) per row
 };
 
 struct GradParams {
@@ -45,12 +55,12 @@ struct GradParams {
     const float* d_entropy;   // or null
     void* dx;                 // [N, V], rows dx_ld apart
     long long dx_ld;
+    int chunks;               // CTAs per row
 };
 
 template <bool kF32>
 __device__ __forceinline__ float logit(const void* x, long long i) {
-    return kF32 ? __ldg(static_cast<const float*>(x) + i)
-                : __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(x) + i));
+    return kF32 ? static_cast<const float*>(x)[i] : __bfloat162float(static_cast<const __nv_bfloat16*>(x)[i]);
 }
 
 __device__ __forceinline__ long long target_of(const void* t, int is64, int row) {
@@ -58,115 +68,362 @@ __device__ __forceinline__ long long target_of(const void* t, int is64, int row)
     return is64 ? __ldg(static_cast<const long long*>(t) + row) : (long long)__ldg(static_cast<const int*>(t) + row);
 }
 
-// Larger key = earlier alternative: the logit's bits in an order that integers share, NaN
-// lowest, then the token id downwards.
+// The larger of two, a NaN if either is one.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// The logit's bits in an order that unsigned numbers share, NaN lowest; -0 and 0 alike.
+__device__ __forceinline__ uint32_t order_bits(float x) {
+    const uint32_t u = __float_as_uint(x + 0.f);
+    return x != x ? 0u : (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float from_order_bits(uint32_t u) {
+    return u == 0u ? __uint_as_float(0x7fffffffu) : __uint_as_float((u & 0x80000000u) ? (u & 0x7fffffffu) : ~u);
+}
+// Larger key = earlier alternative: by logit, then by the lower id.  No logit has the key 0.
 __device__ __forceinline__ unsigned long long order_key(float x, int id) {
-    uint32_t u = __float_as_uint(x);
-    u = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-    if (x != x) u = 0u;
-    if (x == 0.f) u = 0x80000000u;  // -0 and 0 are equal
-    return ((unsigned long long)u << 32) | (uint32_t)(0x7fffffff - id);
+    return ((unsigned long long)order_bits(x) << 32) | (uint32_t)(0x7fffffff - id);
 }
 
-__device__ __forceinline__ void merge(float& m, float& s, float& u, float m2, float s2, float u2) {
-    const float mn = fmaxf(m, m2);
-    if (mn == -INFINITY) return;
-    const float d1 = m - mn, d2 = m2 - mn;  // 0 or negative; -inf for an empty side
-    const float e1 = expf(d1), e2 = expf(d2);
-    // (a term whose weight underflows is dropped before d * s can overflow)
-    u = (e1 == 0.f ? 0.f : (u + d1 * s) * e1) + (e2 == 0.f ? 0.f : (u2 + d2 * s2) * e2);
-    s = s * e1 + s2 * e2;
-    m = mn;
+// Lists of 32 numbers, one per lane, largest first.
+template <typename K>
+__device__ __forceinline__ K keep_larger(K x, int distance, bool larger) {
+    const K y = __shfl_xor_sync(0xffffffffu, x, distance);
+    return larger == (y > x) ? y : x;
 }
-
-// One CTA per row; one pass for the sums, then one pass per alternative.
-template <bool kF32>
-__global__ void __launch_bounds__(kThreads) row_kernel(const Params p) {
-    pdl_enter();
-    __shared__ float sm[kThreads / 32], ss[kThreads / 32], su[kThreads / 32];
-    __shared__ unsigned long long sk[kThreads / 32];
-    const int row = blockIdx.x;
-    const long long base = (long long)row * p.ld;
-    float m = -INFINITY, s = 0.f, u = 0.f;
-    bool bad = false;
-    for (int j = threadIdx.x; j < p.V; j += kThreads) {
-        const float x = logit<kF32>(p.x, base + j);
-        bad |= x != x;
-        if (x > -INFINITY) merge(m, s, u, x, 1.f, 0.f);
+template <typename K>
+__device__ __forceinline__ K sorted(K x) {  // bitonic
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+        for (int d = size >> 1; d > 0; d >>= 1) x = keep_larger(x, d, ((lane & d) == 0) == ((lane & size) == 0 || size == 32));
+    return x;
+}
+// The 32 largest of two lists.
+template <typename K>
+__device__ __forceinline__ K merged(K a, K b) {
+    const int lane = threadIdx.x & 31;
+    b = __shfl_sync(0xffffffffu, b, 31 - lane);
+    a = b > a ? b : a;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) a = keep_larger(a, d, (lane & d) == 0);
+    return a;
+}
+// The 32 largest of the lists of the CTA's first `n` warps (a power of two), in warp 0.
+template <typename K>
+__device__ __forceinline__ K merged_over_warps(K x, int n, K (*scratch)[32]) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int half = n >> 1; half > 0; half >>= 1) {
+        __syncthreads();
+        if (warp >= half && warp < 2 * half) scratch[warp][lane] = x;
+        __syncthreads();
+        if (warp < half) x = merged(x, scratch[warp + half][lane]);
     }
-    if (bad) s = u = NAN;
+    return x;
+}
+
+// s = sum e^(x - m), u = sum (x - m) e^(x - m), relative to m.
+struct Sums {
+    float m = kLowest, s = 0.f, u = 0.f;
+    __device__ __forceinline__ void move_to(float mn) {  // mn >= m
+        const float d = max_nan(m - mn, kFar);
+        const float e = ex2_approx(d * kLog2e);
+        u = (u + d * s) * e;
+        s *= e;
+        m = mn;
+    }
+    __device__ __forceinline__ void add(Sums o) {
+        const float mn = max_nan(m, o.m);
+        move_to(mn);
+        o.move_to(mn);
+        s += o.s;
+        u += o.u;
+    }
+};
+
+// 16 bytes of a row as fp32.
+template <bool kF32>
+struct Vec {
+    static constexpr int kN = kF32 ? 4 : 8;
+    float x[kN];
+};
+
+// One row, or one CTA's share of it, as vectors of 16 aligned bytes; the first and the last may lie
+// partly outside the row, and then only what is inside is read.
+template <bool kF32>
+struct Row {
+    static constexpr int kN = Vec<kF32>::kN;
+    const char* base;  // of vector 0
+    int skip;          // elements of vector 0 before the row
+    int V;
+    __device__ __forceinline__ Row(const void* x, long long first, int V_) : V(V_) {
+        const char* p = static_cast<const char*>(x) + first * (kF32 ? 4 : 2);
+        const int off = (int)(reinterpret_cast<uintptr_t>(p) & 15);
+        skip = off / (kF32 ? 4 : 2);
+        base = p - off;
+    }
+    __device__ __forceinline__ int vectors() const { return (V + skip + kN - 1) / kN; }
+    __device__ __forceinline__ int id(int v, int e) const { return v * kN + e - skip; }
+    __device__ __forceinline__ bool inside(int v) const { return id(v, 0) >= 0 && id(v, kN - 1) < V; }
+    __device__ __forceinline__ uint4 load(int v) const { return __ldg(reinterpret_cast<const uint4*>(base) + v); }
+    __device__ __forceinline__ static Vec<kF32> unpack(uint4 y) {
+        Vec<kF32> r;
+        const uint32_t w[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (kF32) r.x[i] = __uint_as_float(w[i]);
+            else r.x[2 * (i & 3) % kN] = __uint_as_float(w[i] << 16), r.x[(2 * (i & 3) + 1) % kN] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+        return r;
+    }
+    // a vector at either end, -inf where it is outside
+    __device__ __forceinline__ Vec<kF32> edge(int v) const {
+        Vec<kF32> r;
+#pragma unroll
+        for (int e = 0; e < kN; ++e) r.x[e] = id(v, e) >= 0 && id(v, e) < V ? logit<kF32>(base, (long long)v * kN + e) : -INFINITY;
+        return r;
+    }
+};
+
+struct Smem {
+    unsigned long long list[kWarps][32];
+    Sums sums[kWarps];
+    Sums total;                         // of this CTA, for the cluster
+    unsigned long long best[32];        // its alternatives
+    float threshold;
+};
+
+// A cluster of `split` CTAs per row (one, unless the rows are too few to fill the GPU).  One pass
+// gives the sums and every thread's largest logit.  The k-th largest of these is no larger than the
+// row's k-th largest logit, so the alternatives all lie with threads whose largest reaches it: about k of
+// 512, whose logits alone are read again (from L2).  Bound by the read: at V = 100352 fp32 a CTA
+// has 400 KB to read per row and spends about 9 instructions a logit.
+template <bool kF32>
+__global__ void __launch_bounds__(kThreads, 3) row_kernel(const Params p) {
+    pdl_enter();
+    __shared__ Smem sm;
+    constexpr int kN = Vec<kF32>::kN;
+    constexpr int kBatch = 16 / kN;  // vectors at a time
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int row = (int)(blockIdx.x / (unsigned)p.split), rank = (int)(blockIdx.x % (unsigned)p.split);
+    const Row<kF32> r(p.x, (long long)row * p.ld, p.V);
+    const int vectors = r.vectors();
+    const int begin = (int)((long long)vectors * rank / p.split), end = (int)((long long)vectors * (rank + 1) / p.split);
+
+    Sums a;
+    float most = -INFINITY;  // this thread's largest logit, and whether it saw a NaN
+    bool odd = false;
+    auto take = [&](const float(&x)[16]) {
+        float top[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top[i] = max_nan(max_nan(x[4 * i], x[4 * i + 1]), max_nan(x[4 * i + 2], x[4 * i + 3]));
+        const float t = max_nan(max_nan(top[0], top[1]), max_nan(top[2], top[3]));
+        odd |= t != t;
+        most = fmaxf(most, t);
+        a.move_to(max_nan(a.m, t));
+        float s[4] = {0.f, 0.f, 0.f, 0.f}, u[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float d = max_nan(x[i] - a.m, kFar);
+            const float e = ex2_approx(d * kLog2e);
+            s[i & 3] += e;
+            u[i & 3] = fmaf(d, e, u[i & 3]);
+        }
+        a.s += (s[0] + s[1]) + (s[2] + s[3]);
+        a.u += (u[0] + u[1]) + (u[2] + u[3]);
+    };
+    // whole batches; the edges and what is left behind the last batch are taken below
+    const int lo = begin + (r.inside(begin) ? 0 : 1), hi = end - (end > begin && r.inside(end - 1) ? 0 : 1);
+    int v = lo + threadIdx.x;
+    for (; v + (kBatch - 1) * kThreads < hi; v += kBatch * kThreads) {
+        uint4 y[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) y[i] = r.load(v + i * kThreads);
+        float x[16];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const Vec<kF32> z = Row<kF32>::unpack(y[i]);
+#pragma unroll
+            for (int e = 0; e < kN; ++e) x[i * kN + e] = z.x[e];
+        }
+        take(x);
+    }
+    {
+        uint4 y[kBatch];
+        const uint32_t none = kF32 ? 0xff800000u : 0xff80ff80u;  // -inf
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) y[i] = v + i * kThreads < hi ? r.load(v + i * kThreads) : make_uint4(none, none, none, none);
+        if (v < hi) {
+            float x[16];
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                const Vec<kF32> z = Row<kF32>::unpack(y[i]);
+#pragma unroll
+                for (int e = 0; e < kN; ++e) x[i * kN + e] = z.x[e];
+            }
+            take(x);
+        }
+        // thread 0 takes the share's first vector and thread 1 its last, where they cross the row's ends
+        const bool first = threadIdx.x == 0 && lo > begin, last = threadIdx.x == 1 && hi < end && hi >= lo;
+        if (first || last) {
+            const Vec<kF32> z = r.edge(first ? begin : hi);
+            float x[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[e] = e < kN ? z.x[e % kN] : -INFINITY;
+            take(x);
+        }
+    }
+
+    if (p.top > 0) {
+        // a logit that the row's k-th largest reaches
+        const uint32_t k = merged_over_warps<uint32_t>(sorted(order_bits(most)), kWarps, reinterpret_cast<uint32_t(*)[32]>(sm.list));
+        __syncthreads();
+        if (threadIdx.x == p.top - 1) sm.threshold = from_order_bits(k);
+        __syncthreads();
+        const float threshold = sm.threshold;
+        unsigned long long list = 0, least = 0;  // this warp's alternatives, and its k-th
+        uint32_t todo = __ballot_sync(0xffffffffu, odd || most >= threshold);
+        while (todo) {  // the warp reads one thread's vectors again, a lane each
+            const int who = warp * 32 + __ffs(todo) - 1;
+            todo &= todo - 1;
+            const int extra = who == 0 && lo > begin ? begin : who == 1 && hi < end && hi >= lo ? hi : -1;
+            const int n = (hi - lo - who + kThreads - 1) / kThreads + (extra >= 0 ? 1 : 0);
+            for (int i0 = 0; i0 < n; i0 += 32) {
+                const int i = i0 + lane;
+                const int mine = i >= n ? -1 : extra >= 0 && i == n - 1 ? extra : lo + who + i * kThreads;
+                Vec<kF32> z;
+#pragma unroll
+                for (int e = 0; e < kN; ++e) z.x[e] = -INFINITY;
+                if (mine >= 0) z = mine == extra ? r.edge(mine) : Row<kF32>::unpack(r.load(mine));
+#pragma unroll
+                for (int e = 0; e < kN; ++e) {
+                    const int id = r.id(mine, e);
+                    const bool in = mine >= 0 && id >= 0 && id < p.V && (z.x[e] >= threshold || threshold == -INFINITY);
+                    const unsigned long long key = in ? order_key(z.x[e], id) : 0ull;
+                    if (__any_sync(0xffffffffu, key > least)) {
+                        list = merged(list, sorted(key));
+                        least = __shfl_sync(0xffffffffu, list, p.top - 1);
+                    }
+                }
+            }
+        }
+        list = merged_over_warps(list, kWarps, sm.list);
+        if (warp == 0) sm.best[lane] = list;
+    }
+
+    // join the threads' sums, the warps', the cluster's
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-        const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o),
-                    u2 = __shfl_xor_sync(0xffffffffu, u, o);
-        const bool nan = s != s || s2 != s2;
-        merge(m, s, u, m2, s2, u2);
-        if (nan) s = u = NAN;
+        Sums b;
+        b.m = __shfl_xor_sync(0xffffffffu, a.m, o);
+        b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
+        b.u = __shfl_xor_sync(0xffffffffu, a.u, o);
+        a.add(b);
     }
-    if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = m, ss[threadIdx.x >> 5] = s, su[threadIdx.x >> 5] = u;
+    if (lane == 0) sm.sums[warp] = a;
     __syncthreads();
-    m = sm[0], s = ss[0], u = su[0];
-    for (int w = 1; w < kThreads / 32; ++w) {
-        const bool nan = s != s || ss[w] != ss[w];
-        merge(m, s, u, sm[w], ss[w], su[w]);
-        if (nan) s = u = NAN;
-    }
-    const bool empty = s == 0.f;
-    const float ls = logf(s);
-    const float lse = empty ? -INFINITY : m + ls;
     if (threadIdx.x == 0) {
-        const long long t = target_of(p.targets, p.targets64, row);
-        float lp = 0.f;
-        if (t >= 0 && t < p.V) lp = empty ? -INFINITY : (logit<kF32>(p.x, base + t) - m) - ls;
-        if (p.log_prob) p.log_prob[row] = lp;
-        if (p.entropy) p.entropy[row] = empty ? 0.f : ls - u / s;
-        if (p.lse) p.lse[row] = lse;
-    }
-    unsigned long long last = ~0ull;
-    for (int k = 0; k < p.top; ++k) {
-        unsigned long long best = 0;
-        for (int j = threadIdx.x; j < p.V; j += kThreads) {
-            const unsigned long long key = order_key(logit<kF32>(p.x, base + j), j);
-            if (key < last && key > best) best = key;
-        }
+        Sums b = sm.sums[0];
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const unsigned long long other = __shfl_xor_sync(0xffffffffu, best, o);
-            best = other > best ? other : best;
-        }
-        __syncthreads();
-        if ((threadIdx.x & 31) == 0) sk[threadIdx.x >> 5] = best;
-        __syncthreads();
-        for (int w = 0; w < kThreads / 32; ++w) best = sk[w] > best ? sk[w] : best;
-        last = best;
+        for (int w = 1; w < kWarps; ++w) b.add(sm.sums[w]);
+        sm.total = b;
+    }
+    namespace cg = cooperative_groups;
+    cg::cluster_group cluster = cg::this_cluster();
+    if (p.split > 1) cluster.sync();
+    else __syncthreads();
+    if (rank == 0) {
+        Sums b = sm.total;
+        for (int c = 1; c < p.split; ++c) b.add(cluster.map_shared_rank(&sm, c)->total);
+        const bool empty = b.s == 0.f;  // every logit is -inf
+        const float ls = logf(b.s);
         if (threadIdx.x == 0) {
-            const int id = 0x7fffffff - (int)(uint32_t)best;
-            p.top_ids[(long long)row * p.top + k] = id;
-            p.top_log_probs[(long long)row * p.top + k] = empty ? -INFINITY : (logit<kF32>(p.x, base + id) - m) - ls;
+            const long long t = target_of(p.targets, p.targets64, row);
+            float lp = 0.f;
+            if (t >= 0 && t < p.V) lp = empty ? -INFINITY : (logit<kF32>(p.x, (long long)row * p.ld + t) - b.m) - ls;
+            if (p.log_prob) p.log_prob[row] = lp;
+            if (p.entropy) p.entropy[row] = empty ? 0.f : ls - b.u / b.s;
+            if (p.lse) p.lse[row] = empty ? -INFINITY : b.m + ls;
+        }
+        if (p.top > 0) {
+            unsigned long long list = warp < p.split ? (p.split > 1 ? cluster.map_shared_rank(&sm, warp)->best[lane] : sm.best[lane]) : 0ull;
+            list = merged_over_warps(list, kMaxCluster, sm.list);
+            if (threadIdx.x < p.top) {
+                const float x = from_order_bits((uint32_t)(list >> 32));
+                p.top_ids[(long long)row * p.top + lane] = 0x7fffffff - (int)(uint32_t)list;
+                p.top_log_probs[(long long)row * p.top + lane] = empty ? -INFINITY : (x - b.m) - ls;
+            }
         }
     }
+    if (p.split > 1) cluster.sync();  // no CTA leaves while its shared memory is read
 }
 
-template <bool kF32>
-__global__ void __launch_bounds__(kThreads) grad_kernel(const GradParams p) {
+constexpr int kGradThreads = 256;
+constexpr int kGradVectors = 4;  // 16-byte vectors per thread
+
+// One pass: a CTA takes a stretch of a row.  kAligned: the rows of both arrays start equally far from a
+// 16-byte boundary, so vectors of one are vectors of the other; else element by element.
+template <bool kF32, bool kAligned>
+__global__ void __launch_bounds__(kGradThreads) grad_kernel(const GradParams p) {
     pdl_enter();
-    const int row = blockIdx.x;
+    const int row = (int)(blockIdx.x / (unsigned)p.chunks), chunk = (int)(blockIdx.x % (unsigned)p.chunks);
     const long long base = (long long)row * p.ld, dbase = (long long)row * p.dx_ld;
     const long long t = target_of(p.targets, p.targets64, row);
     const bool has = t >= 0 && t < p.V;
     const float g = has && p.d_log_prob ? p.d_log_prob[row] : 0.f;
     const float h = p.d_entropy ? p.d_entropy[row] : 0.f;
     const float lse = p.lse[row], ent = p.entropy ? p.entropy[row] : 0.f;
-    for (int j = threadIdx.x; j < p.V; j += kThreads) {
-        const float x = logit<kF32>(p.x, base + j);
-        float d = 0.f;
-        if (lse != -INFINITY) {
-            const float lp = x - lse;
-            if (x != -INFINITY) d = -expf(lp) * (g + h * (lp + ent));
-            if (j == t) d += g;
-        }
+    const bool empty = lse == -INFINITY;
+    auto grad = [&](float x, int j) {
+        const float lp = max_nan(x - lse, kFar);  // (at -inf too: no weight, and no inf * 0)
+        float d = -ex2_approx(lp * kLog2e) * fmaf(h, lp + ent, g);
+        if (j == t) d += g;
+        return empty ? 0.f : d;
+    };
+    auto put = [&](int j, float d) {
         if (kF32) static_cast<float*>(p.dx)[dbase + j] = d;
         else static_cast<__nv_bfloat16*>(p.dx)[dbase + j] = __float2bfloat16_rn(d);
+    };
+    constexpr int kN = Vec<kF32>::kN;
+    constexpr int kPer = kGradThreads * kGradVectors;  // vectors per CTA
+    if (!kAligned) {
+        const int j0 = chunk * kPer * kN, j1 = min(p.V, j0 + kPer * kN);
+        for (int j = j0 + threadIdx.x; j < j1; j += kGradThreads) put(j, grad(logit<kF32>(p.x, base + j), j));
+        return;
+    }
+    const Row<kF32> r(p.x, base, p.V);
+    char* out = static_cast<char*>(p.dx) + (dbase - r.skip) * (kF32 ? 4 : 2);
+    const int vectors = r.vectors();
+    uint4 y[kGradVectors];
+#pragma unroll
+    for (int i = 0; i < kGradVectors; ++i) {
+        const int v = chunk * kPer + i * kGradThreads + threadIdx.x;
+        // (not __ldg: the gradient may go where the logits are)
+        if (v < vectors && r.inside(v)) y[i] = *(reinterpret_cast<const uint4*>(r.base) + v);
+    }
+#pragma unroll
+    for (int i = 0; i < kGradVectors; ++i) {
+        const int v = chunk * kPer + i * kGradThreads + threadIdx.x;
+        if (v >= vectors) continue;
+        if (r.inside(v)) {
+            const Vec<kF32> z = Row<kF32>::unpack(y[i]);
+            float d[kN];
+#pragma unroll
+            for (int e = 0; e < kN; ++e) d[e] = grad(z.x[e], r.id(v, e));
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = kF32 ? __float_as_uint(d[e % kN]) : pack_bf16x2(d[2 * e % kN], d[(2 * e + 1) % kN]);
+            reinterpret_cast<uint4*>(out)[v] = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+            for (int e = 0; e < kN; ++e) {
+                const int j = r.id(v, e);
+                if (j >= 0 && j < p.V) put(j, grad(logit<kF32>(p.x, base + j), j));
+            }
+        }
     }
 }
 

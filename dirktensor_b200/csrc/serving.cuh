@@ -352,11 +352,27 @@ int dt_token_log_probs(const void* logits, int logits_f32, long long ld, int N, 
     int dev;
     DT_TRY(prepare_device(&dev));
     dt::logprobs::Params p{logits, ld, N, V, targets, targets_int64 ? 1 : 0, top, log_prob, entropy, lse, top_ids,
-                           top_log_probs};
-    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    const dim3 grid((unsigned)N), block(dt::logprobs::kThreads);
-    return logits_f32 ? launch_pdl(dt::logprobs::row_kernel<true>, grid, block, 0, st, p)
-                      : launch_pdl(dt::logprobs::row_kernel<false>, grid, block, 0, st, p);
+                           top_log_probs, 1};
+    // a cluster per row while that leaves SMs idle and every thread a batch of its own
+    while (p.split < dt::logprobs::kMaxCluster && (long long)N * p.split * 2 <= 2 * kPlanSms &&
+           V >= p.split * 2 * dt::logprobs::kThreads * 8)
+        p.split *= 2;
+    if ((long long)N * p.split > 0x7fffffffll) return fail(DT_ERR_INVALID_ARGUMENT, "N is too large");
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = DT_PDL;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)p.split;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(N * p.split));
+    cfg.blockDim = dim3(dt::logprobs::kThreads);
+    cfg.stream = reinterpret_cast<cudaStream_t>(stream);
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    DT_CUDA(cudaLaunchKernelEx(&cfg, logits_f32 ? dt::logprobs::row_kernel<true> : dt::logprobs::row_kernel<false>, p));
+    return DT_OK;
 }
 
 int dt_token_log_probs_bwd(const void* logits, int logits_f32, long long ld, int N, int V, const void* targets,
@@ -375,12 +391,20 @@ int dt_token_log_probs_bwd(const void* logits, int logits_f32, long long ld, int
     if (d_entropy && !entropy) return fail(DT_ERR_INVALID_ARGUMENT, "d_entropy needs entropy");
     int dev;
     DT_TRY(prepare_device(&dev));
+    namespace lp = dt::logprobs;
     dt::logprobs::GradParams p{logits, ld, N, V, targets, targets_int64 ? 1 : 0, lse, entropy, d_log_prob, d_entropy,
-                               d_logits, d_ld};
+                               d_logits, d_ld, 1};
+    const int elem = logits_f32 ? 4 : 2;
+    // (one vector more than V has: a row may start inside one)
+    const long long vectors = ((long long)V * elem + 15) / 16 + 1;
+    p.chunks = (int)((vectors + lp::kGradThreads * lp::kGradVectors - 1) / (lp::kGradThreads * lp::kGradVectors));
+    if ((long long)N * p.chunks > 0x7fffffffll) return fail(DT_ERR_INVALID_ARGUMENT, "N * V is too large");
+    const bool aligned = ((reinterpret_cast<uintptr_t>(logits) ^ reinterpret_cast<uintptr_t>(d_logits)) & 15) == 0 &&
+                         ((ld - d_ld) * elem) % 16 == 0;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    const dim3 grid((unsigned)N), block(dt::logprobs::kThreads);
-    return logits_f32 ? launch_pdl(dt::logprobs::grad_kernel<true>, grid, block, 0, st, p)
-                      : launch_pdl(dt::logprobs::grad_kernel<false>, grid, block, 0, st, p);
+    const dim3 grid((unsigned)(N * p.chunks)), block(lp::kGradThreads);
+    if (logits_f32) return launch_pdl(aligned ? lp::grad_kernel<true, true> : lp::grad_kernel<true, false>, grid, block, 0, st, p);
+    return launch_pdl(aligned ? lp::grad_kernel<false, true> : lp::grad_kernel<false, false>, grid, block, 0, st, p);
 }
 
 }  // extern "C"
