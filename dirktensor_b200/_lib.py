@@ -152,7 +152,7 @@ SIGNATURES = {
     "dt_kv_cache_read": (_I, [_P, _P, _P, _I, _P, _LL, _I, _P, _P, _I, _I, _P]),
     "dt_cache_attn_workspace_bytes": (_SZ, [_I] * 7),
     "dt_cache_attn_fwd": (_I, [_P, _P, _LL, _LL, _I, _P, _P, _P, _P, _LL, _I, _P, _P, _I, _I, _I, _F, _P, _SZ, _P]),
-    "dt_prefix_attn_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I]),
+    "dt_prefix_attn_workspace_bytes": (_SZ, [_I] * 8),
     "dt_prefix_attn_fwd": (_I, [_P, _P, _LL, _LL, _I, _P, _P, _P, _P, _I, _P, _LL, _I, _P, _P, _I, _I, _I, _F, _P, _SZ,
                                 _P]),
     "dt_token_log_probs": (_I, [_P, _I, _LL, _I, _I, _P, _I, _I, _P, _P, _P, _P, _P, _P]),

@@ -28,6 +28,7 @@
 #include "kv_cache.cuh"
 #include "logprobs.cuh"
 #include "model.cuh"
+#include "prefix_attn.cuh"
 #include "prologue.cuh"
 
 namespace dt {

@@ -1,0 +1,570 @@
+// Attention of a whole batch's new tokens over the keys of a prefix that all its sequences share,
+// read once: the queries of all sequences that read a K/V head (B * T * group rows) are one matrix, so
+// both products are tensor-core matrix products (tcgen05, accumulators in TMEM), where the same
+// keys read per sequence would be as many vector products.
+//
+// A CTA takes up to 256 (or 128) query rows of one K/V head and a stretch of the prefix's 128-key tiles:
+//   warps 0-3, 4-7  softmax, one thread per row (TMEM lane).  With more than 128 rows the two
+//                   warpgroups take 128 rows each and both see every tile; otherwise they take every
+//                   other tile of the same rows, as two parts that are joined at the end;
+//   warps 8-11      convert: codes from global memory, as fp16 into the 128-byte-swizzled tiles that
+//                   the MMAs read (K and V, two buffers each), with the next tile's codes in registers;
+//   warp 12         issues the MMAs (one thread) and owns TMEM.
+// TMEM (512 columns): S0 S1 O0 O1 of 128 each; P_i, fp16 pairs, overwrites S_i and feeds the second product
+// from there.  The issue order PV_i(t), S_i(next) keeps the tensor core on one warpgroup's
+// tile while the other does its softmax.
+//
+// Codes are exact in fp16, and so are bf16 queries, each row scaled by a power of two into its
+// range; fp32 queries go in as fp16(q) and the rest, as two products into one accumulator.  Scales stay out of
+// the operands: S is multiplied by k_scale (and the row's factor) in fp32, and the weights p by v_scale before they
+// are rounded to fp16 (once, at 2^-11 below a bf16 result's own 2^-8; for fp32 queries as two numbers
+// again).  f, a power of two that follows the largest v_scale so far, keeps p * v_scale * f
+// below 2^15; a change of it rescales O as a change of the running maximum does.
+#pragma once
+#include "cache_attn.cuh"
+
+namespace dt {
+namespace prefix_attn {
+
+using cache_attn::half_pair;
+using cache_attn::kLog2e;
+using cache_attn::pow2;
+using cache_attn::exponent;
+
+constexpr int kD = 128;
+constexpr int kBM = 128;                   // rows of a Q tile
+constexpr int kBN = 128;                   // keys of a tile
+constexpr int kTileBytes = 128 * kD * 2;   // fp16
+constexpr int kHalfBytes = kTileBytes / 2; // 64 dims: one swizzle span
+constexpr int kThreads = 416;
+constexpr int kConvWarps = 4;
+constexpr float kGrow = 8.f;               // log2 units, as in flash_fwd.cuh
+
+struct Params {
+    cache_attn::Params a;
+    int rows;     // B * T * group
+    int blocks;   // of rows: blocks of 256, or of 128 with `pairs`
+    int pairs;    // 1: one Q tile, the warpgroups take every other key tile; 0: two Q tiles
+    int split;    // stretches of the prefix
+    int tiles;    // of the prefix
+};
+
+struct __align__(1024) Smem {
+    uint8_t q[2][kTileBytes];   // the two Q tiles; or fp16(q) of one and the rest
+    uint8_t k[2][kTileBytes];
+    uint8_t v[2][kTileBytes];
+    float ks[4][kBN];           // of tile t: at t & 3
+    float vs[4][kBN];           // v_scale * f
+    float f[4];
+    uint32_t hidden[4][4];      // keys past the prefix, or on a page that does not exist
+    float factor[2][kBM];       // from S back to scores in log2 units (k_scale apart)
+    float m[kBM], l[kBM], mx[kBM];  // of the second warpgroup, for the first (pairs)
+    uint64_t q_full;
+    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
+    uint64_t s_full[2], p_full[2], o_full[2];
+    uint64_t mma_done;
+    uint32_t tmem_base;
+};
+
+enum : unsigned { kSiteQ = 0x21, kSiteKFull, kSiteKEmpty, kSiteVFull, kSiteVEmpty, kSiteS, kSiteP, kSiteO, kSiteDone };
+
+// tcgen05 instruction descriptor: fp16 A and B, fp32 accumulator.
+constexpr uint32_t idesc_f16(int M, int N, int b_mn_major) {
+    return (1u << 4) | ((uint32_t)b_mn_major << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
+__device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// A 16-byte piece of codes (dims 16 piece ..+15 of row r) as fp16 into a swizzled tile.
+template <int kFmt>
+__device__ __forceinline__ void put_piece(uint32_t tile, int r, int piece, uint4 codes) {
+    const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
+    uint32_t h[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) cache_attn::pairs_of_word<kFmt>(w[i], h[2 * i], h[2 * i + 1]);
+    const uint32_t base = tile + (uint32_t)(piece >> 2) * kHalfBytes + (uint32_t)r * 128;
+    const uint32_t c = 2 * (piece & 3);
+    // the lanes of the second half store their chunks in the other order: no bank conflicts
+    const bool swap = piece >= 4;
+    const uint32_t first = base + (((c + (swap ? 1u : 0u)) ^ (uint32_t)(r & 7)) << 4);
+    const uint32_t second = base + (((c + (swap ? 0u : 1u)) ^ (uint32_t)(r & 7)) << 4);
+    st_shared_v4(first, swap ? h[4] : h[0], swap ? h[5] : h[1], swap ? h[6] : h[2], swap ? h[7] : h[3]);
+    st_shared_v4(second, swap ? h[0] : h[4], swap ? h[1] : h[5], swap ? h[2] : h[6], swap ? h[3] : h[7]);
+}
+
+template <int kFmt, bool kF32>
+__global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const Params pp) {
+    pdl_enter();
+    const cache_attn::Params& p = pp.a;
+    extern __shared__ uint8_t smem_raw[];
+    Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    const int part = (int)(blockIdx.x % (unsigned)pp.split);
+    const int block = (int)(blockIdx.x / (unsigned)pp.split) % pp.blocks;
+    const int hk = (int)(blockIdx.x / (unsigned)pp.split) / pp.blocks;
+    const int row0 = block * (pp.pairs ? kBM : 2 * kBM);
+    const int t0 = (int)((long long)pp.tiles * part / pp.split), t1 = (int)((long long)pp.tiles * (part + 1) / pp.split);
+    const int n = t1 - t0;  // at least one: split <= tiles
+    const bool second_rows = !pp.pairs && row0 + kBM < pp.rows;
+    // steps of warpgroup i: its s-th one is tile s, or 2 s + i
+    const int steps[2] = {pp.pairs ? (n + 1) / 2 : n, pp.pairs ? n / 2 : (second_rows ? n : 0)};
+
+    if (threadIdx.x == 0) {
+        mbar_init(&sm.q_full, 8);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sm.k_full[i], kConvWarps);
+            mbar_init(&sm.v_full[i], kConvWarps);
+            mbar_init(&sm.k_empty[i], 1);
+            mbar_init(&sm.v_empty[i], 1);
+            mbar_init(&sm.s_full[i], 1);
+            mbar_init(&sm.p_full[i], 4);
+            mbar_init(&sm.o_full[i], 1);
+        }
+        mbar_init(&sm.mma_done, 1);
+        fence_mbar_init();
+    }
+    if (warp == 12) {
+        tmem_alloc(&sm.tmem_base, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sm.tmem_base;
+
+    if (warp >= 8 && warp < 12) {
+        // ------------------------------ convert -----------------------------
+        const int cw = warp - 8;
+        const int shift = p.c.page_shift, in_page = (1 << shift) - 1;
+        // this warp's 32 keys of a tile are two groups of 16, each on one page
+        auto page_of = [&](int tile, int g) {
+            const int key = tile * kBN + cw * 32 + g * 16;
+            const int page = key < p.prefix_len ? __ldg(p.prefix_pages + (key >> shift)) : -1;
+            return page >= 0 && page < p.c.pages ? page : -1;
+        };
+        // lane: piece lane & 7 of rows 4 i + lane / 8
+        auto load = [&](const uint8_t* codes, int tile, const int (&page)[2], uint4 (&x)[8]) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int r = 4 * i + (lane >> 3);
+                const int key = tile * kBN + cw * 32 + r;
+                const int pg = page[i >> 2];
+                x[i] = make_uint4(0, 0, 0, 0);  // hidden keys: zeros
+                if (pg >= 0 && key < p.prefix_len) {
+                    const long long row = (((long long)pg * p.c.heads + hk) << shift) + (key & in_page);
+                    x[i] = __ldg(reinterpret_cast<const uint4*>(codes + row * kD) + (lane & 7));
+                }
+            }
+        };
+        auto put = [&](uint8_t* tile, const uint4 (&x)[8]) {
+            const uint32_t base = smem_u32(tile);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) put_piece<kFmt>(base, cw * 32 + 4 * i + (lane >> 3), lane & 7, x[i]);
+        };
+        float f = pow2(100);
+        // the scales of a tile, four keys a lane of the first of these warps
+        auto scales = [&](int tile) {
+            if (cw != 0) return;
+            float k[4], v[4];
+            uint32_t hide = 0;
+            float most = 0.f;
+            const int key = tile * kBN + 4 * lane;
+            const int page = key < p.prefix_len ? __ldg(p.prefix_pages + (key >> shift)) : -1;
+            const bool ok = page >= 0 && page < p.c.pages;
+            const long long row = ok ? (((long long)page * p.c.heads + hk) << shift) + (key & in_page) : 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const bool see = ok && key + e < p.prefix_len;
+                k[e] = see ? __ldg(p.c.ks + row + e) : 0.f;
+                v[e] = see ? __ldg(p.c.vs + row + e) : 0.f;
+                if (!see) hide |= 1u << e;
+                most = fmaxf(most, v[e]);
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+            // p <= 2^8 (the lazy maximum), so p * v_scale * f < 2^15 with f = 2^(6 - exponent)
+            f = fminf(f, pow2(min(max(6 - exponent(most), -120), 100)));
+            const int at = tile - t0;
+            *reinterpret_cast<float4*>(&sm.ks[at & 3][4 * lane]) = make_float4(k[0], k[1], k[2], k[3]);
+            *reinterpret_cast<float4*>(&sm.vs[at & 3][4 * lane]) = make_float4(v[0] * f, v[1] * f, v[2] * f, v[3] * f);
+            // 4 bits from each of 8 lanes make a word
+            uint32_t word = hide << (4 * (lane & 7));
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) word |= __shfl_xor_sync(0xffffffffu, word, o);
+            if ((lane & 7) == 0) sm.hidden[at & 3][lane >> 3] = word;
+            if (lane == 0) sm.f[at & 3] = f;
+        };
+        bool ok = true;
+        uint4 xk[8], xv[8];
+        int pk[2] = {page_of(t0, 0), page_of(t0, 1)};
+        int pv[2] = {pk[0], pk[1]};  // pages of the tile whose V comes next
+        load(p.c.k, t0, pk, xk);
+        load(p.c.v, t0, pk, xv);
+        int next[2] = {page_of(t0 + 1, 0), page_of(t0 + 1, 1)};
+        // order: K0, K1, V0, K2, V1, ...
+        for (int j = 0; ok && j <= n; ++j) {
+            if (j < n) {  // K of tile j
+                const int s = j & 1;
+                if (j >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&sm.k_empty[s], ((j >> 1) - 1) & 1, kSiteKEmpty));
+                if (!ok) break;
+                scales(t0 + j);
+                put(sm.k[s], xk);
+                fence_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.k_full[s]);
+                if (j + 1 < n) load(p.c.k, t0 + j + 1, next, xk);
+            }
+            if (j >= 1) {  // V of tile j - 1
+                const int i = j - 1, s = i & 1;
+                if (i >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&sm.v_empty[s], ((i >> 1) - 1) & 1, kSiteVEmpty));
+                if (!ok) break;
+                put(sm.v[s], xv);
+                fence_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.v_full[s]);
+                if (j < n) {
+                    pv[0] = pk[0], pv[1] = pk[1];
+                    load(p.c.v, t0 + j, pv, xv);
+                }
+            }
+            // pk: pages of tile j + 1, whose V is loaded next; next: of tile j + 2
+            pk[0] = next[0], pk[1] = next[1];
+            next[0] = page_of(t0 + j + 2, 0), next[1] = page_of(t0 + j + 2, 1);
+        }
+    } else if (warp == 12) {
+        // ------------------------------ MMA issue ---------------------------
+        if (lane == 0) {
+            constexpr uint32_t idesc_qk = idesc_f16(kBM, kBN, 0);
+            constexpr uint32_t idesc_pv = idesc_f16(kBM, kD, 1);
+            bool ok = mbar_wait(&sm.q_full, 0, kSiteQ);
+            int k_seen = 0, v_seen = 0;  // tiles whose K and V have been waited for
+            auto want_k = [&](int t) {
+                for (; ok && k_seen <= t; ++k_seen) ok = mbar_wait(&sm.k_full[k_seen & 1], (k_seen >> 1) & 1, kSiteKFull);
+            };
+            auto want_v = [&](int t) {
+                for (; ok && v_seen <= t; ++v_seen) ok = mbar_wait(&sm.v_full[v_seen & 1], (v_seen >> 1) & 1, kSiteVFull);
+            };
+            auto issue_s = [&](int i, int t) {
+                const uint32_t k = smem_u32(sm.k[t & 1]);
+                const uint32_t q = smem_u32(sm.q[0]) + (pp.pairs ? 0u : (uint32_t)i * kTileBytes);
+#pragma unroll
+                for (int half = 0; half < (kF32 ? 2 : 1); ++half)
+#pragma unroll
+                    for (int kk = 0; kk < kD / 16; ++kk) {
+                        const uint32_t off = (kk >> 2) * kHalfBytes + (kk & 3) * 32;
+                        umma_ss(tmem + i * 128, umma_desc_sw128(q + half * kTileBytes + off, 16, 1024),
+                                umma_desc_sw128(k + off, 16, 1024), idesc_qk, kk > 0 || half > 0 ? 1u : 0u);
+                    }
+                umma_commit(&sm.s_full[i]);
+            };
+            auto issue_pv = [&](int i, int t, bool add) {
+                const uint32_t v = smem_u32(sm.v[t & 1]);
+#pragma unroll
+                for (int half = 0; half < (kF32 ? 2 : 1); ++half)
+#pragma unroll
+                    for (int kk = 0; kk < kBN / 16; ++kk)
+                        umma_ts(tmem + 256 + i * 128, tmem + i * 128 + half * 64 + kk * 8,
+                                umma_desc_sw128(v + kk * 2048, kHalfBytes, 1024), idesc_pv, (add || kk > 0 || half > 0) ? 1u : 0u);
+            };
+            auto tile_of = [&](int i, int s) { return pp.pairs ? 2 * s + i : s; };
+            for (int i = 0; i < 2; ++i)
+                if (steps[i] > 0) {
+                    want_k(tile_of(i, 0));
+                    if (!ok) break;
+                    tc_fence_after();
+                    issue_s(i, tile_of(i, 0));
+                    if (pp.pairs || i == 1 || steps[1] == 0) umma_commit(&sm.k_empty[tile_of(i, 0) & 1]);
+                }
+            for (int s = 0; ok && s < steps[0]; ++s) {
+                for (int i = 0; ok && i < 2; ++i) {
+                    if (s >= steps[i]) continue;
+                    const int t = tile_of(i, s), tn = tile_of(i, s + 1);
+                    want_v(t);
+                    if (ok && s + 1 < steps[i]) want_k(tn);
+                    if (ok) ok = mbar_wait(&sm.p_full[i], s & 1, kSiteP);
+                    if (!ok) break;
+                    tc_fence_after();
+                    issue_pv(i, t, s > 0);
+                    const bool last_use = pp.pairs || i == 1 || steps[1] == 0;
+                    if (last_use) umma_commit(&sm.v_empty[t & 1]);
+                    if (s + 1 < steps[i]) {
+                        issue_s(i, tn);
+                        if (last_use) umma_commit(&sm.k_empty[tn & 1]);
+                    } else {
+                        umma_commit(&sm.o_full[i]);
+                    }
+                }
+            }
+            // all issued work is complete before TMEM is released
+            umma_commit(&sm.mma_done);
+            mbar_wait(&sm.mma_done, 0, kSiteDone);
+        }
+        __syncwarp();
+    } else {
+        // ------------------------------ softmax -----------------------------
+        const int i = warp >> 2;  // warpgroup
+        // The Q rows, a warp per row: 16 rows of each Q tile per warp.
+        {
+            const int qtiles = pp.pairs ? 1 : 2;
+            const int per_warp = kBM * qtiles / 8;
+            for (int rr = 0; rr < per_warp; rr += 8) {
+                float x[8][4];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    const int row = row0 + warp * per_warp + rr + u;
+                    const bool in = row < pp.rows;
+                    const int bt = in ? row / p.group : 0;
+                    const long long at = (long long)(bt / p.T) * p.q_batch + (long long)(bt % p.T) * p.q_token +
+                                         ((long long)hk * p.group + (in ? row % p.group : 0)) * kD + 4 * lane;
+                    if (kF32) {
+                        const float4 y = in ? __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + at))
+                                            : make_float4(0.f, 0.f, 0.f, 0.f);
+                        x[u][0] = y.x, x[u][1] = y.y, x[u][2] = y.z, x[u][3] = y.w;
+                    } else {
+                        const uint2 y = in ? __ldg(reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(p.q) + at))
+                                           : make_uint2(0, 0);
+                        x[u][0] = __uint_as_float(y.x << 16), x[u][1] = __uint_as_float(y.x & 0xffff0000u);
+                        x[u][2] = __uint_as_float(y.y << 16), x[u][3] = __uint_as_float(y.y & 0xffff0000u);
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    const int local = warp * per_warp + rr + u;  // row of the CTA
+                    uint32_t top = 0;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(x[u][e]) & 0x7fffffffu);
+                    top = __reduce_max_sync(0xffffffffu, top);
+                    const bool finite = top < 0x7f800000u;
+                    const int ex = finite ? max(exponent(__uint_as_float(top)), -100) : 0;
+                    // (a negative scale changes the queries' sign, so that factor stays positive)
+                    const float mul = finite ? (p.scale < 0.f ? -pow2(13 - ex) : pow2(13 - ex)) : 0.f;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[u][e] = finite ? x[u][e] * mul : 0.f;
+                    const int r = local & (kBM - 1);
+                    const int c = lane >> 1;
+                    const uint32_t addr = smem_u32(sm.q[pp.pairs ? 0 : local >> 7]) + (uint32_t)(c >> 3) * kHalfBytes + (uint32_t)r * 128 +
+                                          (((uint32_t)(c & 7) ^ (uint32_t)(r & 7)) << 4) + (uint32_t)(lane & 1) * 8;
+                    uint32_t hi0, hi1, lo0 = 0, lo1 = 0;
+                    if (kF32) {
+                        cache_attn::split_pair(x[u][0], x[u][1], hi0, lo0);
+                        cache_attn::split_pair(x[u][2], x[u][3], hi1, lo1);
+                        asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(addr + kTileBytes), "r"(lo0), "r"(lo1) : "memory");
+                    } else {
+                        hi0 = half_pair(x[u][0], x[u][1]);
+                        hi1 = half_pair(x[u][2], x[u][3]);
+                    }
+                    asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(addr), "r"(hi0), "r"(hi1) : "memory");
+                    if (lane == 0)
+                        sm.factor[pp.pairs ? 0 : local >> 7][r] =
+                            finite ? pow2(ex - 13) * fabsf(p.scale) * kLog2e : __uint_as_float(0x7fffffffu);
+                }
+            }
+            fence_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.q_full);
+            named_bar_sync(1, 256);  // factors of all rows
+        }
+        const int r = (warp & 3) * 32 + lane;
+        const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t tS = tmem + lane_off + i * 128;
+        const uint32_t tO = tmem + lane_off + 256 + i * 128;
+        const float factor = sm.factor[pp.pairs ? 0 : i][r];
+        float m = -INFINITY, l = 0.f, mx = -INFINITY, f = pow2(100);
+        bool ok = true;
+        for (int s = 0; s < steps[i]; ++s) {
+            // warp-uniform, since the step synchronises the warp
+            if (!__all_sync(0xffffffffu, mbar_wait_sleep(&sm.s_full[i], s & 1, kSiteS))) { ok = false; break; }
+            tc_fence_after();
+            const int at = (pp.pairs ? 2 * s + i : s) & 3;
+            const uint32_t hid[4] = {sm.hidden[at][0], sm.hidden[at][1], sm.hidden[at][2], sm.hidden[at][3]};
+            const bool some = (hid[0] | hid[1] | hid[2] | hid[3]) != 0u;
+            // first pass: the row's largest score
+            float top = -INFINITY;
+#pragma unroll
+            for (int cc = 0; cc < 4; ++cc) {
+                float x[32];
+                tmem_ld32(tS + cc * 32, x);
+                tmem_wait_ld();
+                float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int e = 0; e < 32; e += 4) {
+                    const float4 k = *reinterpret_cast<const float4*>(&sm.ks[at][cc * 32 + e]);
+                    float y[4];
+                    f2_unpack(f2_mul(f2_pack(x[e], x[e + 1]), f2_pack(k.x, k.y)), y[0], y[1]);
+                    f2_unpack(f2_mul(f2_pack(x[e + 2], x[e + 3]), f2_pack(k.z, k.w)), y[2], y[3]);
+                    if (some) {
+#pragma unroll
+                        for (int d = 0; d < 4; ++d)
+                            if ((hid[cc] >> (e + d)) & 1u) y[d] = -INFINITY;
+                    }
+                    best[(e >> 2) & 3] = fmax3(best[(e >> 2) & 3], fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
+                }
+                top = fmax3(top, fmaxf(best[0], best[1]), fmaxf(best[2], best[3]));
+            }
+            top *= factor;  // (-inf where every key is hidden; factor is not negative)
+            if (top != top) top = -INFINITY;  // (a row of NaN factor, or 0 * -inf: no maximum)
+            mx = fmaxf(mx, top);
+            const float fn = sm.f[at];
+            float by = 1.f;
+            if (top > m + kGrow) {
+                by = m == -INFINITY ? 1.f : ex2_approx(m - top);
+                l *= by;
+                m = top;
+            }
+            if (s > 0) {
+                if (fn != f) by *= fn / f;
+                if (__any_sync(0xffffffffu, by != 1.f)) {
+#pragma unroll 1
+                    for (int cc = 0; cc < 8; ++cc) {
+                        float o[16];
+                        tmem_ld16(tO + cc * 16, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) o[e] *= by;
+                        tmem_st16(tO + cc * 16, *reinterpret_cast<uint32_t(*)[16]>(o));
+                    }
+                }
+            }
+            f = fn;
+            // second pass: weights
+            const float m_safe = m == -INFINITY ? 0.f : m;
+            const uint64_t c2 = f2_pack(factor, factor), nm2 = f2_pack(-m_safe, -m_safe);
+            uint64_t sum2[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
+            uint32_t late[kF32 ? 64 : 1];
+#pragma unroll
+            for (int cc = 0; cc < 4; ++cc) {
+                float x[32];
+                tmem_ld32(tS + cc * 32, x);
+                tmem_wait_ld();
+                uint32_t hi[16], lo[kF32 ? 16 : 1];
+#pragma unroll
+                for (int e = 0; e < 32; e += 4) {
+                    const float4 k = *reinterpret_cast<const float4*>(&sm.ks[at][cc * 32 + e]);
+                    const float4 v = *reinterpret_cast<const float4*>(&sm.vs[at][cc * 32 + e]);
+                    float y[4];
+                    f2_unpack(f2_fma(f2_mul(f2_pack(x[e], x[e + 1]), f2_pack(k.x, k.y)), c2, nm2), y[0], y[1]);
+                    f2_unpack(f2_fma(f2_mul(f2_pack(x[e + 2], x[e + 3]), f2_pack(k.z, k.w)), c2, nm2), y[2], y[3]);
+                    if (some) {
+#pragma unroll
+                        for (int d = 0; d < 4; ++d)
+                            if ((hid[cc] >> (e + d)) & 1u) y[d] = -INFINITY;
+                    }
+                    const uint64_t p0 = f2_pack(ex2_approx(y[0]), ex2_approx(y[1])), p1 = f2_pack(ex2_approx(y[2]), ex2_approx(y[3]));
+                    sum2[0] = f2_add(sum2[0], p0);
+                    sum2[1] = f2_add(sum2[1], p1);
+                    float u[4];
+                    f2_unpack(f2_mul(p0, f2_pack(v.x, v.y)), u[0], u[1]);
+                    f2_unpack(f2_mul(p1, f2_pack(v.z, v.w)), u[2], u[3]);
+                    if (kF32) {
+                        cache_attn::split_pair(u[0], u[1], hi[e / 2], lo[kF32 ? e / 2 : 0]);
+                        cache_attn::split_pair(u[2], u[3], hi[e / 2 + 1], lo[kF32 ? e / 2 + 1 : 0]);
+                    } else {
+                        hi[e / 2] = half_pair(u[0], u[1]);
+                        hi[e / 2 + 1] = half_pair(u[2], u[3]);
+                    }
+                }
+                tmem_st16(tS + cc * 16, hi);  // columns below the ones still to be read
+                if (kF32) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) late[kF32 ? cc * 16 + e : 0] = lo[kF32 ? e : 0];
+                }
+            }
+            if (kF32) {  // the rests, at the columns whose scores have now been read
+#pragma unroll
+                for (int cc = 0; cc < 4; ++cc) tmem_st16(tS + 64 + cc * 16, *reinterpret_cast<uint32_t(*)[16]>(late + (kF32 ? cc * 16 : 0)));
+            }
+            float s0, s1;
+            f2_unpack(f2_add(sum2[0], sum2[1]), s0, s1);
+            l += s0 + s1;
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.p_full[i]);
+        }
+        // ---- the rows' sums, in units of 2^-m
+        bool have = false;
+        if (steps[i] > 0 && ok) have = mbar_wait_sleep(&sm.o_full[i], 0, kSiteO);
+        have = __all_sync(0xffffffffu, have);
+        if (have) tc_fence_after();
+        const float inv = 1.f / f;
+        named_bar_sync(1, 256);  // both warpgroups' products are done: the K tiles are free
+        if (pp.pairs) {
+            // the second warpgroup's rows go through shared memory (64 KB: K's two tiles) to the first's
+            float4* mine = reinterpret_cast<float4*>(sm.k[0]) + r * (kD / 4);
+            if (i == 1) {
+                if (have) {
+#pragma unroll 1
+                    for (int cc = 0; cc < 4; ++cc) {
+                        float o[32];
+                        tmem_ld32(tO + cc * 32, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            mine[(cc * 8 + e) ^ (r & 7)] = make_float4(o[4 * e] * inv, o[4 * e + 1] * inv, o[4 * e + 2] * inv, o[4 * e + 3] * inv);
+                    }
+                }
+                sm.m[r] = have ? m : -INFINITY, sm.l[r] = have ? l : 0.f, sm.mx[r] = have ? mx : -INFINITY;
+            }
+            named_bar_sync(1, 256);
+        }
+        if (i == 0 || !pp.pairs) {
+            const int row = row0 + (pp.pairs ? 0 : i * kBM) + r;
+            const bool in = row < pp.rows && have;
+            const int bt = in ? row / p.group : 0;
+            const long long rows = (long long)p.B * p.T * p.heads;
+            const long long at = (long long)part * rows + (long long)bt * p.heads + (long long)hk * p.group + (in ? row % p.group : 0);
+            float a0 = inv, a1 = 0.f, best = m, sum = l, big = mx;
+            const bool both = pp.pairs && steps[1] > 0;
+            if (both) {
+                const float m1 = sm.m[r], l1 = sm.l[r];
+                best = fmaxf(m, m1);
+                const float e0 = m == -INFINITY ? 1.f : ex2_approx(m - best), e1 = m1 == -INFINITY ? 1.f : ex2_approx(m1 - best);
+                a0 = inv * e0;
+                a1 = e1;
+                sum = l * e0 + l1 * e1;
+                big = fmaxf(mx, sm.mx[r]);
+            }
+            const float4* other = reinterpret_cast<const float4*>(sm.k[0]) + r * (kD / 4);
+            float4* dst = reinterpret_cast<float4*>(p.shared_o + at * kD);
+#pragma unroll 1
+            for (int cc = 0; cc < 4; ++cc) {
+                float o[32];
+                if (have) {
+                    tmem_ld32(tO + cc * 32, o);
+                    tmem_wait_ld();
+                }
+                if (in) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        float4 y = make_float4(o[4 * e] * a0, o[4 * e + 1] * a0, o[4 * e + 2] * a0, o[4 * e + 3] * a0);
+                        if (both) {
+                            const float4 z = other[(cc * 8 + e) ^ (r & 7)];
+                            y.x = fmaf(z.x, a1, y.x), y.y = fmaf(z.y, a1, y.y), y.z = fmaf(z.z, a1, y.z), y.w = fmaf(z.w, a1, y.w);
+                        }
+                        dst[cc * 8 + e] = y;
+                    }
+                }
+            }
+            if (in) p.shared_s[at] = make_float4(best, sum, big, 0.f);
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 12) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+}  // namespace prefix_attn
+}  // namespace dt

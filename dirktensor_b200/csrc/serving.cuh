@@ -149,6 +149,24 @@ AttnPlan plan_attn(int B, int T, int heads, int kv_heads, int q_f32, int page_si
     return s;
 }
 
+// How the prefix's part is cut: one CTA per SM, each with a block of query rows of a K/V head and an
+// even stretch of the prefix.  Two Q tiles per CTA, so that keys are converted once for 256 rows,
+// where there are more than 128 rows; fp32 queries take both tiles' memory for their two parts.
+struct PrefixPlan {
+    int rows, blocks, pairs, tiles, split;
+};
+PrefixPlan plan_prefix(int B, int T, int heads, int kv_heads, int q_f32, int prefix_len) {
+    PrefixPlan s{};
+    s.rows = B * T * (heads / kv_heads);
+    s.pairs = q_f32 || s.rows <= 128;
+    s.blocks = (s.rows + (s.pairs ? 127 : 255)) / (s.pairs ? 128 : 256);
+    s.tiles = (int)(((long long)prefix_len + 127) / 128);
+    const long long groups = (long long)kv_heads * s.blocks;
+    s.split = (int)std::max<long long>(1, std::min<long long>(s.tiles, kPlanSms / groups));
+    return s;
+}
+constexpr size_t kPrefixSmem = sizeof(dt::prefix_attn::Smem) + 1024;
+
 // Workspace of a plan: the tile counts, the CTAs' parts, the prefix's parts.
 struct AttnSpace {
     size_t starts, part_s, part_o, shared_s, shared_o, total;
@@ -221,11 +239,30 @@ int launch_stream(const dt::cache_attn::Params& p, const AttnPlan& plan, int for
     return launch_pdl(join, grid, block, 0, st, p);
 }
 
+int launch_prefix(const dt::cache_attn::Params& p, const PrefixPlan& plan, int format, int q_f32, cudaStream_t st) {
+    namespace pa = dt::prefix_attn;
+    pa::Params pp{};
+    pp.a = p;
+    pp.rows = plan.rows;
+    pp.blocks = plan.blocks;
+    pp.pairs = plan.pairs;
+    pp.split = plan.split;
+    pp.tiles = plan.tiles;
+    const long long ctas = (long long)p.c.heads * plan.blocks * plan.split;
+    if (ctas > 0x7fffffffll) return fail(DT_ERR_INVALID_ARGUMENT, "B * T * heads is too large");
+    auto* k = format == DT_KV_INT8 ? (q_f32 ? pa::prefix_kernel<0, true> : pa::prefix_kernel<0, false>)
+                                   : (q_f32 ? pa::prefix_kernel<1, true> : pa::prefix_kernel<1, false>);
+    return launch_pdl(k, dim3((unsigned)ctas), dim3(pa::kThreads), kPrefixSmem, st, pp);
+}
+
 // Per-device attributes of the kernels below (called with g_mu held, from ensure_attrs).
 int serving_attrs() {
     for (int i = 0; i < 24; ++i)
         DT_CUDA(cudaFuncSetAttribute(attn_kernel_of(i & 1, (i >> 1) & 1, (i >> 2) & 1, i / 8),
                                      cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(dt::cache_attn::Smem)));
+    for (auto* k : {dt::prefix_attn::prefix_kernel<0, false>, dt::prefix_attn::prefix_kernel<0, true>,
+                    dt::prefix_attn::prefix_kernel<1, false>, dt::prefix_attn::prefix_kernel<1, true>})
+        DT_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPrefixSmem));
     return DT_OK;
 }
 
@@ -266,38 +303,33 @@ int cache_attn(const dt_kv_cache* cache, const void* q, long long q_batch_stride
     p.heads = heads;
     p.group = heads / cache->kv_heads;
     p.scale = scale;
-    const AttnPlan plan = plan_attn(B, T, heads, cache->kv_heads, q_f32, cache->page_size, max_pages, 0);
+    AttnPlan plan = plan_attn(B, T, heads, cache->kv_heads, q_f32, cache->page_size, max_pages, prefix_len);
+    if (max_pages == 0) plan.shares = plan.split = 0;  // no keys of their own
+    if (plan.shares < 0)
+        return fail(DT_ERR_INVALID_ARGUMENT, "behind a prefix, B must be at most %d and the page table below 2^31 tokens",
+                    dt::cache_attn::kMaxBatch);
     if (plan.items * std::max(plan.split, 1) > 0x7fffffffll)
         return fail(DT_ERR_INVALID_ARGUMENT, "B * kv_heads * query rows is too large");
-    const AttnSpace space = attn_space(plan, B, T, heads, 0);
-    if (prefix_len == 0 && space.total > 0 && (!workspace || workspace_bytes < space.total || !aligned16(workspace)))
+    const PrefixPlan prefix = prefix_len > 0 ? plan_prefix(B, T, heads, cache->kv_heads, q_f32, prefix_len) : PrefixPlan{};
+    const AttnSpace space = attn_space(plan, B, T, heads, prefix.split);
+    if (space.total > 0 && (!workspace || workspace_bytes < space.total || !aligned16(workspace)))
         return fail(DT_ERR_INVALID_ARGUMENT, "workspace must be >= %zu bytes and 16-byte aligned", space.total);
     int dev;
     DT_TRY(prepare_device(&dev));
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    if (prefix_len == 0) {
-        if (max_pages == 0) {  // no keys: zeros
-            p.shares = 0;
-            return launch_stream(p, AttnPlan{}, cache->format, q_f32, st);
-        }
-        p.split = plan.split;
-        p.shares = plan.shares;
-        p.by_length = plan.by_length;
-        if (plan.shares > 0) {
-            uint8_t* w = static_cast<uint8_t*>(workspace);
-            p.starts = reinterpret_cast<int*>(w + space.starts);
-            p.part_s = reinterpret_cast<float4*>(w + space.part_s);
-            p.part_o = reinterpret_cast<float*>(w + space.part_o);
-            return launch_stream(p, plan, cache->format, q_f32, st);
-        }
-        return launch_split(attn_kernel_of(false, cache->format, q_f32, plan.form), p, plan.items, st);
-    }
-    const dim3 grid((unsigned)(((long long)B * T * heads + 3) / 4)), block(128);
-    if (cache->format == DT_KV_INT8)
-        return q_f32 ? launch_pdl(dt::cache_attn::row_kernel<0, true>, grid, block, 0, st, p)
-                     : launch_pdl(dt::cache_attn::row_kernel<0, false>, grid, block, 0, st, p);
-    return q_f32 ? launch_pdl(dt::cache_attn::row_kernel<1, true>, grid, block, 0, st, p)
-                 : launch_pdl(dt::cache_attn::row_kernel<1, false>, grid, block, 0, st, p);
+    p.split = plan.split;
+    p.by_length = plan.by_length;
+    p.shares = plan.shares;
+    p.n_shared = prefix.split;
+    uint8_t* w = static_cast<uint8_t*>(workspace);
+    p.starts = reinterpret_cast<int*>(w + space.starts);
+    p.part_s = reinterpret_cast<float4*>(w + space.part_s);
+    p.part_o = reinterpret_cast<float*>(w + space.part_o);
+    p.shared_s = reinterpret_cast<float4*>(w + space.shared_s);
+    p.shared_o = reinterpret_cast<float*>(w + space.shared_o);
+    if (plan.split > 0) return launch_split(attn_kernel_of(false, cache->format, q_f32, plan.form), p, plan.items, st);
+    if (prefix_len > 0) DT_TRY(launch_prefix(p, prefix, cache->format, q_f32, st));
+    return launch_stream(p, plan, cache->format, q_f32, st);
 }
 
 }  // namespace
@@ -320,9 +352,14 @@ size_t dt_cache_attn_workspace_bytes(int B, int T, int heads, int kv_heads, int 
     return attn_space(plan_attn(B, T, heads, kv_heads, q_f32, page_size, max_pages, 0), B, T, heads, 0).total;
 }
 
-size_t dt_prefix_attn_workspace_bytes(int B, int T, int heads, int kv_heads, int prefix_len) {
-    if (B <= 0 || T <= 0 || heads <= 0 || kv_heads <= 0 || prefix_len <= 0) return 0;
-    return 0;
+size_t dt_prefix_attn_workspace_bytes(int B, int T, int heads, int kv_heads, int q_f32, int page_size, int max_pages,
+                                      int prefix_len) {
+    if (prefix_len <= 0) return dt_cache_attn_workspace_bytes(B, T, heads, kv_heads, q_f32, page_size, max_pages);
+    if (B <= 0 || T <= 0 || kv_heads <= 0 || heads < kv_heads || page_size <= 0 || max_pages < 0) return 0;
+    if ((long long)B * T * heads > 0x7fffffffll) return 0;
+    AttnPlan plan = plan_attn(B, T, heads, kv_heads, q_f32, page_size, max_pages, prefix_len);
+    if (max_pages == 0) plan.shares = plan.split = 0;
+    return attn_space(plan, B, T, heads, plan_prefix(B, T, heads, kv_heads, q_f32, prefix_len).split).total;
 }
 
 int dt_prefix_attn_fwd(const dt_kv_cache* cache, const void* q, long long q_batch_stride, long long q_token_stride,

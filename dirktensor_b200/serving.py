@@ -201,11 +201,11 @@ def prefix_attention_forward(q, cache: KVCache, prefix_pages, prefix_len: int, p
     table, stride, n = (None, 0, 0) if page_table is None else _table(page_table, cache.device, B)
     lens = _ints("seq_lens", seq_lens, cache.device, B)
     o, m, l = _outputs(q, out, return_stats)
-    L = lib()
-    nbytes = L.dt_prefix_attn_workspace_bytes(B, T, H, cache.kv_heads, prefix_len)
+    f32, L = int(q.dtype == torch.float32), lib()
+    nbytes = L.dt_prefix_attn_workspace_bytes(B, T, H, cache.kv_heads, f32, cache.page_size, n, prefix_len)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=cache.device) if nbytes else None
     with _on(cache.device):
-        check(L.dt_prefix_attn_fwd(cache._ref, q.data_ptr(), s[0], s[1], int(q.dtype == torch.float32), o.data_ptr(),
+        check(L.dt_prefix_attn_fwd(cache._ref, q.data_ptr(), s[0], s[1], f32, o.data_ptr(),
                                    m.data_ptr() if return_stats else None, l.data_ptr() if return_stats else None,
                                    pages, prefix_len, table, stride, n, lens,
                                    _ints("q_lens", q_lens, cache.device, B), B, T, H, float(scale),

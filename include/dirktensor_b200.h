@@ -437,10 +437,11 @@ int dt_cache_attn_fwd(const dt_kv_cache* cache, const void* q, long long q_batch
  * device int[ceil(prefix_len / page_size)]) and then its own sequence's keys
  * as above, whose positions, page_table and seq_lens count from the prefix's
  * end.  The prefix is read once for the whole batch, not once per sequence.
- * max_pages may be 0 (no keys of their own).  workspace: at least
+ * max_pages may be 0 (no keys of their own); B is at most 8192.  workspace: at least
  * dt_prefix_attn_workspace_bytes, 16-byte aligned (NULL when that is 0); calls
  * that may overlap on the GPU need one each. */
-size_t dt_prefix_attn_workspace_bytes(int B, int T, int heads, int kv_heads, int prefix_len);
+size_t dt_prefix_attn_workspace_bytes(int B, int T, int heads, int kv_heads, int q_f32, int page_size, int max_pages,
+                                      int prefix_len);
 int dt_prefix_attn_fwd(const dt_kv_cache* cache, const void* q, long long q_batch_stride, long long q_token_stride,
                        int q_f32, void* o, float* softmax_m, float* softmax_l, const int* prefix_pages, int prefix_len,
                        const int* page_table, long long page_table_stride, int max_pages, const int* seq_lens,

@@ -74,8 +74,19 @@ def test_attention_refusals():
 
     assert prefix(n=-1) == 1 and b"prefix_len" in L.dt_last_error()
     assert prefix(pages=None) == 1 and b"prefix_len" in L.dt_last_error()
-    assert L.dt_prefix_attn_workspace_bytes(0, 1, 4, 4, 100) == 0
-    assert L.dt_prefix_attn_workspace_bytes(4, 1, 4, 4, 0) == 0
+    assert prefix(ws=None) == 1 and b"workspace" in L.dt_last_error()
+    assert prefix(size=64) == 1 and b"workspace" in L.dt_last_error()
+    assert prefix(ws=FAKE + 8) == 1 and b"workspace" in L.dt_last_error()
+    assert L.dt_prefix_attn_workspace_bytes(0, 1, 4, 4, 0, 64, 4, 100) == 0
+    assert L.dt_prefix_attn_workspace_bytes(4, 1, 4, 4, 0, 64, 4, 0) == L.dt_cache_attn_workspace_bytes(4, 1, 4, 4, 0, 64, 4)
+    # one part of the prefix and no keys of their own: (m, l, ...) and 128 sums per row
+    assert L.dt_prefix_attn_workspace_bytes(4, 1, 4, 4, 0, 64, 0, 100) == 16 * 16 + 16 * 512
+    # few items of many keys are shared out, and need room for the parts
+    assert L.dt_cache_attn_workspace_bytes(1, 1, 4, 4, 0, 64, 4096) > 0
+    assert attn(n=1 << 26) == 1 and b"page_table_stride" in L.dt_last_error()
+    st = L.dt_cache_attn_fwd(cache(), FAKE, 512, 512, 0, FAKE, None, None, FAKE, 1 << 26, 1 << 26, FAKE, None, 1, 1, 4, 0.1,
+                             FAKE, 1 << 40, None)
+    assert st == 1 and b"2^30" in L.dt_last_error()
 
 
 def test_log_prob_refusals():
