@@ -163,6 +163,12 @@ __device__ __forceinline__ float column_sum(float x) {
     return x;
 }
 
+__device__ __forceinline__ float warp_max(float x) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+    return x;
+}
+
 // 2^e for e in [-126, 127]
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
 // floor(log2 |x|) of a normal number
@@ -178,6 +184,10 @@ struct Joined {
         const float a = pl != pl ? pl : ex2_approx(pm - best);  // (scores that are all NaN leave pm at -inf)
         l += pl * a;
         o.x += po.x * a, o.y += po.y * a, o.z += po.z * a, o.w += po.w * a;
+    }
+    __device__ __forceinline__ void scale(float a) {
+        l *= a;
+        o.x *= a, o.y *= a, o.z *= a, o.w *= a;
     }
 };
 
@@ -617,6 +627,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kF32, kForm)) split_kern
         for (int i = threadIdx.x; i < p.B; i += kThreads) {
             const int mine = lens[i];
             int rank = 0;
+#pragma unroll 8
             for (int j = 0; j < p.B; ++j) rank += lens[j] > mine || (lens[j] == mine && j < i);
             if (rank == b) sm.om[0] = __int_as_float(i);
         }
@@ -653,7 +664,30 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kF32, kForm)) split_kern
             y.add(other->om[row], other->ol[row], best,
                   reinterpret_cast<const float4*>(other->joined(row))[lane]);
         }
-        store_row<kF32>(p, ((long long)b * p.T + rr / p.group) * p.heads + hk * p.group + rr % p.group, lane, y, best, big);
+        const long long out = ((long long)b * p.T + rr / p.group) * p.heads + hk * p.group + rr % p.group;
+        // the prefix's parts (at most 16: all of them on their way at once)
+        const int q_len = p.q_lens ? min(p.q_lens[b], p.T) : p.T;
+        const int shared = rr / p.group < q_len ? p.n_shared : 0;
+        if (shared > 0) {
+            const long long all = (long long)p.B * p.T * p.heads;
+            float4 s = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
+            if (lane < shared) s = p.shared_s[lane * all + out];
+            const float own = best;
+            best = fmaxf(best, warp_max(s.x)), big = fmaxf(big, warp_max(s.z));
+            if (own != -INFINITY) y.scale(ex2_approx(own - best));
+#pragma unroll 1
+            for (int c0 = 0; c0 < shared; c0 += 8) {
+                float4 o[8];
+#pragma unroll
+                for (int c = 0; c < 8; ++c)
+                    o[c] = c0 + c < shared ? reinterpret_cast<const float4*>(p.shared_o + ((c0 + c) * all + out) * kD)[lane]
+                                           : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int c = 0; c < 8; ++c)
+                    y.add(__shfl_sync(0xffffffffu, s.x, c0 + c), __shfl_sync(0xffffffffu, s.y, c0 + c), best, o[c]);
+            }
+        }
+        store_row<kF32>(p, out, lane, y, best, big);
     }
     if (p.split > 1) cluster.sync();  // no CTA leaves while another reads its shared memory
 }
@@ -818,8 +852,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const Params p) {
         if (top > m) {
             const float a = m == -INFINITY ? 1.f : ex2_approx(m - top);  // (at -inf there may be NaNs, which stay)
             m = top;
-            y.l *= a;
-            y.o.x *= a, y.o.y *= a, y.o.z *= a, y.o.w *= a;
+            y.scale(a);
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i)

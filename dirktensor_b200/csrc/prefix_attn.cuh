@@ -54,9 +54,9 @@ struct __align__(1024) Smem {
     uint8_t k[2][kTileBytes];
     uint8_t v[2][kTileBytes];
     float ks[4][kBN];           // of tile t: at t & 3
-    float vs[4][kBN];           // v_scale * f
-    float f[4];
-    uint32_t hidden[4][4];      // keys past the prefix, or on a page that does not exist
+    float vs[4][kBN];
+    float most[4][kConvWarps];  // largest v_scale of the 32 keys of each converting warp
+    uint32_t hidden[4][kConvWarps];  // keys past the prefix, or on a page that does not exist
     float factor[2][kBM];       // from S back to scores in log2 units (k_scale apart)
     float m[kBM], l[kBM], mx[kBM];  // of the second warpgroup, for the first (pairs)
     uint64_t q_full;
@@ -83,21 +83,16 @@ __device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
 }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// A 16-byte piece of codes (dims 16 piece ..+15 of row r) as fp16 into a swizzled tile.
+// A 16-byte piece of codes (16 dims of one key) as fp16: two 16-byte chunks of a swizzled tile.  The
+// lanes of the second half of the dims store theirs in the other order (`swap`): no bank conflicts.
 template <int kFmt>
-__device__ __forceinline__ void put_piece(uint32_t tile, int r, int piece, uint4 codes) {
-    const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
+__device__ __forceinline__ void put_piece(uint32_t first, uint32_t second, bool swap, uint4 c) {
+    const uint32_t w[4] = {swap ? c.z : c.x, swap ? c.w : c.y, swap ? c.x : c.z, swap ? c.y : c.w};
     uint32_t h[8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) cache_attn::pairs_of_word<kFmt>(w[i], h[2 * i], h[2 * i + 1]);
-    const uint32_t base = tile + (uint32_t)(piece >> 2) * kHalfBytes + (uint32_t)r * 128;
-    const uint32_t c = 2 * (piece & 3);
-    // the lanes of the second half store their chunks in the other order: no bank conflicts
-    const bool swap = piece >= 4;
-    const uint32_t first = base + (((c + (swap ? 1u : 0u)) ^ (uint32_t)(r & 7)) << 4);
-    const uint32_t second = base + (((c + (swap ? 0u : 1u)) ^ (uint32_t)(r & 7)) << 4);
-    st_shared_v4(first, swap ? h[4] : h[0], swap ? h[5] : h[1], swap ? h[6] : h[2], swap ? h[7] : h[3]);
-    st_shared_v4(second, swap ? h[0] : h[4], swap ? h[1] : h[5], swap ? h[2] : h[6], swap ? h[3] : h[7]);
+    st_shared_v4(first, h[0], h[1], h[2], h[3]);
+    st_shared_v4(second, h[4], h[5], h[6], h[7]);
 }
 
 template <int kFmt, bool kF32>
@@ -152,106 +147,108 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const Params pp) {
             return page >= 0 && page < p.c.pages ? page : -1;
         };
         // lane: piece lane & 7 of rows 4 i + lane / 8
+        const int rl = lane >> 3, piece = lane & 7;
         auto load = [&](const uint8_t* codes, int tile, const int (&page)[2], uint4 (&x)[8]) {
+            const int key0 = tile * kBN + cw * 32;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int r = 4 * i + (lane >> 3);
-                const int key = tile * kBN + cw * 32 + r;
-                const int pg = page[i >> 2];
-                x[i] = make_uint4(0, 0, 0, 0);  // hidden keys: zeros
-                if (pg >= 0 && key < p.prefix_len) {
-                    const long long row = (((long long)pg * p.c.heads + hk) << shift) + (key & in_page);
-                    x[i] = __ldg(reinterpret_cast<const uint4*>(codes + row * kD) + (lane & 7));
-                }
+            for (int g = 0; g < 2; ++g) {
+                // hidden keys: zeros (a page that does not exist hides all 16)
+                const int left = page[g] >= 0 ? p.prefix_len - (key0 + 16 * g) : 0;
+                const uint32_t row = ((uint32_t)(page[g] * p.c.heads + hk) << shift) + ((key0 + 16 * g) & in_page);
+                const uint4* src = reinterpret_cast<const uint4*>(codes + (size_t)row * kD) + rl * (kD / 16) + piece;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    x[4 * g + i] = 4 * i + rl < left ? __ldg(src + i * 4 * (kD / 16)) : make_uint4(0, 0, 0, 0);
             }
         };
+        // offsets of a lane's chunks in a tile, of even and odd i (row & 7 is rl, or 4 + rl)
+        const bool swap = piece >= 4;
+        uint32_t off[2][2];
+#pragma unroll
+        for (int o = 0; o < 2; ++o)
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+                off[o][c] = (uint32_t)(piece >> 2) * kHalfBytes + (uint32_t)(cw * 32 + 4 * o + rl) * 128 +
+                            (((2 * (piece & 3) + ((c == 0) == swap ? 1 : 0)) ^ (4 * o + rl)) << 4);
         auto put = [&](uint8_t* tile, const uint4 (&x)[8]) {
             const uint32_t base = smem_u32(tile);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) put_piece<kFmt>(base, cw * 32 + 4 * i + (lane >> 3), lane & 7, x[i]);
+            for (int i = 0; i < 8; ++i)
+                put_piece<kFmt>(base + off[i & 1][0] + (i >> 1) * 1024, base + off[i & 1][1] + (i >> 1) * 1024, swap, x[i]);
         };
-        float f = pow2(100);
-        // the scales of a tile, four keys a lane of the first of these warps
-        auto scales = [&](int tile) {
-            if (cw != 0) return;
-            float k[4], v[4];
-            uint32_t hide = 0;
-            float most = 0.f;
-            const int key = tile * kBN + 4 * lane;
-            const int page = key < p.prefix_len ? __ldg(p.prefix_pages + (key >> shift)) : -1;
-            const bool ok = page >= 0 && page < p.c.pages;
-            const long long row = ok ? (((long long)page * p.c.heads + hk) << shift) + (key & in_page) : 0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const bool see = ok && key + e < p.prefix_len;
-                k[e] = see ? __ldg(p.c.ks + row + e) : 0.f;
-                v[e] = see ? __ldg(p.c.vs + row + e) : 0.f;
-                if (!see) hide |= 1u << e;
-                most = fmaxf(most, v[e]);
+        // scales of a tile, one key a lane
+        auto load_scales = [&](int tile, const int (&page)[2], float& k, float& v, bool& see) {
+            const int key = tile * kBN + cw * 32 + lane;
+            const int pg = lane < 16 ? page[0] : page[1];
+            see = pg >= 0 && key < p.prefix_len;
+            k = 1.f, v = 0.f;  // (a hidden key's score becomes -inf)
+            if (see) {
+                const uint32_t row = ((uint32_t)(pg * p.c.heads + hk) << shift) + (key & in_page);
+                k = __ldg(p.c.ks + row);
+                v = __ldg(p.c.vs + row);
             }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-            // p <= 2^8 (the lazy maximum), so p * v_scale * f < 2^15 with f = 2^(6 - exponent)
-            f = fminf(f, pow2(min(max(6 - exponent(most), -120), 100)));
-            const int at = tile - t0;
-            *reinterpret_cast<float4*>(&sm.ks[at & 3][4 * lane]) = make_float4(k[0], k[1], k[2], k[3]);
-            *reinterpret_cast<float4*>(&sm.vs[at & 3][4 * lane]) = make_float4(v[0] * f, v[1] * f, v[2] * f, v[3] * f);
-            // 4 bits from each of 8 lanes make a word
-            uint32_t word = hide << (4 * (lane & 7));
-#pragma unroll
-            for (int o = 1; o < 8; o <<= 1) word |= __shfl_xor_sync(0xffffffffu, word, o);
-            if ((lane & 7) == 0) sm.hidden[at & 3][lane >> 3] = word;
-            if (lane == 0) sm.f[at & 3] = f;
         };
+        // Pieces in the order K0, K1, V0, K2, V1, ...: a tile's codes are on their way while the tile before
+        // is converted, and its page numbers for a tile longer.
         bool ok = true;
         uint4 xk[8], xv[8];
-        int pk[2] = {page_of(t0, 0), page_of(t0, 1)};
-        int pv[2] = {pk[0], pk[1]};  // pages of the tile whose V comes next
-        load(p.c.k, t0, pk, xk);
-        load(p.c.v, t0, pk, xv);
-        int next[2] = {page_of(t0 + 1, 0), page_of(t0 + 1, 1)};
-        // order: K0, K1, V0, K2, V1, ...
-        for (int j = 0; ok && j <= n; ++j) {
+        float ks, vs;
+        bool see;
+        int page0[2], page1[2], page2[2];  // of tiles j, j + 1, j + 2
+        auto look_up = [&](int tile, int (&page)[2]) { page[0] = page_of(tile, 0), page[1] = page_of(tile, 1); };
+        look_up(t0, page0);
+        look_up(t0 + 1, page1);
+        load(p.c.k, t0, page0, xk);
+        load_scales(t0, page0, ks, vs, see);
+        load(p.c.v, t0, page0, xv);
+        look_up(t0 + 2, page2);
+#pragma unroll 1
+        for (int j = 0; j <= n; ++j) {
+            const int s = j & 1;
             if (j < n) {  // K of tile j
-                const int s = j & 1;
-                if (j >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&sm.k_empty[s], ((j >> 1) - 1) & 1, kSiteKEmpty));
+                if (j >= 2) ok = __all_sync(0xffffffffu, mbar_wait_sleep(&sm.k_empty[s], ((j >> 1) - 1) & 1, kSiteKEmpty));
                 if (!ok) break;
-                scales(t0 + j);
+                sm.ks[j & 3][cw * 32 + lane] = ks;
+                sm.vs[j & 3][cw * 32 + lane] = vs;
+                // (scales are not negative, so their bits order as they do; a NaN is not a largest)
+                const uint32_t most = __reduce_max_sync(0xffffffffu, vs == vs && vs > 0.f ? __float_as_uint(vs) : 0u);
+                const uint32_t seen = __ballot_sync(0xffffffffu, see);
+                if (lane == 0) sm.most[j & 3][cw] = __uint_as_float(most), sm.hidden[j & 3][cw] = ~seen;
                 put(sm.k[s], xk);
                 fence_async();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sm.k_full[s]);
-                if (j + 1 < n) load(p.c.k, t0 + j + 1, next, xk);
-            }
-            if (j >= 1) {  // V of tile j - 1
-                const int i = j - 1, s = i & 1;
-                if (i >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&sm.v_empty[s], ((i >> 1) - 1) & 1, kSiteVEmpty));
-                if (!ok) break;
-                put(sm.v[s], xv);
-                fence_async();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sm.v_full[s]);
-                if (j < n) {
-                    pv[0] = pk[0], pv[1] = pk[1];
-                    load(p.c.v, t0 + j, pv, xv);
+                if (j + 1 < n) {
+                    load(p.c.k, t0 + j + 1, page1, xk);
+                    load_scales(t0 + j + 1, page1, ks, vs, see);
                 }
             }
-            // pk: pages of tile j + 1, whose V is loaded next; next: of tile j + 2
-            pk[0] = next[0], pk[1] = next[1];
-            next[0] = page_of(t0 + j + 2, 0), next[1] = page_of(t0 + j + 2, 1);
+            if (j >= 1) {  // V of tile j - 1
+                const int i = j - 1;
+                if (i >= 2) ok = __all_sync(0xffffffffu, mbar_wait_sleep(&sm.v_empty[i & 1], ((i >> 1) - 1) & 1, kSiteVEmpty));
+                if (!ok) break;
+                put(sm.v[i & 1], xv);
+                fence_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.v_full[i & 1]);
+                if (j < n) load(p.c.v, t0 + j, page0, xv);
+            }
+            page0[0] = page1[0], page0[1] = page1[1];
+            page1[0] = page2[0], page1[1] = page2[1];
+            look_up(t0 + j + 3, page2);
         }
     } else if (warp == 12) {
         // ------------------------------ MMA issue ---------------------------
         if (lane == 0) {
             constexpr uint32_t idesc_qk = idesc_f16(kBM, kBN, 0);
             constexpr uint32_t idesc_pv = idesc_f16(kBM, kD, 1);
-            bool ok = mbar_wait(&sm.q_full, 0, kSiteQ);
+            bool ok = mbar_wait_sleep(&sm.q_full, 0, kSiteQ);
             int k_seen = 0, v_seen = 0;  // tiles whose K and V have been waited for
             auto want_k = [&](int t) {
-                for (; ok && k_seen <= t; ++k_seen) ok = mbar_wait(&sm.k_full[k_seen & 1], (k_seen >> 1) & 1, kSiteKFull);
+                for (; ok && k_seen <= t; ++k_seen) ok = mbar_wait_sleep(&sm.k_full[k_seen & 1], (k_seen >> 1) & 1, kSiteKFull);
             };
             auto want_v = [&](int t) {
-                for (; ok && v_seen <= t; ++v_seen) ok = mbar_wait(&sm.v_full[v_seen & 1], (v_seen >> 1) & 1, kSiteVFull);
+                for (; ok && v_seen <= t; ++v_seen) ok = mbar_wait_sleep(&sm.v_full[v_seen & 1], (v_seen >> 1) & 1, kSiteVFull);
             };
             auto issue_s = [&](int i, int t) {
                 const uint32_t k = smem_u32(sm.k[t & 1]);
@@ -272,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const Params pp) {
                 for (int half = 0; half < (kF32 ? 2 : 1); ++half)
 #pragma unroll
                     for (int kk = 0; kk < kBN / 16; ++kk)
-                        umma_ts(tmem + 256 + i * 128, tmem + i * 128 + half * 64 + kk * 8,
+                        umma_ts(tmem + 256 + i * 128, tmem + i * 128 + (kF32 ? (kk >> 1) * 32 + half * 16 + (kk & 1) * 8 : kk * 8),
                                 umma_desc_sw128(v + kk * 2048, kHalfBytes, 1024), idesc_pv, (add || kk > 0 || half > 0) ? 1u : 0u);
             };
             auto tile_of = [&](int i, int s) { return pp.pairs ? 2 * s + i : s; };
@@ -290,7 +287,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const Params pp) {
                     const int t = tile_of(i, s), tn = tile_of(i, s + 1);
                     want_v(t);
                     if (ok && s + 1 < steps[i]) want_k(tn);
-                    if (ok) ok = mbar_wait(&sm.p_full[i], s & 1, kSiteP);
+                    if (ok) ok = mbar_wait_sleep(&sm.p_full[i], s & 1, kSiteP);
                     if (!ok) break;
                     tc_fence_after();
                     issue_pv(i, t, s > 0);
@@ -306,7 +303,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const Params pp) {
             }
             // all issued work is complete before TMEM is released
             umma_commit(&sm.mma_done);
-            mbar_wait(&sm.mma_done, 0, kSiteDone);
+            mbar_wait_sleep(&sm.mma_done, 0, kSiteDone);
         }
         __syncwarp();
     } else {
@@ -377,19 +374,40 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const Params pp) {
         const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t tS = tmem + lane_off + i * 128;
         const uint32_t tO = tmem + lane_off + 256 + i * 128;
-        const float factor = sm.factor[pp.pairs ? 0 : i][r];
-        float m = -INFINITY, l = 0.f, mx = -INFINITY, f = pow2(100);
+        float factor = sm.factor[pp.pairs ? 0 : i][r];
+        if (factor == 0.f) factor = 1e-37f;  // (no 0 * -inf; scores of 1e-37 weigh as 0 do)
+        // Weights are computed as p * f: l and O hold sums with that factor.
+        float m = -INFINITY, l = 0.f, mx = -INFINITY;
+        int fe = 100;  // f = 2^fe
+        const bool idle = row0 + (pp.pairs ? 0 : i * kBM) + (warp & 3) * 32 >= pp.rows;  // no query in this warp's rows
         bool ok = true;
         for (int s = 0; s < steps[i]; ++s) {
             // warp-uniform, since the step synchronises the warp
             if (!__all_sync(0xffffffffu, mbar_wait_sleep(&sm.s_full[i], s & 1, kSiteS))) { ok = false; break; }
+            if (idle) {  // (what stays in their P rows reaches only their O rows)
+                if (lane == 0) mbar_arrive(&sm.p_full[i]);
+                continue;
+            }
             tc_fence_after();
             const int at = (pp.pairs ? 2 * s + i : s) & 3;
-            const uint32_t hid[4] = {sm.hidden[at][0], sm.hidden[at][1], sm.hidden[at][2], sm.hidden[at][3]};
-            const bool some = (hid[0] | hid[1] | hid[2] | hid[3]) != 0u;
+            const bool some = (sm.hidden[at][0] | sm.hidden[at][1] | sm.hidden[at][2] | sm.hidden[at][3]) != 0u;
+            if (some) {  // the last tile, or a page that does not exist: hidden scores become -inf
+#pragma unroll 1
+                for (int cc = 0; cc < 8; ++cc) {
+                    float x[16];
+                    tmem_ld16(tS + cc * 16, x);
+                    tmem_wait_ld();
+                    const uint32_t bits = sm.hidden[at][cc >> 1] >> (16 * (cc & 1));
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if ((bits >> e) & 1u) x[e] = -INFINITY;
+                    tmem_st16(tS + cc * 16, *reinterpret_cast<uint32_t(*)[16]>(x));
+                }
+                tmem_wait_st();
+            }
             // first pass: the row's largest score
             float top = -INFINITY;
-#pragma unroll
+#pragma unroll 1
             for (int cc = 0; cc < 4; ++cc) {
                 float x[32];
                 tmem_ld32(tS + cc * 32, x);
@@ -401,46 +419,40 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const Params pp) {
                     float y[4];
                     f2_unpack(f2_mul(f2_pack(x[e], x[e + 1]), f2_pack(k.x, k.y)), y[0], y[1]);
                     f2_unpack(f2_mul(f2_pack(x[e + 2], x[e + 3]), f2_pack(k.z, k.w)), y[2], y[3]);
-                    if (some) {
-#pragma unroll
-                        for (int d = 0; d < 4; ++d)
-                            if ((hid[cc] >> (e + d)) & 1u) y[d] = -INFINITY;
-                    }
                     best[(e >> 2) & 3] = fmax3(best[(e >> 2) & 3], fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
                 }
                 top = fmax3(top, fmaxf(best[0], best[1]), fmaxf(best[2], best[3]));
             }
             top *= factor;  // (-inf where every key is hidden; factor is not negative)
-            if (top != top) top = -INFINITY;  // (a row of NaN factor, or 0 * -inf: no maximum)
+            if (top != top) top = -INFINITY;  // (a row whose query is not finite: no maximum)
             mx = fmaxf(mx, top);
-            const float fn = sm.f[at];
+            const float4 most = *reinterpret_cast<const float4*>(sm.most[at]);
+            // p <= 2^8 (the lazy maximum), so p * v_scale * f < 2^15
+            const int fn = min(fe, min(max(6 - exponent(fmaxf(fmaxf(most.x, most.y), fmaxf(most.z, most.w))), -120), 100));
             float by = 1.f;
             if (top > m + kGrow) {
                 by = m == -INFINITY ? 1.f : ex2_approx(m - top);
-                l *= by;
                 m = top;
             }
-            if (s > 0) {
-                if (fn != f) by *= fn / f;
-                if (__any_sync(0xffffffffu, by != 1.f)) {
+            if (fn != fe && s > 0) by *= pow2(max(fn - fe, -126));
+            fe = fn;
+            l *= by;
+            if (s > 0 && __any_sync(0xffffffffu, by != 1.f)) {
 #pragma unroll 1
-                    for (int cc = 0; cc < 8; ++cc) {
-                        float o[16];
-                        tmem_ld16(tO + cc * 16, o);
-                        tmem_wait_ld();
+                for (int cc = 0; cc < 8; ++cc) {
+                    float o[16];
+                    tmem_ld16(tO + cc * 16, o);
+                    tmem_wait_ld();
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) o[e] *= by;
-                        tmem_st16(tO + cc * 16, *reinterpret_cast<uint32_t(*)[16]>(o));
-                    }
+                    for (int e = 0; e < 16; ++e) o[e] *= by;
+                    tmem_st16(tO + cc * 16, *reinterpret_cast<uint32_t(*)[16]>(o));
                 }
             }
-            f = fn;
             // second pass: weights
-            const float m_safe = m == -INFINITY ? 0.f : m;
+            const float m_safe = (m == -INFINITY ? 0.f : m) - (float)fe;
             const uint64_t c2 = f2_pack(factor, factor), nm2 = f2_pack(-m_safe, -m_safe);
             uint64_t sum2[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
-            uint32_t late[kF32 ? 64 : 1];
-#pragma unroll
+#pragma unroll 1
             for (int cc = 0; cc < 4; ++cc) {
                 float x[32];
                 tmem_ld32(tS + cc * 32, x);
@@ -453,11 +465,6 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const Params pp) {
                     float y[4];
                     f2_unpack(f2_fma(f2_mul(f2_pack(x[e], x[e + 1]), f2_pack(k.x, k.y)), c2, nm2), y[0], y[1]);
                     f2_unpack(f2_fma(f2_mul(f2_pack(x[e + 2], x[e + 3]), f2_pack(k.z, k.w)), c2, nm2), y[2], y[3]);
-                    if (some) {
-#pragma unroll
-                        for (int d = 0; d < 4; ++d)
-                            if ((hid[cc] >> (e + d)) & 1u) y[d] = -INFINITY;
-                    }
                     const uint64_t p0 = f2_pack(ex2_approx(y[0]), ex2_approx(y[1])), p1 = f2_pack(ex2_approx(y[2]), ex2_approx(y[3]));
                     sum2[0] = f2_add(sum2[0], p0);
                     sum2[1] = f2_add(sum2[1], p1);
@@ -472,15 +479,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const Params pp) {
                         hi[e / 2 + 1] = half_pair(u[2], u[3]);
                     }
                 }
-                tmem_st16(tS + cc * 16, hi);  // columns below the ones still to be read
-                if (kF32) {
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) late[kF32 ? cc * 16 + e : 0] = lo[kF32 ? e : 0];
-                }
-            }
-            if (kF32) {  // the rests, at the columns whose scores have now been read
-#pragma unroll
-                for (int cc = 0; cc < 4; ++cc) tmem_st16(tS + 64 + cc * 16, *reinterpret_cast<uint32_t(*)[16]>(late + (kF32 ? cc * 16 : 0)));
+                // P takes the columns of scores that have been read: chunk cc's 16 (and the rests' 16 behind them)
+                tmem_st16(tS + cc * (kF32 ? 32 : 16), hi);
+                if (kF32) tmem_st16(tS + cc * 32 + 16, *reinterpret_cast<uint32_t(*)[16]>(lo));
             }
             float s0, s1;
             f2_unpack(f2_add(sum2[0], sum2[1]), s0, s1);
@@ -495,7 +496,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const Params pp) {
         if (steps[i] > 0 && ok) have = mbar_wait_sleep(&sm.o_full[i], 0, kSiteO);
         have = __all_sync(0xffffffffu, have);
         if (have) tc_fence_after();
-        const float inv = 1.f / f;
+        const float inv = pow2(-fe);
+        l *= inv;
         named_bar_sync(1, 256);  // both warpgroups' products are done: the K tiles are free
         if (pp.pairs) {
             // the second warpgroup's rows go through shared memory (64 KB: K's two tiles) to the first's

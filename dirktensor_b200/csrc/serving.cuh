@@ -117,38 +117,6 @@ namespace {
 
 constexpr int kPlanSms = 148;  // B200; the plan is made without a device, for the workspace size
 
-// How the attention's work is cut.
-struct AttnPlan {
-    int form;         // query rows per item: rows_of(form)
-    long long items;  // (sequence, K/V head, rows)
-    int split;        // CTAs per item (split_kernel), or
-    bool by_length;   // longest sequences first (split_kernel)
-    int shares;       // CTAs of stream_kernel, which join_kernel follows (0: split_kernel)
-};
-
-// split_kernel, with as many CTAs per item as the GPU holds at once, up to a cluster, and no more
-// than there are tiles for; stream_kernel where that leaves most of the GPU idle: few items with
-// many keys.  (8 x 131071 keys: 71 us shared by 444 CTAs, 149 us in 8 clusters of 8.)
-AttnPlan plan_attn(int B, int T, int heads, int kv_heads, int q_f32, int page_size, int max_pages, int prefix_len) {
-    namespace ca = dt::cache_attn;
-    AttnPlan s{};
-    const int rows = T * (heads / kv_heads);
-    s.form = rows <= 4 ? ca::kFew : q_f32 || rows <= 8 ? ca::kEight : ca::kWide;
-    s.items = (long long)B * kv_heads * ((rows + ca::rows_of(s.form) - 1) / ca::rows_of(s.form));
-    const long long tiles = ((long long)max_pages * page_size + ca::kTile - 1) / ca::kTile;
-    const int slots = ca::ctas_per_sm(q_f32, s.form) * kPlanSms;
-    const bool fits = B <= ca::kMaxBatch && tiles * B < 0x7fffffffll && s.items < 0x7fffffffll - slots;
-    const bool few = s.items * ca::kMaxCluster * 2 < slots && tiles > 4ll * ca::kMaxCluster * ca::kWarps;
-    if (prefix_len > 0 || (fits && few)) {
-        s.shares = fits ? (int)std::min<long long>(slots, (s.items * tiles + ca::kWarps - 1) / ca::kWarps) : -1;
-        return s;
-    }
-    s.split = 1;
-    while (s.split < ca::kMaxCluster && s.items * (s.split + 1) <= slots && tiles > (long long)s.split * ca::kWarps) ++s.split;
-    s.by_length = s.items > slots && B <= 256;
-    return s;
-}
-
 // How the prefix's part is cut: one CTA per SM, each with a block of query rows of a K/V head and an
 // even stretch of the prefix.  Two Q tiles per CTA, so that keys are converted once for 256 rows,
 // where there are more than 128 rows; fp32 queries take both tiles' memory for their two parts.
@@ -165,6 +133,40 @@ PrefixPlan plan_prefix(int B, int T, int heads, int kv_heads, int q_f32, int pre
     s.split = (int)std::max<long long>(1, std::min<long long>(s.tiles, kPlanSms / groups));
     return s;
 }
+// How the attention's work is cut.
+struct AttnPlan {
+    int form;         // query rows per item: rows_of(form)
+    long long items;  // (sequence, K/V head, rows)
+    int split;        // CTAs per item (split_kernel), or
+    bool by_length;   // longest sequences first (split_kernel)
+    int shares;       // CTAs of stream_kernel, which join_kernel follows (0: split_kernel)
+};
+
+// split_kernel, with as many CTAs per item as the GPU holds at once, up to a cluster, and no more
+// than there are tiles for; stream_kernel where that leaves most of the GPU idle: few items with
+// many keys.  (8 x 131071 keys: 71 us shared by 444 CTAs, 149 us in 8 clusters of 8.)
+// Behind a prefix, split_kernel also joins its rows with the prefix's n_shared parts, if these are few.
+AttnPlan plan_attn(int B, int T, int heads, int kv_heads, int q_f32, int page_size, int max_pages, int n_shared) {
+    namespace ca = dt::cache_attn;
+    AttnPlan s{};
+    const int rows = T * (heads / kv_heads);
+    s.form = rows <= 4 ? ca::kFew : q_f32 || rows <= 8 ? ca::kEight : ca::kWide;
+    s.items = (long long)B * kv_heads * ((rows + ca::rows_of(s.form) - 1) / ca::rows_of(s.form));
+    const long long tiles = ((long long)max_pages * page_size + ca::kTile - 1) / ca::kTile;
+    const int slots = ca::ctas_per_sm(q_f32, s.form) * kPlanSms;
+    const bool fits = B <= ca::kMaxBatch && tiles * B < 0x7fffffffll && s.items < 0x7fffffffll - slots;
+    const bool few = s.items * ca::kMaxCluster * 2 < slots && tiles > 4ll * ca::kMaxCluster * ca::kWarps;
+    if (max_pages == 0) return s;  // no keys of their own: join_kernel alone
+    if (n_shared > 16 || (fits && few)) {
+        s.shares = fits ? (int)std::min<long long>(slots, (s.items * tiles + ca::kWarps - 1) / ca::kWarps) : -1;
+        return s;
+    }
+    s.split = 1;
+    while (s.split < ca::kMaxCluster && s.items * (s.split + 1) <= slots && tiles > (long long)s.split * ca::kWarps) ++s.split;
+    s.by_length = s.items > slots && B <= 256 && tiles >= 64;  // (ranking the lengths takes a microsecond)
+    return s;
+}
+
 constexpr size_t kPrefixSmem = sizeof(dt::prefix_attn::Smem) + 1024;
 
 // Workspace of a plan: the tile counts, the CTAs' parts, the prefix's parts.
@@ -303,14 +305,13 @@ int cache_attn(const dt_kv_cache* cache, const void* q, long long q_batch_stride
     p.heads = heads;
     p.group = heads / cache->kv_heads;
     p.scale = scale;
-    AttnPlan plan = plan_attn(B, T, heads, cache->kv_heads, q_f32, cache->page_size, max_pages, prefix_len);
-    if (max_pages == 0) plan.shares = plan.split = 0;  // no keys of their own
+    const PrefixPlan prefix = prefix_len > 0 ? plan_prefix(B, T, heads, cache->kv_heads, q_f32, prefix_len) : PrefixPlan{};
+    const AttnPlan plan = plan_attn(B, T, heads, cache->kv_heads, q_f32, cache->page_size, max_pages, prefix.split);
     if (plan.shares < 0)
         return fail(DT_ERR_INVALID_ARGUMENT, "behind a prefix, B must be at most %d and the page table below 2^31 tokens",
                     dt::cache_attn::kMaxBatch);
     if (plan.items * std::max(plan.split, 1) > 0x7fffffffll)
         return fail(DT_ERR_INVALID_ARGUMENT, "B * kv_heads * query rows is too large");
-    const PrefixPlan prefix = prefix_len > 0 ? plan_prefix(B, T, heads, cache->kv_heads, q_f32, prefix_len) : PrefixPlan{};
     const AttnSpace space = attn_space(plan, B, T, heads, prefix.split);
     if (space.total > 0 && (!workspace || workspace_bytes < space.total || !aligned16(workspace)))
         return fail(DT_ERR_INVALID_ARGUMENT, "workspace must be >= %zu bytes and 16-byte aligned", space.total);
@@ -327,8 +328,8 @@ int cache_attn(const dt_kv_cache* cache, const void* q, long long q_batch_stride
     p.part_o = reinterpret_cast<float*>(w + space.part_o);
     p.shared_s = reinterpret_cast<float4*>(w + space.shared_s);
     p.shared_o = reinterpret_cast<float*>(w + space.shared_o);
-    if (plan.split > 0) return launch_split(attn_kernel_of(false, cache->format, q_f32, plan.form), p, plan.items, st);
     if (prefix_len > 0) DT_TRY(launch_prefix(p, prefix, cache->format, q_f32, st));
+    if (plan.split > 0) return launch_split(attn_kernel_of(false, cache->format, q_f32, plan.form), p, plan.items, st);
     return launch_stream(p, plan, cache->format, q_f32, st);
 }
 
@@ -357,9 +358,8 @@ size_t dt_prefix_attn_workspace_bytes(int B, int T, int heads, int kv_heads, int
     if (prefix_len <= 0) return dt_cache_attn_workspace_bytes(B, T, heads, kv_heads, q_f32, page_size, max_pages);
     if (B <= 0 || T <= 0 || kv_heads <= 0 || heads < kv_heads || page_size <= 0 || max_pages < 0) return 0;
     if ((long long)B * T * heads > 0x7fffffffll) return 0;
-    AttnPlan plan = plan_attn(B, T, heads, kv_heads, q_f32, page_size, max_pages, prefix_len);
-    if (max_pages == 0) plan.shares = plan.split = 0;
-    return attn_space(plan, B, T, heads, plan_prefix(B, T, heads, kv_heads, q_f32, prefix_len).split).total;
+    const int n_shared = plan_prefix(B, T, heads, kv_heads, q_f32, prefix_len).split;
+    return attn_space(plan_attn(B, T, heads, kv_heads, q_f32, page_size, max_pages, n_shared), B, T, heads, n_shared).total;
 }
 
 int dt_prefix_attn_fwd(const dt_kv_cache* cache, const void* q, long long q_batch_stride, long long q_token_stride,
