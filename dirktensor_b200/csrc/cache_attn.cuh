@@ -16,6 +16,10 @@ namespace cache_attn {
 
 constexpr int kD = 128;
 
+// Query row r of a K/V head is query head r % group of token r / group.  (A group of one, the model's own case,
+// spares the division, which takes some 30 instructions that are run for a few tiles only.)
+__device__ __forceinline__ int token_of(int r, int group) { return group == 1 ? r : (int)((unsigned)r / (unsigned)group); }
+
 struct Params {
     kv::Cache c;
     const void* q;
@@ -255,8 +259,8 @@ __device__ __forceinline__ void attend(const Params& p, Stage* ring, int b, int 
     for (int z = 0; z < kSets; ++z) {
         const int r = row0 + (kCols == 1 ? g >> 1 : g) + 8 * z;
         const bool in = r < p.T * p.group && (kCols == 2 || !(g & 1));
-        const int tq = in ? r / p.group : 0;
-        const int h = hk * p.group + (in ? r % p.group : 0);
+        const int tq = in ? token_of(r, p.group) : 0;
+        const int h = hk * p.group + (in ? r - tq * p.group : 0);
         const long long at = (long long)b * p.q_batch + (long long)tq * p.q_token + (long long)h * kD + 16 * t;
         const uint4* src = kF32 ? reinterpret_cast<const uint4*>(static_cast<const float*>(p.q) + at)
                                 : reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.q) + at);
@@ -291,7 +295,7 @@ __device__ __forceinline__ void attend(const Params& p, Stage* ring, int b, int 
 #pragma unroll
         for (int c = 0; c < kCols; ++c) {
             const int r = row0 + kCols * t + c + 8 * z;
-            const int tq = r / p.group;
+            const int tq = token_of(r, p.group);
             lim[z][c] = tq < q_len ? (int)max(0ll, min(base + tq, cap)) : 0;
             if (r >= p.T * p.group) lim[z][c] = 0x7fffffff;  // (a column that no query fills: nothing to mask, and never stored)
             else keys = max(keys, lim[z][c]);
@@ -614,12 +618,12 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kF32, kForm)) split_kern
     extern __shared__ __align__(16) uint8_t smem_raw[];
     Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rank = (int)(blockIdx.x % (unsigned)p.split);
-    const int item = (int)(blockIdx.x / (unsigned)p.split);
+    const int item = p.split == 1 ? (int)blockIdx.x : (int)(blockIdx.x / (unsigned)p.split);
+    const int rank = (int)blockIdx.x - item * p.split;
     const int per_head = (p.T * p.group + kRows - 1) / kRows;
-    const int hk = item / per_head % p.c.heads;
-    const int row0 = item % per_head * kRows;
-    int b = item / per_head / p.c.heads;
+    const int of_head = per_head == 1 ? item : (int)((unsigned)item / (unsigned)per_head);
+    int b = (int)((unsigned)of_head / (unsigned)p.c.heads);
+    const int hk = of_head - b * p.c.heads, row0 = (item - of_head * per_head) * kRows;
     if (p.by_length) {  // the b-th longest, ties by number: every thread ranks its sequences
         int* lens = reinterpret_cast<int*>(&sm.ring);
         for (int i = threadIdx.x; i < p.B; i += kThreads) lens[i] = p.seq_lens[i];
@@ -664,10 +668,11 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kF32, kForm)) split_kern
             y.add(other->om[row], other->ol[row], best,
                   reinterpret_cast<const float4*>(other->joined(row))[lane]);
         }
-        const long long out = ((long long)b * p.T + rr / p.group) * p.heads + hk * p.group + rr % p.group;
+        const int tq = token_of(rr, p.group);
+        const long long out = ((long long)b * p.T + tq) * p.heads + hk * p.group + rr - tq * p.group;
         // the prefix's parts (at most 16: all of them on their way at once)
         const int q_len = p.q_lens ? min(p.q_lens[b], p.T) : p.T;
-        const int shared = rr / p.group < q_len ? p.n_shared : 0;
+        const int shared = tq < q_len ? p.n_shared : 0;
         if (shared > 0) {
             const long long all = (long long)p.B * p.T * p.heads;
             float4 s = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);

@@ -103,11 +103,13 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const Params pp) {
     Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    const int part = (int)(blockIdx.x % (unsigned)pp.split);
-    const int block = (int)(blockIdx.x / (unsigned)pp.split) % pp.blocks;
-    const int hk = (int)(blockIdx.x / (unsigned)pp.split) / pp.blocks;
+    const int group = (int)(blockIdx.x / (unsigned)pp.split);
+    const int part = (int)blockIdx.x - group * pp.split;
+    const int hk = (int)((unsigned)group / (unsigned)pp.blocks), block = group - hk * pp.blocks;
     const int row0 = block * (pp.pairs ? kBM : 2 * kBM);
-    const int t0 = (int)((long long)pp.tiles * part / pp.split), t1 = (int)((long long)pp.tiles * (part + 1) / pp.split);
+    // (tiles and parts are at most 2^24 and 148)
+    const int t0 = (int)((unsigned)pp.tiles / (unsigned)pp.split) * part + min(part, (int)((unsigned)pp.tiles % (unsigned)pp.split));
+    const int t1 = t0 + (int)((unsigned)pp.tiles / (unsigned)pp.split) + (part < (int)((unsigned)pp.tiles % (unsigned)pp.split) ? 1 : 0);
     const int n = t1 - t0;  // at least one: split <= tiles
     const bool second_rows = !pp.pairs && row0 + kBM < pp.rows;
     // steps of warpgroup i: its s-th one is tile s, or 2 s + i
@@ -313,15 +315,23 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const Params pp) {
         {
             const int qtiles = pp.pairs ? 1 : 2;
             const int per_warp = kBM * qtiles / 8;
+            long long mine;  // where row `lane` of this warp's starts; -1: there is none
+            {
+                const int row = row0 + warp * per_warp + lane;
+                const int bt = cache_attn::token_of(row, p.group);
+                const int b = cache_attn::token_of(bt, p.T);
+                mine = row < pp.rows && lane < per_warp ? (long long)b * p.q_batch + (long long)(bt - b * p.T) * p.q_token +
+                                                              ((long long)hk * p.group + (row - bt * p.group)) * kD
+                                                        : -1;
+            }
+#pragma unroll 1
             for (int rr = 0; rr < per_warp; rr += 8) {
                 float x[8][4];
 #pragma unroll
                 for (int u = 0; u < 8; ++u) {
-                    const int row = row0 + warp * per_warp + rr + u;
-                    const bool in = row < pp.rows;
-                    const int bt = in ? row / p.group : 0;
-                    const long long at = (long long)(bt / p.T) * p.q_batch + (long long)(bt % p.T) * p.q_token +
-                                         ((long long)hk * p.group + (in ? row % p.group : 0)) * kD + 4 * lane;
+                    const long long from = __shfl_sync(0xffffffffu, mine, rr + u);
+                    const bool in = from >= 0;
+                    const long long at = from + 4 * lane;
                     if (kF32) {
                         const float4 y = in ? __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + at))
                                             : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -521,9 +531,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const Params pp) {
         if (i == 0 || !pp.pairs) {
             const int row = row0 + (pp.pairs ? 0 : i * kBM) + r;
             const bool in = row < pp.rows && have;
-            const int bt = in ? row / p.group : 0;
+            const int bt = in ? cache_attn::token_of(row, p.group) : 0;
             const long long rows = (long long)p.B * p.T * p.heads;
-            const long long at = (long long)part * rows + (long long)bt * p.heads + (long long)hk * p.group + (in ? row % p.group : 0);
+            const long long at = (long long)part * rows + (long long)bt * p.heads + (long long)hk * p.group + (in ? row - bt * p.group : 0);
             float a0 = inv, a1 = 0.f, best = m, sum = l, big = mx;
             const bool both = pp.pairs && steps[1] > 0;
             if (both) {
