@@ -36,8 +36,9 @@ constexpr int kBM = 128;                   // rows of a Q tile
 constexpr int kBN = 128;                   // keys of a tile
 constexpr int kTileBytes = 128 * kD * 2;   // fp16
 constexpr int kHalfBytes = kTileBytes / 2; // 64 dims: one swizzle span
-constexpr int kThreads = 416;
 constexpr int kConvWarps = 4;
+constexpr int kMmaWarp = 8 + kConvWarps;
+constexpr int kThreads = (kMmaWarp + 1) * 32;
 constexpr float kGrow = 8.f;               // log2 units, as in flash_fwd.cuh
 
 struct Params {
@@ -82,6 +83,13 @@ __device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
     return r;
 }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// Waits for this thread's TMEM loads; x is valid afterwards, and the compiler uses it no earlier.
+__device__ __forceinline__ void wait_for(float (&x)[32]) {
+    tmem_wait_ld();
+#pragma unroll
+    for (int e = 0; e < 32; ++e) asm volatile("" : "+f"(x[e]));
+}
 
 // A 16-byte piece of codes (16 dims of one key) as fp16: two 16-byte chunks of a swizzled tile.  The
 // lanes of the second half of the dims store theirs in the other order (`swap`): no bank conflicts.
@@ -129,7 +137,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const Params pp) {
         mbar_init(&sm.mma_done, 1);
         fence_mbar_init();
     }
-    if (warp == 12) {
+    if (warp == kMmaWarp) {
         tmem_alloc(&sm.tmem_base, 512);
         tmem_relinquish();
     }
@@ -138,26 +146,29 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const Params pp) {
     tc_fence_after();
     const uint32_t tmem = sm.tmem_base;
 
-    if (warp >= 8 && warp < 12) {
+    if (warp >= 8 && warp < kMmaWarp) {
         // ------------------------------ convert -----------------------------
         const int cw = warp - 8;
         const int shift = p.c.page_shift, in_page = (1 << shift) - 1;
-        // this warp's 32 keys of a tile are two groups of 16, each on one page
-        auto page_of = [&](int tile, int g) {
-            const int key = tile * kBN + cw * 32 + g * 16;
+        // this warp's 32 keys of a tile are two groups of 16, each on one page: lanes 0-15 and 16-31 look up one
+        auto look_up = [&](int tile) {
+            const int key = tile * kBN + cw * 32 + (lane & 16);
             const int page = key < p.prefix_len ? __ldg(p.prefix_pages + (key >> shift)) : -1;
             return page >= 0 && page < p.c.pages ? page : -1;
         };
         // lane: piece lane & 7 of rows 4 i + lane / 8
         const int rl = lane >> 3, piece = lane & 7;
-        auto load = [&](const uint8_t* codes, int tile, const int (&page)[2], uint4 (&x)[8]) {
-            const int key0 = tile * kBN + cw * 32;
+        // row of the cache where group g of a tile starts
+        auto row_at = [&](int tile, int page, int g) {
+            return ((uint32_t)(page * p.c.heads + hk) << shift) + ((tile * kBN + cw * 32 + 16 * g) & in_page);
+        };
+        auto load = [&](const uint8_t* codes, int tile, int pages, uint4 (&x)[8]) {
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
-                // hidden keys: zeros (a page that does not exist hides all 16)
-                const int left = page[g] >= 0 ? p.prefix_len - (key0 + 16 * g) : 0;
-                const uint32_t row = ((uint32_t)(page[g] * p.c.heads + hk) << shift) + ((key0 + 16 * g) & in_page);
-                const uint4* src = reinterpret_cast<const uint4*>(codes + (size_t)row * kD) + rl * (kD / 16) + piece;
+                const int page = __shfl_sync(0xffffffffu, pages, 16 * g);
+                // hidden keys: zeros
+                const int left = page >= 0 ? p.prefix_len - (tile * kBN + cw * 32 + 16 * g) : 0;
+                const uint4* src = reinterpret_cast<const uint4*>(codes + (size_t)row_at(tile, page, g) * kD) + rl * (kD / 16) + piece;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     x[4 * g + i] = 4 * i + rl < left ? __ldg(src + i * 4 * (kD / 16)) : make_uint4(0, 0, 0, 0);
@@ -178,32 +189,23 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const Params pp) {
             for (int i = 0; i < 8; ++i)
                 put_piece<kFmt>(base + off[i & 1][0] + (i >> 1) * 1024, base + off[i & 1][1] + (i >> 1) * 1024, swap, x[i]);
         };
-        // scales of a tile, one key a lane
-        auto load_scales = [&](int tile, const int (&page)[2], float& k, float& v, bool& see) {
-            const int key = tile * kBN + cw * 32 + lane;
-            const int pg = lane < 16 ? page[0] : page[1];
-            see = pg >= 0 && key < p.prefix_len;
-            k = 1.f, v = 0.f;  // (a hidden key's score becomes -inf)
-            if (see) {
-                const uint32_t row = ((uint32_t)(pg * p.c.heads + hk) << shift) + (key & in_page);
-                k = __ldg(p.c.ks + row);
-                v = __ldg(p.c.vs + row);
-            }
+        // scales of a tile, one key a lane (a hidden key's score becomes -inf)
+        auto load_scales = [&](int tile, int page, float& k, float& v, bool& see) {
+            see = page >= 0 && tile * kBN + cw * 32 + lane < p.prefix_len;
+            const uint32_t row = row_at(tile, page, lane >> 4) + (lane & 15);
+            k = see ? __ldg(p.c.ks + row) : 1.f;
+            v = see ? __ldg(p.c.vs + row) : 0.f;
         };
         // Pieces in the order K0, K1, V0, K2, V1, ...: a tile's codes are on their way while the tile before
-        // is converted, and its page numbers for a tile longer.
-        bool ok = true;
+        // is converted, and its page number for a tile longer.
+        bool ok = true, see;
         uint4 xk[8], xv[8];
         float ks, vs;
-        bool see;
-        int page0[2], page1[2], page2[2];  // of tiles j, j + 1, j + 2
-        auto look_up = [&](int tile, int (&page)[2]) { page[0] = page_of(tile, 0), page[1] = page_of(tile, 1); };
-        look_up(t0, page0);
-        look_up(t0 + 1, page1);
+        int page0 = look_up(t0), page1 = look_up(t0 + 1), page2;  // of tiles j, j + 1, j + 2
         load(p.c.k, t0, page0, xk);
         load_scales(t0, page0, ks, vs, see);
         load(p.c.v, t0, page0, xv);
-        look_up(t0 + 2, page2);
+        page2 = look_up(t0 + 2);
 #pragma unroll 1
         for (int j = 0; j <= n; ++j) {
             const int s = j & 1;
@@ -213,7 +215,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const Params pp) {
                 sm.ks[j & 3][cw * 32 + lane] = ks;
                 sm.vs[j & 3][cw * 32 + lane] = vs;
                 // (scales are not negative, so their bits order as they do; a NaN is not a largest)
-                const uint32_t most = __reduce_max_sync(0xffffffffu, vs == vs && vs > 0.f ? __float_as_uint(vs) : 0u);
+                const uint32_t most = __reduce_max_sync(0xffffffffu, vs > 0.f ? __float_as_uint(vs) : 0u);
                 const uint32_t seen = __ballot_sync(0xffffffffu, see);
                 if (lane == 0) sm.most[j & 3][cw] = __uint_as_float(most), sm.hidden[j & 3][cw] = ~seen;
                 put(sm.k[s], xk);
@@ -235,11 +237,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const Params pp) {
                 if (lane == 0) mbar_arrive(&sm.v_full[i & 1]);
                 if (j < n) load(p.c.v, t0 + j, page0, xv);
             }
-            page0[0] = page1[0], page0[1] = page1[1];
-            page1[0] = page2[0], page1[1] = page2[1];
-            look_up(t0 + j + 3, page2);
+            page0 = page1, page1 = page2;
+            page2 = look_up(t0 + j + 3);
         }
-    } else if (warp == 12) {
+    } else if (warp == kMmaWarp) {
         // ------------------------------ MMA issue ---------------------------
         if (lane == 0) {
             constexpr uint32_t idesc_qk = idesc_f16(kBM, kBN, 0);
@@ -252,27 +253,31 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const Params pp) {
             auto want_v = [&](int t) {
                 for (; ok && v_seen <= t; ++v_seen) ok = mbar_wait_sleep(&sm.v_full[v_seen & 1], (v_seen >> 1) & 1, kSiteVFull);
             };
+            // descriptors of the tiles' starts; offsets add to their address fields (in 16 bytes)
+            const uint64_t q_desc = umma_desc_sw128(smem_u32(sm.q[0]), 16, 1024);
+            const uint64_t k_desc = umma_desc_sw128(smem_u32(sm.k[0]), 16, 1024);
+            const uint64_t v_desc = umma_desc_sw128(smem_u32(sm.v[0]), kHalfBytes, 1024);
+            constexpr uint64_t kTileStep = kTileBytes >> 4;
             auto issue_s = [&](int i, int t) {
-                const uint32_t k = smem_u32(sm.k[t & 1]);
-                const uint32_t q = smem_u32(sm.q[0]) + (pp.pairs ? 0u : (uint32_t)i * kTileBytes);
+                const uint64_t k = k_desc + (t & 1) * kTileStep, q = q_desc + (pp.pairs ? 0 : i * kTileStep);
 #pragma unroll
                 for (int half = 0; half < (kF32 ? 2 : 1); ++half)
 #pragma unroll
                     for (int kk = 0; kk < kD / 16; ++kk) {
-                        const uint32_t off = (kk >> 2) * kHalfBytes + (kk & 3) * 32;
-                        umma_ss(tmem + i * 128, umma_desc_sw128(q + half * kTileBytes + off, 16, 1024),
-                                umma_desc_sw128(k + off, 16, 1024), idesc_qk, kk > 0 || half > 0 ? 1u : 0u);
+                        constexpr uint64_t kHalfStep = kHalfBytes >> 4;
+                        const uint64_t off = (kk >> 2) * kHalfStep + (kk & 3) * 2;
+                        umma_ss(tmem + i * 128, q + half * kTileStep + off, k + off, idesc_qk, kk > 0 || half > 0 ? 1u : 0u);
                     }
                 umma_commit(&sm.s_full[i]);
             };
             auto issue_pv = [&](int i, int t, bool add) {
-                const uint32_t v = smem_u32(sm.v[t & 1]);
+                const uint64_t v = v_desc + (t & 1) * kTileStep;
 #pragma unroll
                 for (int half = 0; half < (kF32 ? 2 : 1); ++half)
 #pragma unroll
                     for (int kk = 0; kk < kBN / 16; ++kk)
                         umma_ts(tmem + 256 + i * 128, tmem + i * 128 + (kF32 ? (kk >> 1) * 32 + half * 16 + (kk & 1) * 8 : kk * 8),
-                                umma_desc_sw128(v + kk * 2048, kHalfBytes, 1024), idesc_pv, (add || kk > 0 || half > 0) ? 1u : 0u);
+                                v + kk * (2048 >> 4), idesc_pv, (add || kk > 0 || half > 0) ? 1u : 0u);
             };
             auto tile_of = [&](int i, int s) { return pp.pairs ? 2 * s + i : s; };
             for (int i = 0; i < 2; ++i)
@@ -311,68 +316,67 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const Params pp) {
     } else {
         // ------------------------------ softmax -----------------------------
         const int i = warp >> 2;  // warpgroup
-        // The Q rows, a warp per row: 16 rows of each Q tile per warp.
+        // The Q rows: 16 of a Q tile per warp and round, two lanes a row, 64 dims each.  (Few instructions: they
+        // run once, and are fetched for that.)
         {
-            const int qtiles = pp.pairs ? 1 : 2;
-            const int per_warp = kBM * qtiles / 8;
-            long long mine;  // where row `lane` of this warp's starts; -1: there is none
-            {
-                const int row = row0 + warp * per_warp + lane;
+#pragma unroll 1
+            for (int z = 0; z < (pp.pairs ? 1 : 2); ++z) {
+                const int r = warp * 16 + (lane >> 1);  // row of the tile
+                const int half = lane & 1;
+                const int row = row0 + z * kBM + r;
+                const bool in = row < pp.rows;
                 const int bt = cache_attn::token_of(row, p.group);
                 const int b = cache_attn::token_of(bt, p.T);
-                mine = row < pp.rows && lane < per_warp ? (long long)b * p.q_batch + (long long)(bt - b * p.T) * p.q_token +
-                                                              ((long long)hk * p.group + (row - bt * p.group)) * kD
-                                                        : -1;
-            }
-#pragma unroll 1
-            for (int rr = 0; rr < per_warp; rr += 8) {
-                float x[8][4];
+                const long long at = (long long)b * p.q_batch + (long long)(bt - b * p.T) * p.q_token +
+                                     ((long long)hk * p.group + (row - bt * p.group)) * kD + 64 * half;
+                constexpr int kPieces = kF32 ? 16 : 8;
+                const uint4* src = kF32 ? reinterpret_cast<const uint4*>(static_cast<const float*>(p.q) + at)
+                                        : reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.q) + at);
+                uint4 x[kPieces];
 #pragma unroll
-                for (int u = 0; u < 8; ++u) {
-                    const long long from = __shfl_sync(0xffffffffu, mine, rr + u);
-                    const bool in = from >= 0;
-                    const long long at = from + 4 * lane;
-                    if (kF32) {
-                        const float4 y = in ? __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + at))
-                                            : make_float4(0.f, 0.f, 0.f, 0.f);
-                        x[u][0] = y.x, x[u][1] = y.y, x[u][2] = y.z, x[u][3] = y.w;
-                    } else {
-                        const uint2 y = in ? __ldg(reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(p.q) + at))
-                                           : make_uint2(0, 0);
-                        x[u][0] = __uint_as_float(y.x << 16), x[u][1] = __uint_as_float(y.x & 0xffff0000u);
-                        x[u][2] = __uint_as_float(y.y << 16), x[u][3] = __uint_as_float(y.y & 0xffff0000u);
+                for (int i = 0; i < kPieces; ++i) x[i] = in ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
+                // largest magnitude as an integer: infinities and NaNs order above every finite value
+                uint32_t top = 0;
+#pragma unroll
+                for (int i = 0; i < kPieces; ++i) {
+                    const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        top = max(top, w[e] & 0x7fffffffu);
+                        if (!kF32) top = max(top, (w[e] << 16) & 0x7fffffffu);
                     }
                 }
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                if (!kF32) top &= 0xffff0000u;  // (the lower value's bits below an upper one's)
+                const bool finite = top < 0x7f800000u;
+                const int ex = finite ? max(exponent(__uint_as_float(top)), -100) : 0;
+                // (a negative scale changes the queries' sign, so that factor stays positive)
+                const float mul = finite ? (p.scale < 0.f ? -pow2(13 - ex) : pow2(13 - ex)) : 0.f;
+                if (half == 0) sm.factor[z][r] = finite ? pow2(ex - 13) * fabsf(p.scale) * kLog2e : __uint_as_float(0x7fffffffu);
+                const uint32_t dst = smem_u32(sm.q[z]) + (uint32_t)half * kHalfBytes + (uint32_t)r * 128;
 #pragma unroll
-                for (int u = 0; u < 8; ++u) {
-                    const int local = warp * per_warp + rr + u;  // row of the CTA
-                    uint32_t top = 0;
+                for (int c = 0; c < 8; ++c) {  // 16-byte chunks of the tile: 8 dims
+                    float y[8];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(x[u][e]) & 0x7fffffffu);
-                    top = __reduce_max_sync(0xffffffffu, top);
-                    const bool finite = top < 0x7f800000u;
-                    const int ex = finite ? max(exponent(__uint_as_float(top)), -100) : 0;
-                    // (a negative scale changes the queries' sign, so that factor stays positive)
-                    const float mul = finite ? (p.scale < 0.f ? -pow2(13 - ex) : pow2(13 - ex)) : 0.f;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) x[u][e] = finite ? x[u][e] * mul : 0.f;
-                    const int r = local & (kBM - 1);
-                    const int c = lane >> 1;
-                    const uint32_t addr = smem_u32(sm.q[pp.pairs ? 0 : local >> 7]) + (uint32_t)(c >> 3) * kHalfBytes + (uint32_t)r * 128 +
-                                          (((uint32_t)(c & 7) ^ (uint32_t)(r & 7)) << 4) + (uint32_t)(lane & 1) * 8;
-                    uint32_t hi0, hi1, lo0 = 0, lo1 = 0;
-                    if (kF32) {
-                        cache_attn::split_pair(x[u][0], x[u][1], hi0, lo0);
-                        cache_attn::split_pair(x[u][2], x[u][3], hi1, lo1);
-                        asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(addr + kTileBytes), "r"(lo0), "r"(lo1) : "memory");
-                    } else {
-                        hi0 = half_pair(x[u][0], x[u][1]);
-                        hi1 = half_pair(x[u][2], x[u][3]);
+                    for (int e = 0; e < 4; ++e) {
+                        if (kF32) {
+                            const uint4 u = x[(2 * c + (e >> 1)) % kPieces];
+                            y[2 * e] = __uint_as_float(e & 1 ? u.z : u.x), y[2 * e + 1] = __uint_as_float(e & 1 ? u.w : u.y);
+                        } else {
+                            const uint32_t w = e == 0 ? x[c].x : e == 1 ? x[c].y : e == 2 ? x[c].z : x[c].w;
+                            y[2 * e] = __uint_as_float(w << 16), y[2 * e + 1] = __uint_as_float(w & 0xffff0000u);
+                        }
                     }
-                    asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(addr), "r"(hi0), "r"(hi1) : "memory");
-                    if (lane == 0)
-                        sm.factor[pp.pairs ? 0 : local >> 7][r] =
-                            finite ? pow2(ex - 13) * fabsf(p.scale) * kLog2e : __uint_as_float(0x7fffffffu);
+                    uint32_t hi[4], lo[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float y0 = finite ? y[2 * e] * mul : 0.f, y1 = finite ? y[2 * e + 1] * mul : 0.f;
+                        if (kF32) cache_attn::split_pair(y0, y1, hi[e], lo[e]);
+                        else hi[e] = half_pair(y0, y1);
+                    }
+                    const uint32_t to = dst + ((uint32_t)(c ^ (r & 7)) << 4);
+                    st_shared_v4(to, hi[0], hi[1], hi[2], hi[3]);
+                    if (kF32) st_shared_v4(to + kTileBytes, lo[0], lo[1], lo[2], lo[3]);
                 }
             }
             fence_async();
@@ -400,7 +404,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const Params pp) {
             }
             tc_fence_after();
             const int at = (pp.pairs ? 2 * s + i : s) & 3;
-            const bool some = (sm.hidden[at][0] | sm.hidden[at][1] | sm.hidden[at][2] | sm.hidden[at][3]) != 0u;
+            const uint4 hidden = *reinterpret_cast<const uint4*>(sm.hidden[at]);
+            const bool some = (hidden.x | hidden.y | hidden.z | hidden.w) != 0u;
             if (some) {  // the last tile, or a page that does not exist: hidden scores become -inf
 #pragma unroll 1
                 for (int cc = 0; cc < 8; ++cc) {
@@ -415,13 +420,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const Params pp) {
                 }
                 tmem_wait_st();
             }
-            // first pass: the row's largest score
+            // first pass: the row's largest score (the next 32 columns are on their way while 32 are looked at)
             float top = -INFINITY;
-#pragma unroll 1
-            for (int cc = 0; cc < 4; ++cc) {
-                float x[32];
-                tmem_ld32(tS + cc * 32, x);
-                tmem_wait_ld();
+            float xa[32], xb[32];
+            auto largest = [&](const float(&x)[32], int cc) {
                 float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                 for (int e = 0; e < 32; e += 4) {
@@ -432,6 +434,16 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const Params pp) {
                     best[(e >> 2) & 3] = fmax3(best[(e >> 2) & 3], fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
                 }
                 top = fmax3(top, fmaxf(best[0], best[1]), fmaxf(best[2], best[3]));
+            };
+            tmem_ld32(tS, xa);
+#pragma unroll 1
+            for (int cc = 0; cc < 4; cc += 2) {
+                wait_for(xa);
+                tmem_ld32(tS + cc * 32 + 32, xb);
+                largest(xa, cc);
+                wait_for(xb);
+                tmem_ld32(tS + ((cc * 32 + 64) & 127), xa);  // (the last: column 0 again, for the second pass)
+                largest(xb, cc + 1);
             }
             top *= factor;  // (-inf where every key is hidden; factor is not negative)
             if (top != top) top = -INFINITY;  // (a row whose query is not finite: no maximum)
@@ -462,11 +474,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const Params pp) {
             const float m_safe = (m == -INFINITY ? 0.f : m) - (float)fe;
             const uint64_t c2 = f2_pack(factor, factor), nm2 = f2_pack(-m_safe, -m_safe);
             uint64_t sum2[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
-#pragma unroll 1
-            for (int cc = 0; cc < 4; ++cc) {
-                float x[32];
-                tmem_ld32(tS + cc * 32, x);
-                tmem_wait_ld();
+            auto weigh = [&](const float(&x)[32], int cc) {
                 uint32_t hi[16], lo[kF32 ? 16 : 1];
 #pragma unroll
                 for (int e = 0; e < 32; e += 4) {
@@ -492,6 +500,15 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const Params pp) {
                 // P takes the columns of scores that have been read: chunk cc's 16 (and the rests' 16 behind them)
                 tmem_st16(tS + cc * (kF32 ? 32 : 16), hi);
                 if (kF32) tmem_st16(tS + cc * 32 + 16, *reinterpret_cast<uint32_t(*)[16]>(lo));
+            };
+#pragma unroll 1
+            for (int cc = 0; cc < 4; cc += 2) {
+                wait_for(xa);
+                tmem_ld32(tS + cc * 32 + 32, xb);
+                weigh(xa, cc);
+                wait_for(xb);
+                if (cc == 0) tmem_ld32(tS + 64, xa);
+                weigh(xb, cc + 1);
             }
             float s0, s1;
             f2_unpack(f2_add(sum2[0], sum2[1]), s0, s1);
@@ -572,7 +589,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const Params pp) {
 
     tc_fence_before();
     __syncthreads();
-    if (warp == 12) {
+    if (warp == kMmaWarp) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
