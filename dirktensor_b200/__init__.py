@@ -38,7 +38,8 @@ def __getattr__(name):
     if name in _SERVING:
         from . import serving
 
-        return getattr(serving, name)
+        globals().update({n: getattr(serving, n) for n in _SERVING})
+        return globals()[name]
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 

@@ -10,7 +10,6 @@ CrossEntropyLoss.cpp:8-43 reduces the loss to one number.
 from __future__ import annotations
 
 import ctypes
-from contextlib import nullcontext
 from typing import NamedTuple, Optional
 
 import torch
@@ -23,46 +22,59 @@ _FORMAT_OF = {torch.int8: 0, torch.float8_e4m3fn: 1}
 _VALUES = (torch.bfloat16, torch.float32)
 
 
-def _on(device: torch.device):
-    """The library works on the current device: makes it the tensors' own."""
-    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+# A decoding step's calls take a few microseconds on the GPU, so the checks below look at each
+# tensor as few times as they can.
+_current_device = torch._C._cuda_getDevice
+_current_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+def _call(index: int, function, *args) -> None:
+    """Calls an entry point on the current stream of device `index`, which is made the current device."""
+    if _current_device() == index:
+        status = function(*args, _current_stream(index))
+    else:
+        with torch.cuda.device(index):
+            status = function(*args, _current_stream(index))
+    if status:
+        check(status)
 
 
-def _values(name: str, t, device, heads: Optional[int] = None):
-    """[B, T, heads, 128] of bf16 or fp32 whose rows start on 16-byte boundaries."""
-    if not (isinstance(t, torch.Tensor) and t.device == device and t.dtype in _VALUES and t.dim() == 4
-            and t.shape[3] == head_dim):
-        raise ValueError(f"{name} must be a bfloat16 or float32 tensor [B, T, heads, {head_dim}] on {device}")
-    if heads is not None and t.shape[2] != heads:
+def _index_of(t) -> int:
+    """The device of a CUDA tensor, -1 for anything else."""
+    return t.get_device() if isinstance(t, torch.Tensor) else -1
+
+
+def _values(name: str, t, index: int, heads: Optional[int] = None):
+    """Shape and strides of [B, T, heads, 128] of bf16 or fp32 whose rows start on 16-byte boundaries."""
+    if _index_of(t) != index or t.dtype not in _VALUES or t.dim() != 4 or t.shape[3] != head_dim:
+        raise ValueError(f"{name} must be a bfloat16 or float32 tensor [B, T, heads, {head_dim}] on cuda:{index}")
+    shape, s = t.shape, t.stride()
+    if heads is not None and shape[2] != heads:
         raise ValueError(f"{name} must have {heads} heads")
-    s = t.stride()
-    if (t.numel() and (s[3] != 1 or (t.shape[2] > 1 and s[2] != head_dim) or (s[0] | s[1]) % (16 // t.element_size())
-                       or s[0] < 0 or s[1] < 0 or t.data_ptr() & 15)):
+    if ((s[3] != 1 or (s[2] != head_dim and shape[2] > 1) or (s[0] | s[1]) % (16 // t.element_size()) or s[0] < 0
+         or s[1] < 0 or t.data_ptr() & 15) and t.numel()):
         raise ValueError(f"{name}: heads must be {head_dim} apart, and rows must start on 16-byte boundaries")
-    return s
+    return shape, s
 
 
-def _ints(name: str, t, device, n: Optional[int]):
+def _ints(name: str, t, index: int, n: Optional[int]):
     if t is None:
         return None
-    if not (isinstance(t, torch.Tensor) and t.device == device and t.dtype == torch.int32 and t.dim() == 1
-            and (n is None or t.shape[0] == n) and (t.shape[0] < 2 or t.stride(0) == 1)):
-        raise ValueError(f"{name} must be a contiguous int32 tensor{'' if n is None else f' of {n} entries'} on {device}")
+    if (_index_of(t) != index or t.dtype != torch.int32 or t.dim() != 1 or (n is not None and t.shape[0] != n)
+            or not t.is_contiguous()):
+        raise ValueError(f"{name} must be a contiguous int32 tensor{'' if n is None else f' of {n} entries'} "
+                         f"on cuda:{index}")
     return t.data_ptr()
 
 
-def _table(t, device, B: int):
-    if not (isinstance(t, torch.Tensor) and t.device == device and t.dtype == torch.int32 and t.dim() == 2
-            and t.shape[0] == B):
-        raise ValueError(f"page_table must be an int32 tensor [{B}, pages] on {device}")
+def _table(t, index: int, B: int):
+    if _index_of(t) != index or t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] != B:
+        raise ValueError(f"page_table must be an int32 tensor [{B}, pages] on cuda:{index}")
     n = t.shape[1]
-    if (n > 1 and t.stride(1) != 1) or (B > 1 and t.stride(0) < n):
+    row, column = t.stride()
+    if (n > 1 and column != 1) or (B > 1 and row < n):
         raise ValueError("page_table rows must be contiguous and must not overlap")
-    return t.data_ptr(), max(t.stride(0), n), n
+    return t.data_ptr(), max(row, n), n
 
 
 class KVCache:
@@ -106,7 +118,7 @@ class KVCache:
         self.num_pages, self.kv_heads, self.page_size = k.shape[:3]
         if self.page_size not in (16, 32, 64, 128, 256):
             raise ValueError("page_size must be 16, 32, 64, 128 or 256")
-        self.device = k.device
+        self.device, self._index = k.device, k.get_device()
         self._c = dt_kv_cache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), self.num_pages,
                               self.page_size, self.kv_heads, _FORMAT_OF[k.dtype])
         self._ref = ctypes.byref(self._c)
@@ -120,41 +132,58 @@ class KVCache:
         of sequence b at position start[b] + t.  start, lens: int32 [B] tensors (default 0 and
         T).  Tokens without a valid page are skipped; where the page table gives two tokens of
         the call one slot, the one of the highest (sequence, position) is kept."""
-        ks, vs = _values("k", k, self.device, self.kv_heads), _values("v", v, self.device, self.kv_heads)
+        (B, T, _, _), ks = _values("k", k, self._index, self.kv_heads)
+        _, vs = _values("v", v, self._index, self.kv_heads)
         if k.shape != v.shape or k.dtype != v.dtype:
             raise ValueError("k and v differ in shape or type")
-        B, T = k.shape[:2]
-        table, stride, n = _table(page_table, self.device, B)
-        with _on(self.device):
-            check(lib().dt_kv_cache_append(self._ref, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
-                                           int(k.dtype == torch.float32), table, stride, n,
-                                           _ints("start", start, self.device, B), _ints("lens", lens, self.device, B),
-                                           B, T, _stream(self.device)))
+        table, stride, n = _table(page_table, self._index, B)
+        _call(self._index, lib().dt_kv_cache_append, self._ref, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
+              k.dtype == torch.float32, table, stride, n, _ints("start", start, self._index, B),
+              _ints("lens", lens, self._index, B), B, T)
 
     def read(self, page_table, start, T: int, lens=None, dtype=torch.bfloat16):
         """The values of positions start[b] .. start[b] + T - 1 as k, v [B, T, kv_heads, 128] of
         ``dtype`` (bf16 or fp32).  Rows t >= lens[b] and positions without a valid page are zeros."""
         if dtype not in _VALUES:
             raise ValueError("dtype must be bfloat16 or float32")
-        B = page_table.shape[0]
-        table, stride, n = _table(page_table, self.device, B)
-        k = torch.empty((B, int(T), self.kv_heads, head_dim), dtype=dtype, device=self.device)
+        if not isinstance(page_table, torch.Tensor) or page_table.dim() != 2:
+            raise ValueError("page_table must be an int32 tensor [B, pages]")
+        B, T = page_table.shape[0], int(T)
+        table, stride, n = _table(page_table, self._index, B)
+        k = torch.empty((B, T, self.kv_heads, head_dim), dtype=dtype, device=self.device)
         v = torch.empty_like(k)
-        with _on(self.device):
-            check(lib().dt_kv_cache_read(self._ref, k.data_ptr(), v.data_ptr(), int(dtype == torch.float32), table,
-                                         stride, n, _ints("start", start, self.device, B),
-                                         _ints("lens", lens, self.device, B), B, int(T), _stream(self.device)))
+        _call(self._index, lib().dt_kv_cache_read, self._ref, k.data_ptr(), v.data_ptr(), dtype == torch.float32, table,
+              stride, n, _ints("start", start, self._index, B), _ints("lens", lens, self._index, B), B, T)
         return k, v
 
 
-def _outputs(q, out, return_stats):
+def _outputs(q, shape, out, return_stats):
+    """Output and statistics tensors, and their addresses."""
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    elif not (out.device == q.device and out.dtype == q.dtype and out.shape == q.shape and out.is_contiguous()):
+        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+    elif not (out.device == q.device and out.dtype == q.dtype and out.shape == shape and out.is_contiguous()):
         raise ValueError("out must be a contiguous tensor of q's shape and type")
     if not return_stats:
-        return out, None, None
-    return out, *(torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) for _ in range(2))
+        return out, None, None, out.data_ptr(), None, None
+    m, l = (torch.empty(shape[:3], dtype=torch.float32, device=q.device) for _ in range(2))
+    return out, m, l, out.data_ptr(), m.data_ptr(), l.data_ptr()
+
+
+_workspace_bytes: dict = {}
+
+
+def _workspace(cache, *sizes):
+    """A workspace of its own for each call (from torch's caching allocator, which knows streams and
+    captured graphs), and its address and size."""
+    nbytes = _workspace_bytes.get(sizes)
+    if nbytes is None:
+        if len(_workspace_bytes) > 4096:
+            _workspace_bytes.clear()
+        nbytes = _workspace_bytes[sizes] = (lib().dt_prefix_attn_workspace_bytes(*sizes))
+    if nbytes == 0:
+        return None, None, 0
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=cache.device)
+    return ws, ws.data_ptr(), nbytes
 
 
 def cache_attention_forward(q, cache: KVCache, page_table, seq_lens, scale: float, q_lens=None, out=None,
@@ -167,19 +196,16 @@ def cache_attention_forward(q, cache: KVCache, page_table, seq_lens, scale: floa
     and come back as zeros, as do rows that see no key.  Returns the output [B, T, heads, 128]
     of q's type, or with return_stats a ``FlashAttentionResult`` with softmax_m and softmax_l.
     """
-    s = _values("q", q, cache.device)
-    B, T, H = q.shape[:3]
-    table, stride, n = _table(page_table, cache.device, B)
-    lens = _ints("seq_lens", seq_lens, cache.device, B)
-    o, m, l = _outputs(q, out, return_stats)
-    f32, L = int(q.dtype == torch.float32), lib()
-    nbytes = L.dt_cache_attn_workspace_bytes(B, T, H, cache.kv_heads, f32, cache.page_size, n)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=cache.device) if nbytes else None
-    with _on(cache.device):
-        check(L.dt_cache_attn_fwd(cache._ref, q.data_ptr(), s[0], s[1], f32, o.data_ptr(),
-                                  m.data_ptr() if return_stats else None, l.data_ptr() if return_stats else None,
-                                  table, stride, n, lens, _ints("q_lens", q_lens, cache.device, B), B, T, H,
-                                  float(scale), ws.data_ptr() if nbytes else None, nbytes, _stream(cache.device)))
+    index = cache._index
+    shape, s = _values("q", q, index)
+    B, T, H, _ = shape
+    table, stride, n = _table(page_table, index, B)
+    lens = _ints("seq_lens", seq_lens, index, B)
+    f32 = q.dtype == torch.float32
+    o, m, l, po, pm, pl = _outputs(q, shape, out, return_stats)
+    ws, pw, nbytes = _workspace(cache, B, T, H, cache.kv_heads, f32, cache.page_size, n, 0)
+    _call(index, lib().dt_cache_attn_fwd, cache._ref, q.data_ptr(), s[0], s[1], f32, po, pm, pl, table, stride, n, lens,
+          _ints("q_lens", q_lens, index, B), B, T, H, scale, pw, nbytes)
     return FlashAttentionResult(o, m, l) if return_stats else o
 
 
@@ -190,26 +216,22 @@ def prefix_attention_forward(q, cache: KVCache, prefix_pages, prefix_len: int, p
     page_table and seq_lens describe what follows the prefix in each sequence; both may be None when
     nothing does.
     """
-    s = _values("q", q, cache.device)
-    B, T, H = q.shape[:3]
+    index = cache._index
+    shape, s = _values("q", q, index)
+    B, T, H, _ = shape
     prefix_len = int(prefix_len)
-    pages = _ints("prefix_pages", prefix_pages, cache.device, None)
+    pages = _ints("prefix_pages", prefix_pages, index, None)
     if prefix_len < 0 or prefix_len > (0 if prefix_pages is None else prefix_pages.shape[0] * cache.page_size):
         raise ValueError("prefix_len must be >= 0 and within prefix_pages")
     if (page_table is None) != (seq_lens is None):
         raise ValueError("page_table and seq_lens come together")
-    table, stride, n = (None, 0, 0) if page_table is None else _table(page_table, cache.device, B)
-    lens = _ints("seq_lens", seq_lens, cache.device, B)
-    o, m, l = _outputs(q, out, return_stats)
-    f32, L = int(q.dtype == torch.float32), lib()
-    nbytes = L.dt_prefix_attn_workspace_bytes(B, T, H, cache.kv_heads, f32, cache.page_size, n, prefix_len)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=cache.device) if nbytes else None
-    with _on(cache.device):
-        check(L.dt_prefix_attn_fwd(cache._ref, q.data_ptr(), s[0], s[1], f32, o.data_ptr(),
-                                   m.data_ptr() if return_stats else None, l.data_ptr() if return_stats else None,
-                                   pages, prefix_len, table, stride, n, lens,
-                                   _ints("q_lens", q_lens, cache.device, B), B, T, H, float(scale),
-                                   ws.data_ptr() if nbytes else None, nbytes, _stream(cache.device)))
+    table, stride, n = (None, 0, 0) if page_table is None else _table(page_table, index, B)
+    lens = _ints("seq_lens", seq_lens, index, B)
+    f32 = q.dtype == torch.float32
+    o, m, l, po, pm, pl = _outputs(q, shape, out, return_stats)
+    ws, pw, nbytes = _workspace(cache, B, T, H, cache.kv_heads, f32, cache.page_size, n, prefix_len)
+    _call(index, lib().dt_prefix_attn_fwd, cache._ref, q.data_ptr(), s[0], s[1], f32, po, pm, pl, pages, prefix_len, table,
+          stride, n, lens, _ints("q_lens", q_lens, index, B), B, T, H, scale, pw, nbytes)
     return FlashAttentionResult(o, m, l) if return_stats else o
 
 
@@ -227,7 +249,7 @@ def _rows(name, t):
         raise ValueError(f"{name} must be a bfloat16 or float32 CUDA tensor [..., vocabulary]")
     V = t.shape[-1]
     if t.is_contiguous():
-        return t.numel() // V, V
+        return (t.shape[0] if t.dim() == 2 else t.numel() // V), V
     n, ld = 1, None
     if V == 1 or t.stride(-1) == 1:
         for size, stride in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
@@ -267,16 +289,18 @@ def token_log_probs(logits, targets=None, top: int = 0) -> TokenLogProbs:
     top = int(top)
     if not 0 <= top <= min(32, V):
         raise ValueError("top must be 0..32 and at most the vocabulary")
-    lp = torch.empty(shape, dtype=torch.float32, device=dev) if targets is not None else None
-    ent, lse = torch.empty(shape, dtype=torch.float32, device=dev), torch.empty(shape, dtype=torch.float32, device=dev)
+    # one allocation for the three results of a row, one for its alternatives' log probabilities
+    three = torch.empty((3,) + shape, dtype=torch.float32, device=dev)
+    lse, ent, lp = three.unbind(0)
+    at = three.data_ptr()
     ids = tlp = None
     if top:
         ids = torch.empty(shape + (top,), dtype=torch.int32, device=dev)
         tlp = torch.empty(shape + (top,), dtype=torch.float32, device=dev)
-    with _on(dev):
-        check(lib().dt_token_log_probs(logits.data_ptr(), int(logits.dtype == torch.float32), ld, n, V, t, t64, top,
-                                       lp.data_ptr() if t else None, ent.data_ptr(), lse.data_ptr(),
-                                       ids.data_ptr() if top else None, tlp.data_ptr() if top else None, _stream(dev)))
+    _call(logits.get_device(), lib().dt_token_log_probs, logits.data_ptr(), logits.dtype == torch.float32, ld, n, V, t, t64, top,
+          at + 8 * n if t else None, at + 4 * n, at, ids.data_ptr() if top else None, tlp.data_ptr() if top else None)
+    if targets is None:
+        lp = None
     return TokenLogProbs(lp, ent, lse, ids, tlp)
 
 
@@ -303,8 +327,6 @@ def token_log_probs_backward(logits, targets, lse, entropy, d_log_prob, d_entrop
         raise ValueError("out must have the logits' shape and type")
     dn, dld = _rows("out", out)
     ptr = lambda x: None if x is None else x.data_ptr()  # noqa: E731
-    with _on(dev):
-        check(lib().dt_token_log_probs_bwd(logits.data_ptr(), int(logits.dtype == torch.float32), ld, n, V, t, t64,
-                                           lse.data_ptr(), ptr(entropy), ptr(d_log_prob), ptr(d_entropy),
-                                           out.data_ptr(), dld, _stream(dev)))
+    _call(logits.get_device(), lib().dt_token_log_probs_bwd, logits.data_ptr(), logits.dtype == torch.float32, ld, n, V, t,
+          t64, lse.data_ptr(), ptr(entropy), ptr(d_log_prob), ptr(d_entropy), out.data_ptr(), dld)
     return out
