@@ -75,6 +75,12 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return r;
 }
 
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
 // The logit's bits in an order that unsigned numbers share, NaN lowest; -0 and 0 alike.
 __device__ __forceinline__ uint32_t order_bits(float x) {
     const uint32_t u = __float_as_uint(x + 0.f);
@@ -128,7 +134,8 @@ __device__ __forceinline__ K merged_over_warps(K x, int n, K (*scratch)[32]) {
 
 // s = sum e^(x - m), u = sum (x - m) e^(x - m), relative to m.
 struct Sums {
-    float m = kLowest, s = 0.f, u = 0.f;
+    float m, s, u;
+    static __device__ __forceinline__ Sums none() { return {kLowest, 0.f, 0.f}; }
     __device__ __forceinline__ void move_to(float mn) {  // mn >= m
         const float d = max_nan(m - mn, kFar);
         const float e = ex2_approx(d * kLog2e);
@@ -189,19 +196,26 @@ struct Row {
     }
 };
 
+constexpr int kGroups = kThreads / 8;     // of threads, whose largest logits bound the k-th
+constexpr int kCandidates = 512;
+
 struct Smem {
     unsigned long long list[kWarps][32];
+    unsigned long long found[kCandidates];  // logits that reach the threshold
+    unsigned long long best[32];            // the CTA's alternatives
     Sums sums[kWarps];
-    Sums total;                         // of this CTA, for the cluster
-    unsigned long long best[32];        // its alternatives
+    Sums total;                             // of the CTA, for the cluster
+    float groups[kGroups];
     float threshold;
+    int count;
 };
 
-// A cluster of `split` CTAs per row (one, unless the rows are too few to fill the GPU).  One pass
-// gives the sums and every thread's largest logit.  The k-th largest of these is no larger than the
-// row's k-th largest logit, so the alternatives all lie with threads whose largest reaches it: about k of
-// 512, whose logits alone are read again (from L2).  Bound by the read: at V = 100352 fp32 a CTA
-// has 400 KB to read per row and spends about 9 instructions a logit.
+// A cluster of `split` CTAs per row (one, unless the rows are too few to fill the GPU).  One pass gives the
+// sums and every thread's largest logit.  The k-th largest of 64 groups' largest logits is no larger than
+// the row's k-th largest logit, so the alternatives all lie with threads whose largest logit reaches it: about k
+// of 512.  Each of these reads the 16 logits around its largest again, or, where another of its batches
+// reaches the threshold too, its warp reads all of its logits.  What reaches the threshold is collected
+// and sorted by one warp; rows with more than 512 such logits (ties) are sorted by all warps instead.
 template <bool kF32>
 __global__ void __launch_bounds__(kThreads, 3) row_kernel(const Params p) {
     pdl_enter();
@@ -209,89 +223,135 @@ __global__ void __launch_bounds__(kThreads, 3) row_kernel(const Params p) {
     constexpr int kN = Vec<kF32>::kN;
     constexpr int kBatch = 16 / kN;  // vectors at a time
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int row = (int)(blockIdx.x / (unsigned)p.split), rank = (int)(blockIdx.x % (unsigned)p.split);
+    const int row = p.split == 1 ? (int)blockIdx.x : (int)(blockIdx.x / (unsigned)p.split), rank = (int)blockIdx.x - row * p.split;
     const Row<kF32> r(p.x, (long long)row * p.ld, p.V);
     const int vectors = r.vectors();
     const int begin = (int)((long long)vectors * rank / p.split), end = (int)((long long)vectors * (rank + 1) / p.split);
-
-    Sums a;
-    float most = -INFINITY;  // this thread's largest logit, and whether it saw a NaN
-    bool odd = false;
-    auto take = [&](const float(&x)[16]) {
-        float top[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) top[i] = max_nan(max_nan(x[4 * i], x[4 * i + 1]), max_nan(x[4 * i + 2], x[4 * i + 3]));
-        const float t = max_nan(max_nan(top[0], top[1]), max_nan(top[2], top[3]));
-        odd |= t != t;
-        most = fmaxf(most, t);
-        a.move_to(max_nan(a.m, t));
-        float s[4] = {0.f, 0.f, 0.f, 0.f}, u[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const float d = max_nan(x[i] - a.m, kFar);
-            const float e = ex2_approx(d * kLog2e);
-            s[i & 3] += e;
-            u[i & 3] = fmaf(d, e, u[i & 3]);
-        }
-        a.s += (s[0] + s[1]) + (s[2] + s[3]);
-        a.u += (u[0] + u[1]) + (u[2] + u[3]);
-    };
-    // whole batches; the edges and what is left behind the last batch are taken below
+    // whole vectors; the first and the last may cross the row's ends
     const int lo = begin + (r.inside(begin) ? 0 : 1), hi = end - (end > begin && r.inside(end - 1) ? 0 : 1);
-    int v = lo + threadIdx.x;
-    for (; v + (kBatch - 1) * kThreads < hi; v += kBatch * kThreads) {
-        uint4 y[kBatch];
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) y[i] = r.load(v + i * kThreads);
-        float x[16];
+    // thread 0 takes the share's first vector and thread 1 its last, where they do
+    const int edge = threadIdx.x == 0 && lo > begin ? begin : threadIdx.x == 1 && hi < end && hi >= lo ? hi : -1;
+
+    Sums a = Sums::none();
+    float most = -INFINITY, next = -INFINITY;  // this thread's largest logit, and that of its other batches
+    int where = 0;                             // first vector of the batch that has it
+    bool odd = false;                          // it saw a NaN
+    auto take = [&](const uint4 (&y)[kBatch], int v) {
+        uint64_t x[8];  // pairs
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
-            const Vec<kF32> z = Row<kF32>::unpack(y[i]);
+            const uint32_t w[4] = {y[i].x, y[i].y, y[i].z, y[i].w};
 #pragma unroll
-            for (int e = 0; e < kN; ++e) x[i * kN + e] = z.x[e];
+            for (int e = 0; e < kN / 2; ++e)
+                x[i * (kN / 2) + e] = kF32 ? f2_pack(__uint_as_float(w[2 * e % 4]), __uint_as_float(w[(2 * e + 1) % 4]))
+                                           : f2_pack(__uint_as_float(w[e % 4] << 16), __uint_as_float(w[e % 4] & 0xffff0000u));
         }
-        take(x);
-    }
-    {
-        uint4 y[kBatch];
-        const uint32_t none = kF32 ? 0xff800000u : 0xff80ff80u;  // -inf
+        float t = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            float x0, x1, x2, x3;
+            f2_unpack(x[i], x0, x1);
+            f2_unpack(x[i + 1], x2, x3);
+            t = max_nan(t, max_nan(max3_nan(x0, x1, x2), x3));
+        }
+        odd |= t != t;
+        const bool larger = t > most;
+        next = fmaxf(next, larger ? most : t);
+        where = larger ? v : where;
+        most = larger ? t : most;
+        if (!(t <= a.m)) a.move_to(max_nan(a.m, t));  // (a NaN too)
+        const uint64_t minus = f2_pack(-a.m, -a.m);
+        uint64_t s = f2_pack(0.f, 0.f), u = f2_pack(0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float d0, d1;
+            f2_unpack(f2_add(x[i], minus), d0, d1);
+            d0 = max_nan(d0, kFar), d1 = max_nan(d1, kFar);
+            const uint64_t e = f2_pack(ex2_approx(d0 * kLog2e), ex2_approx(d1 * kLog2e));
+            s = f2_add(s, e);
+            u = f2_fma(f2_pack(d0, d1), e, u);
+        }
+        float s0, s1, u0, u1;
+        f2_unpack(s, s0, s1);
+        f2_unpack(u, u0, u1);
+        a.s += s0 + s1;
+        a.u += u0 + u1;
+    };
+    const uint32_t none = kF32 ? 0xff800000u : 0xff80ff80u;  // -inf
+    auto fetch = [&](uint4 (&y)[kBatch], int v) {
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) y[i] = v + i * kThreads < hi ? r.load(v + i * kThreads) : make_uint4(none, none, none, none);
+    };
+    if (kF32) {
+        int v = lo + threadIdx.x;
+        for (; v + (kBatch - 1) * kThreads < hi; v += kBatch * kThreads) {
+            uint4 y[kBatch];
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) y[i] = r.load(v + i * kThreads);
+            take(y, v);
+        }
         if (v < hi) {
-            float x[16];
-#pragma unroll
-            for (int i = 0; i < kBatch; ++i) {
-                const Vec<kF32> z = Row<kF32>::unpack(y[i]);
-#pragma unroll
-                for (int e = 0; e < kN; ++e) x[i * kN + e] = z.x[e];
-            }
-            take(x);
+            uint4 y[kBatch];
+            fetch(y, v);
+            take(y, v);
         }
-        // thread 0 takes the share's first vector and thread 1 its last, where they cross the row's ends
-        const bool first = threadIdx.x == 0 && lo > begin, last = threadIdx.x == 1 && hi < end && hi >= lo;
-        if (first || last) {
-            const Vec<kF32> z = r.edge(first ? begin : hi);
-            float x[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) x[e] = e < kN ? z.x[e % kN] : -INFINITY;
-            take(x);
+    } else {  // two vectors a batch: the next batch is on its way while this one is added up
+        uint4 y[kBatch], z[kBatch];
+        fetch(y, lo + threadIdx.x);
+        for (int v = lo + threadIdx.x; v < hi; v += 2 * kBatch * kThreads) {
+            fetch(z, v + kBatch * kThreads);
+            take(y, v);
+            fetch(y, v + 2 * kBatch * kThreads);
+            if (v + kBatch * kThreads < hi) take(z, v + kBatch * kThreads);
         }
+    }
+    if (edge >= 0) {
+        const Vec<kF32> z = r.edge(edge);
+        uint4 y[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) y[i] = make_uint4(none, none, none, none);
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            w[e] = kF32 ? __float_as_uint(z.x[e % kN]) : (__float_as_uint(z.x[2 * e % kN]) >> 16) | __float_as_uint(z.x[(2 * e + 1) % kN]);
+        y[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        take(y, edge);
+        next = most;  // (its batch is not as the others': all of its logits are read again)
     }
 
     if (p.top > 0) {
         // a logit that the row's k-th largest reaches
-        const uint32_t k = merged_over_warps<uint32_t>(sorted(order_bits(most)), kWarps, reinterpret_cast<uint32_t(*)[32]>(sm.list));
+        float top = most;
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if ((lane & 7) == 0) sm.groups[threadIdx.x >> 3] = top;
+        if (threadIdx.x == 0) sm.count = 0;
         __syncthreads();
-        if (threadIdx.x == p.top - 1) sm.threshold = from_order_bits(k);
+        if (threadIdx.x < kGroups) {
+            const float mine = sm.groups[threadIdx.x];
+            int above = 0;
+#pragma unroll 8
+            for (int j = 0; j < kGroups; ++j) {
+                const float x = sm.groups[j];
+                above += x > mine || (x == mine && j < (int)threadIdx.x);
+            }
+            if (above == p.top - 1) sm.threshold = mine;
+        }
         __syncthreads();
         const float threshold = sm.threshold;
-        unsigned long long list = 0, least = 0;  // this warp's alternatives, and its k-th
-        uint32_t todo = __ballot_sync(0xffffffffu, odd || most >= threshold);
-        while (todo) {  // the warp reads one thread's vectors again, a lane each
-            const int who = warp * 32 + __ffs(todo) - 1;
-            todo &= todo - 1;
+        // (at -inf everything counts, NaNs too)
+        auto reaches = [&](float x, int id) { return id >= 0 && id < p.V && (x >= threshold || threshold == -INFINITY); };
+        auto collect = [&](float x, int id) {
+            if (reaches(x, id)) {
+                const int at = atomicAdd(&sm.count, 1);
+                if (at < kCandidates) sm.found[at] = order_key(x, id);
+            }
+        };
+        // reads all vectors of thread `who` again, a lane each, and calls each(element, key of this lane or 0)
+        auto again = [&](int who, auto each) {
             const int extra = who == 0 && lo > begin ? begin : who == 1 && hi < end && hi >= lo ? hi : -1;
             const int n = (hi - lo - who + kThreads - 1) / kThreads + (extra >= 0 ? 1 : 0);
+#pragma unroll 1
             for (int i0 = 0; i0 < n; i0 += 32) {
                 const int i = i0 + lane;
                 const int mine = i >= n ? -1 : extra >= 0 && i == n - 1 ? extra : lo + who + i * kThreads;
@@ -300,18 +360,41 @@ __global__ void __launch_bounds__(kThreads, 3) row_kernel(const Params p) {
                 for (int e = 0; e < kN; ++e) z.x[e] = -INFINITY;
                 if (mine >= 0) z = mine == extra ? r.edge(mine) : Row<kF32>::unpack(r.load(mine));
 #pragma unroll
-                for (int e = 0; e < kN; ++e) {
-                    const int id = r.id(mine, e);
-                    const bool in = mine >= 0 && id >= 0 && id < p.V && (z.x[e] >= threshold || threshold == -INFINITY);
-                    const unsigned long long key = in ? order_key(z.x[e], id) : 0ull;
+                for (int e = 0; e < kN; ++e) each(z.x[e], mine >= 0 ? r.id(mine, e) : -1);
+            }
+        };
+        const bool flagged = odd || most >= threshold;
+        const bool all = odd || next >= threshold;
+        if (flagged && !all) {
+            uint4 y[kBatch];
+            fetch(y, where);
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                const Vec<kF32> z = Row<kF32>::unpack(y[i]);
+#pragma unroll
+                for (int e = 0; e < kN; ++e) collect(z.x[e], where + i * kThreads < hi ? r.id(where + i * kThreads, e) : -1);
+            }
+        }
+        for (uint32_t todo = __ballot_sync(0xffffffffu, flagged && all); todo; todo &= todo - 1)
+            again(warp * 32 + __ffs(todo) - 1, collect);
+        __syncthreads();
+        const int count = sm.count;
+        unsigned long long list = 0;
+        if (count <= kCandidates) {
+            if (warp == 0)
+                for (int i = 0; i < count; i += 32) list = merged(list, sorted(i + lane < count ? sm.found[i + lane] : 0ull));
+        } else {
+            unsigned long long least = 0;  // this warp's k-th
+            for (uint32_t todo = __ballot_sync(0xffffffffu, flagged); todo; todo &= todo - 1)
+                again(warp * 32 + __ffs(todo) - 1, [&](float x, int id) {
+                    const unsigned long long key = reaches(x, id) ? order_key(x, id) : 0ull;
                     if (__any_sync(0xffffffffu, key > least)) {
                         list = merged(list, sorted(key));
                         least = __shfl_sync(0xffffffffu, list, p.top - 1);
                     }
-                }
-            }
+                });
+            list = merged_over_warps(list, kWarps, sm.list);
         }
-        list = merged_over_warps(list, kWarps, sm.list);
         if (warp == 0) sm.best[lane] = list;
     }
 
@@ -326,36 +409,51 @@ __global__ void __launch_bounds__(kThreads, 3) row_kernel(const Params p) {
     }
     if (lane == 0) sm.sums[warp] = a;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        Sums b = sm.sums[0];
+    if (warp == 0) {
+        a = lane < kWarps ? sm.sums[lane] : Sums::none();
 #pragma unroll
-        for (int w = 1; w < kWarps; ++w) b.add(sm.sums[w]);
-        sm.total = b;
+        for (int o = kWarps / 2; o > 0; o >>= 1) {
+            Sums b;
+            b.m = __shfl_xor_sync(0xffffffffu, a.m, o);
+            b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
+            b.u = __shfl_xor_sync(0xffffffffu, a.u, o);
+            a.add(b);
+        }
+        if (lane == 0) sm.total = a;
     }
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
     if (p.split > 1) cluster.sync();
-    else __syncthreads();
-    if (rank == 0) {
-        Sums b = sm.total;
-        for (int c = 1; c < p.split; ++c) b.add(cluster.map_shared_rank(&sm, c)->total);
-        const bool empty = b.s == 0.f;  // every logit is -inf
-        const float ls = logf(b.s);
-        if (threadIdx.x == 0) {
+    if (rank == 0 && warp == 0) {
+        if (p.split > 1) {  // a lane per CTA
+            a = lane < p.split ? cluster.map_shared_rank(&sm, lane)->total : Sums::none();
+#pragma unroll
+            for (int o = kMaxCluster / 2; o > 0; o >>= 1) {
+                Sums b;
+                b.m = __shfl_xor_sync(0xffffffffu, a.m, o);
+                b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
+                b.u = __shfl_xor_sync(0xffffffffu, a.u, o);
+                a.add(b);
+            }
+        }
+        a.m = __shfl_sync(0xffffffffu, a.m, 0), a.s = __shfl_sync(0xffffffffu, a.s, 0), a.u = __shfl_sync(0xffffffffu, a.u, 0);
+        const bool empty = a.s == 0.f;  // every logit is -inf
+        const float ls = logf(a.s);
+        if (lane == 0) {
             const long long t = target_of(p.targets, p.targets64, row);
             float lp = 0.f;
-            if (t >= 0 && t < p.V) lp = empty ? -INFINITY : (logit<kF32>(p.x, (long long)row * p.ld + t) - b.m) - ls;
+            if (t >= 0 && t < p.V) lp = empty ? -INFINITY : (logit<kF32>(p.x, (long long)row * p.ld + t) - a.m) - ls;
             if (p.log_prob) p.log_prob[row] = lp;
-            if (p.entropy) p.entropy[row] = empty ? 0.f : ls - b.u / b.s;
-            if (p.lse) p.lse[row] = empty ? -INFINITY : b.m + ls;
+            if (p.entropy) p.entropy[row] = empty ? 0.f : ls - a.u / a.s;
+            if (p.lse) p.lse[row] = empty ? -INFINITY : a.m + ls;
         }
         if (p.top > 0) {
-            unsigned long long list = warp < p.split ? (p.split > 1 ? cluster.map_shared_rank(&sm, warp)->best[lane] : sm.best[lane]) : 0ull;
-            list = merged_over_warps(list, kMaxCluster, sm.list);
-            if (threadIdx.x < p.top) {
+            unsigned long long list = sm.best[lane];
+            for (int c = 1; c < p.split; ++c) list = merged(list, cluster.map_shared_rank(&sm, c)->best[lane]);
+            if (lane < p.top) {
                 const float x = from_order_bits((uint32_t)(list >> 32));
                 p.top_ids[(long long)row * p.top + lane] = 0x7fffffff - (int)(uint32_t)list;
-                p.top_log_probs[(long long)row * p.top + lane] = empty ? -INFINITY : (x - b.m) - ls;
+                p.top_log_probs[(long long)row * p.top + lane] = empty ? -INFINITY : (x - a.m) - ls;
             }
         }
     }

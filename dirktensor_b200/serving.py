@@ -160,7 +160,7 @@ class KVCache:
 def _outputs(q, shape, out, return_stats):
     """Output and statistics tensors, and their addresses."""
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q) if q.is_contiguous() else torch.empty(shape, dtype=q.dtype, device=q.device)
     elif not (out.device == q.device and out.dtype == q.dtype and out.shape == shape and out.is_contiguous()):
         raise ValueError("out must be a contiguous tensor of q's shape and type")
     if not return_stats:
