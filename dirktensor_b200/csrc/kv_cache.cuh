@@ -74,15 +74,16 @@ __device__ __forceinline__ int position(int start, int t) {
 // lanes share the entries: lane `part` of `parts`.
 __device__ __forceinline__ bool written_above(const Span& s, const Cache& c, int b, int j0, int pos, int page, int part,
                                               int parts) {
-    const int width = (s.T >> c.page_shift) + 2;  // pages that one sequence's T tokens can touch
-    const long long n = (long long)(s.B - b) * width;
+    const unsigned width = (unsigned)(s.T >> c.page_shift) + 2u;  // pages that one sequence's T tokens can touch
+    const unsigned n = (unsigned)(s.B - b) * width;               // (below 2^31: B * T is)
     const int off = pos & ((1 << c.page_shift) - 1);
-    for (long long i = part; i < n; i += parts) {
-        const int b2 = b + (int)(i / width);
+    for (unsigned i = part; i < n; i += parts) {
+        const unsigned skip = i / width;
+        const int b2 = b + (int)skip;
         const int len = s.lens ? min(s.lens[b2], s.T) : s.T;
         const long long first = s.start ? s.start[b2] : 0, last = first + len - 1;
         if (len <= 0) continue;
-        const long long j = (first >> c.page_shift) + i % width;
+        const long long j = (first >> c.page_shift) + (i - skip * width);
         if (j < 0 || j > (last >> c.page_shift) || j >= s.max_pages || (b2 == b && j <= j0)) continue;
         if (__ldg(s.table + (long long)b2 * s.table_stride + j) != page) continue;
         const long long at = (j << c.page_shift) + off;
@@ -91,19 +92,39 @@ __device__ __forceinline__ bool written_above(const Span& s, const Cache& c, int
     return false;
 }
 
-// Codes of four values: round(x * mul / den), mul / den = Q / amax.
+// Codes of four values: round(x * mul / den), mul / den = Q / amax, inv = 1 / den.
+// int8: x * mul * inv is within three units of fp32's last place of the rounded quotient, so its code is the
+// quotient's unless a border between two codes is as near: then, for one value in some 10,000, the quotient
+// itself is formed (25 us instead of 30 for 131072 rows).  e4m3's borders lie at many distances, and
+// looking for them takes longer than the division (32 us instead of 28).
 template <int kFmt>
-__device__ __forceinline__ uint32_t encode4(const float (&x)[4], float mul, float den) {
-    uint32_t w = 0;
+__device__ __forceinline__ uint32_t encode4(const float (&x)[4], float mul, float den, float inv) {
+    constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: the sum's low byte is the rounded value
+    float y[4];
+    if constexpr (kFmt == kInt8) {
+        bool near = false;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float y = __fdiv_rn(__fmul_rn(x[i], mul), den);
-        uint32_t c;
-        if (kFmt == kInt8) c = (uint32_t)__float2int_rn(y) & 0xffu;
-        else c = (uint32_t)__nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
-        w |= c << (8 * i);
+        for (int i = 0; i < 4; ++i) {
+            y[i] = __fmul_rn(__fmul_rn(x[i], mul), inv);
+            // |y| <= 127 and a bit: three units of its last place are below 2.3e-5
+            const float whole = __fsub_rn(__fadd_rn(y[i], kMagic), kMagic);
+            near |= fabsf(__fsub_rn(y[i], whole)) > 0.49995f;
+        }
+        if (near) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] = __fdiv_rn(__fmul_rn(x[i], mul), den);
+        }
+        uint32_t c[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c[i] = __float_as_uint(__fadd_rn(y[i], kMagic));
+        return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = __fdiv_rn(__fmul_rn(x[i], mul), den);
+        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3);
+        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3);
+        return lo | (hi << 16);
     }
-    return w;
 }
 
 // Four codes to fp32 (exact: both formats' values have at most 8 significant bits).
@@ -146,82 +167,94 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendParams p) 
     if (t0 >= t1) return;
     const int start = p.s.start ? p.s.start[b] : 0;
     const int lane = threadIdx.x & (kRowLanes - 1);
-    const int rows = (t1 - t0) * 2 * p.c.heads;
+    const int per_token = 2 * p.c.heads;
+    const int rows = (t1 - t0) * per_token;
     // Does a later token of this call write one of this tile's pages?  (A tile is at most a
-    // page long, so it touches two pages at most.)  Almost always not.
-    bool contested = false;
-    {
+    // page long, so it touches two pages at most.)  Almost always not.  (Asked while the first
+    // rows are on their way.)
+    auto ask = [&] {
         const int first = position(start, t0), last = position(start, t1 - 1);
         const int pa = page_of(p.s, p.c, b, first), pb = page_of(p.s, p.c, b, last);
         const int ja = first >> p.c.page_shift, jb = last >> p.c.page_shift;
+        bool contested = false;
         if (pa >= 0) contested = written_above(p.s, p.c, b, ja, -1, pa, threadIdx.x, kThreads);
         if (pb >= 0 && jb != ja) contested |= written_above(p.s, p.c, b, jb, -1, pb, threadIdx.x, kThreads);
-        contested = __syncthreads_or(contested) != 0;
-    }
+        return __syncthreads_or(contested) != 0;
+    };
+    // A row of 8 lanes: K or V of head h of a token; the next one is 32 rows on.
+    const int token_step = (int)((unsigned)kRows / (unsigned)per_token), rest_step = kRows - token_step * per_token;
+    int r = threadIdx.x >> 3;
+    int t = t0 + (int)((unsigned)r / (unsigned)per_token);
+    int rest = r - (t - t0) * per_token;
+    constexpr int kPieces = kF32 ? 4 : 2, kSize = kF32 ? 4 : 2;
+    const char* k_src = static_cast<const char*>(p.k) + ((long long)b * p.k_batch * kSize + 16 * lane);
+    const char* v_src = static_cast<const char*>(p.v) + ((long long)b * p.v_batch * kSize + 16 * lane);
+    const int* table = p.s.table + (long long)b * p.s.table_stride;
+    auto load = [&](uint4 (&raw)[kPieces]) {
+        const bool is_v = rest >= p.c.heads;
+        const char* src = is_v ? v_src : k_src;
+        const long long at = (long long)t * (is_v ? p.v_token : p.k_token) + (is_v ? rest - p.c.heads : rest) * kD;
+        const uint4* f = reinterpret_cast<const uint4*>(src + at * kSize);
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) raw[i] = r < rows ? __ldg(f + 8 * i) : make_uint4(0, 0, 0, 0);
+    };
+    uint4 ahead[kPieces];
+    load(ahead);
+    const bool contested = ask();
     for (int r0 = 0; r0 < rows; r0 += kRows) {
-        const int r = r0 + (threadIdx.x >> 3);
         const bool in = r < rows;
-        const int t = t0 + (in ? r / (2 * p.c.heads) : 0);
-        const int rest = in ? r % (2 * p.c.heads) : 0;
         const bool is_v = rest >= p.c.heads;
         const int h = is_v ? rest - p.c.heads : rest;
-        const int pos = position(start, t);
-        int page = in ? page_of(p.s, p.c, b, pos) : -1;
+        const int pos = in ? position(start, t) : -1;
+        int page = -1;
+        if (pos >= 0 && (pos >> p.c.page_shift) < p.s.max_pages) {
+            page = __ldg(table + (pos >> p.c.page_shift));
+            if (page >= p.c.pages) page = -1;
+        }
+        uint4 raw[kPieces];
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) raw[i] = ahead[i];
+        r += kRows, t += token_step, rest += rest_step;
+        if (rest >= per_token) rest -= per_token, ++t;
+        if (r0 + kRows < rows) load(ahead);  // the next rows are on their way while these are coded
         if (contested) {
             const bool lost = page >= 0 && written_above(p.s, p.c, b, pos >> p.c.page_shift, pos, page, lane, kRowLanes);
             const uint32_t votes = __ballot_sync(0xffffffffu, lost);
             if ((votes >> (threadIdx.x & 24)) & 0xffu) page = -1;
         }
         float x[16];
-        if (page >= 0) {
-            const long long at = is_v ? (long long)b * p.v_batch + (long long)t * p.v_token
-                                      : (long long)b * p.k_batch + (long long)t * p.k_token;
-            const void* src = is_v ? p.v : p.k;
-            if (kF32) {
-                const float4* f = reinterpret_cast<const float4*>(static_cast<const float*>(src) + at + h * kD) + lane;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float4 y = __ldg(f + 8 * i);
-                    x[4 * i] = y.x, x[4 * i + 1] = y.y, x[4 * i + 2] = y.z, x[4 * i + 3] = y.w;
-                }
-            } else {
-                const uint4* f =
-                    reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(src) + at + h * kD) + lane;
+        for (int i = 0; i < kPieces; ++i) {
+            const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const uint4 y = __ldg(f + 8 * i);
-                    const uint32_t w[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        x[8 * i + 2 * e] = __uint_as_float(w[e] << 16);
-                        x[8 * i + 2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
-                    }
-                }
+            for (int e = 0; e < 4; ++e) {
+                if (kF32) x[4 * i + e] = __uint_as_float(w[e]);
+                else x[8 * (i & 1) + 2 * e] = __uint_as_float(w[e] << 16), x[8 * (i & 1) + 2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) x[i] = 0.f;
         }
-        // largest magnitude as an integer: infinities and NaNs order above every finite value
-        uint32_t top = 0;
+        // the largest magnitude, and 0 or, where a value is not finite, NaN
+        float amax = 0.f, odd = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+        for (int i = 0; i < 16; ++i) amax = fmaxf(amax, fabsf(x[i])), odd = fmaf(x[i], 0.f, odd);
 #pragma unroll
-        for (int o = 4; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        for (int o = 4; o > 0; o >>= 1) {
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+            odd += __shfl_xor_sync(0xffffffffu, odd, o);
+        }
         if (page < 0) continue;  // (whole row groups: no lane of a live row leaves)
-        const float amax = __uint_as_float(top);
-        const bool finite = top < 0x7f800000u;
+        const bool finite = odd == 0.f;
         const bool live = finite && amax >= kTiny;
         constexpr float kTop = kFmt == kInt8 ? 127.f : 448.f;
         // x * Q could overflow from 2^119 on: there both sides of the quotient lose a factor of 2^20, exactly
         const float pre = amax >= kHuge ? 9.5367431640625e-07f : 1.f;
-        const float mul = kTop * pre, den = amax * pre;
-        const long long row = row_of(p.c, page, h, pos);
-        uint8_t* dst = (is_v ? p.c.v : p.c.k) + row * kD;
+        const float mul = kTop * pre, den = amax * pre, inv = live ? __fdiv_rn(1.f, den) : 0.f;
+        // (a cache has fewer than 2^31 rows)
+        const uint32_t row = ((uint32_t)(page * p.c.heads + h) << p.c.page_shift) + (pos & ((1 << p.c.page_shift) - 1));
+        uint8_t* dst = (is_v ? p.c.v : p.c.k) + (size_t)row * kD;
         uint32_t w[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            w[i] = live ? encode4<kFmt>(*reinterpret_cast<const float(*)[4]>(x + 4 * i), mul, den) : 0u;
+            w[i] = live ? encode4<kFmt>(*reinterpret_cast<const float(*)[4]>(x + 4 * i), mul, den, inv) : 0u;
         if (kF32) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) reinterpret_cast<uint32_t*>(dst)[8 * i + lane] = w[i];

@@ -5,6 +5,8 @@
 
 namespace {
 
+constexpr int kPlanSms = 148;  // B200; the plan is made without a device, for the workspace size
+
 int check_cache(const dt_kv_cache* c, dt::kv::Cache* out) {
     if (!c) return fail(DT_ERR_INVALID_ARGUMENT, "null cache");
     if (c->format != DT_KV_INT8 && c->format != DT_KV_E4M3)
@@ -72,9 +74,15 @@ int dt_kv_cache_append(const dt_kv_cache* cache, const void* k, long long k_batc
     p.v_token = v_token_stride;
     int dev;
     DT_TRY(prepare_device(&dev));
-    p.tile = (long long)B * T > 148 * 8 ? 8 : 1;
+    // A CTA takes 32 rows at a time: as many tokens as that are, or up to four times so many where there are more CTAs than
+    // the GPU holds (8 per SM); at most 16, the smallest page.
+    const long long rows = 2ll * B * T * p.c.heads;
+    const int once = std::max(1, dt::kv::kRows / (2 * p.c.heads));
+    const int times = (int)std::min<long long>(4, std::max<long long>(1, rows / (dt::kv::kRows * 8ll * kPlanSms)));
+    p.tile = std::min(16, once * times);
     p.tiles = (T + p.tile - 1) / p.tile;
-    if ((long long)p.tiles * B > 0x7fffffffll) return fail(DT_ERR_INVALID_ARGUMENT, "B * T is too large");
+    if ((long long)p.tiles * B > 0x7fffffffll || (T / cache->page_size + 2ll) * B > 0x7fffffffll)
+        return fail(DT_ERR_INVALID_ARGUMENT, "B * T is too large");
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     const dim3 grid((unsigned)(p.tiles * B)), block(dt::kv::kThreads);
     if (cache->format == DT_KV_INT8)
@@ -115,7 +123,6 @@ int dt_kv_cache_read(const dt_kv_cache* cache, void* k, void* v, int dst_f32, co
 
 namespace {
 
-constexpr int kPlanSms = 148;  // B200; the plan is made without a device, for the workspace size
 
 // How the prefix's part is cut: one CTA per SM, each with a block of query rows of a K/V head and an
 // even stretch of the prefix.  Two Q tiles per CTA, so that keys are converted once for 256 rows,
