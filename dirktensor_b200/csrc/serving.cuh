@@ -386,7 +386,7 @@ int dt_token_log_probs(const void* logits, int logits_f32, long long ld, int N, 
                        int targets_int64, int top, float* log_prob, float* entropy, float* lse, int* top_ids,
                        float* top_log_probs, void* stream) {
     t_last_error.clear();
-    if (N < 0 || V < 1) return fail(DT_ERR_INVALID_ARGUMENT, "N must be >= 0 and V >= 1");
+    if (N < 0 || V < 1 || V > (1 << 30)) return fail(DT_ERR_INVALID_ARGUMENT, "N must be >= 0 and V 1..2^30");
     if (top < 0 || top > dt::logprobs::kMaxTop || top > V)
         return fail(DT_ERR_INVALID_ARGUMENT, "top must be 0..%d and at most V", dt::logprobs::kMaxTop);
     if (N == 0) return DT_OK;
@@ -427,7 +427,7 @@ int dt_token_log_probs_bwd(const void* logits, int logits_f32, long long ld, int
                            int targets_int64, const float* lse, const float* entropy, const float* d_log_prob,
                            const float* d_entropy, void* d_logits, long long d_ld, void* stream) {
     t_last_error.clear();
-    if (N < 0 || V < 1) return fail(DT_ERR_INVALID_ARGUMENT, "N must be >= 0 and V >= 1");
+    if (N < 0 || V < 1 || V > (1 << 30)) return fail(DT_ERR_INVALID_ARGUMENT, "N must be >= 0 and V 1..2^30");
     if (N == 0) return DT_OK;
     if (!logits || !d_logits || ld < V || d_ld < V)
         return fail(DT_ERR_INVALID_ARGUMENT, "logits and d_logits must be non-null with ld >= V");

@@ -449,7 +449,7 @@ int dt_prefix_attn_fwd(const dt_kv_cache* cache, const void* q, long long q_batc
                        size_t workspace_bytes, void* stream);
 
 /* ---- scoring: log probabilities of given tokens ----------------------------
- * For each of N rows of V logits (fp32 or bf16, rows ld elements apart):
+ * For each of N rows of V (1..2^30) logits (fp32 or bf16, rows ld elements apart):
  *   log_prob = x[target] - lse, lse = log sum exp x, entropy = -sum p log p,
  * and the `top` (0..32) most likely tokens, by logit and then by lower id, with
  * their log probabilities ([N, top]).  Sums are fp32.  The unreduced loss of
@@ -467,7 +467,8 @@ int dt_token_log_probs(const void* logits, int logits_f32, long long ld, int N, 
  * d_log_prob and d_entropy (fp32 [N]; either may be NULL for zero):
  *   d_logits[j] = d_log_prob (1[j = target] - p_j) - d_entropy p_j (log p_j + entropy)
  * Rows whose lse is -inf get zeros; d_log_prob of an ignored target is not
- * used.  d_logits may be the logits' own memory (with d_ld = ld). */
+ * used.  d_logits may be the logits' own memory (with d_ld = ld), and must not
+ * overlap it otherwise. */
 int dt_token_log_probs_bwd(const void* logits, int logits_f32, long long ld, int N, int V, const void* targets,
                            int targets_int64, const float* lse, const float* entropy, const float* d_log_prob,
                            const float* d_entropy, void* d_logits, long long d_ld, void* stream);
