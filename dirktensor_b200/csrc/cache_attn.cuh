@@ -225,6 +225,12 @@ __device__ __forceinline__ void store_row(const Params& p, long long row, int la
 // each 16-key half of a tile,
 //   K: keys g and g + 8, dims 16 (4 hf + t) ..+15;      S, P: keys g and g + 8, queries 2t and 2t + 1;
 //   V: keys 2t, 2t + 1, 2t + 8, 2t + 9, dims 16 g ..+15;  O: dims 16 g ..+15, queries 2t and 2t + 1.
+//
+// Bound by the codes' read (256 bytes a key and head against 8 to 16 tensor products a query) and, next, by the
+// latency of its own chain: a 32-key tile takes a warp some 650 instructions, 230 of them conversions.  64 sequences
+// of 1024 to 4096 keys and 16 heads, 692 MB, take 132 us (5.25 TB/s, 0.82 of the measured copy); 512 keys
+// of one sequence 6.1 us.  Keys as MMA columns and queries as rows, the first form, left half of each MMA idle and
+// needed twice the accumulators (159 us); register-resident tiles without the ring were slower still (207 us).
 template <int kForm>
 struct State {
     static constexpr int kSets = kForm == kWide ? 2 : 1, kCols = kForm == kFew ? 1 : 2;

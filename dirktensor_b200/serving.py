@@ -289,18 +289,16 @@ def token_log_probs(logits, targets=None, top: int = 0) -> TokenLogProbs:
     top = int(top)
     if not 0 <= top <= min(32, V):
         raise ValueError("top must be 0..32 and at most the vocabulary")
-    # one allocation for the three results of a row, one for its alternatives' log probabilities
-    three = torch.empty((3,) + shape, dtype=torch.float32, device=dev)
-    lse, ent, lp = three.unbind(0)
-    at = three.data_ptr()
+    lse = torch.empty(shape, dtype=torch.float32, device=dev)
+    ent = torch.empty_like(lse)
+    lp = None if targets is None else torch.empty_like(lse)
     ids = tlp = None
     if top:
-        ids = torch.empty(shape + (top,), dtype=torch.int32, device=dev)
         tlp = torch.empty(shape + (top,), dtype=torch.float32, device=dev)
+        ids = torch.empty_like(tlp, dtype=torch.int32)
     _call(logits.get_device(), lib().dt_token_log_probs, logits.data_ptr(), logits.dtype == torch.float32, ld, n, V, t, t64, top,
-          at + 8 * n if t else None, at + 4 * n, at, ids.data_ptr() if top else None, tlp.data_ptr() if top else None)
-    if targets is None:
-        lp = None
+          None if lp is None else lp.data_ptr(), ent.data_ptr(), lse.data_ptr(), ids.data_ptr() if top else None,
+          tlp.data_ptr() if top else None)
     return TokenLogProbs(lp, ent, lse, ids, tlp)
 
 
