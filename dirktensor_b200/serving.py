@@ -205,7 +205,7 @@ def cache_attention_forward(q, cache: KVCache, page_table, seq_lens, scale: floa
     o, m, l, po, pm, pl = _outputs(q, shape, out, return_stats)
     ws, pw, nbytes = _workspace(cache, B, T, H, cache.kv_heads, f32, cache.page_size, n, 0)
     _call(index, lib().dt_cache_attn_fwd, cache._ref, q.data_ptr(), s[0], s[1], f32, po, pm, pl, table, stride, n, lens,
-          _ints("q_lens", q_lens, index, B), B, T, H, scale, pw, nbytes)
+          _ints("q_lens", q_lens, index, B), B, T, H, float(scale), pw, nbytes)
     return FlashAttentionResult(o, m, l) if return_stats else o
 
 
@@ -231,7 +231,7 @@ def prefix_attention_forward(q, cache: KVCache, prefix_pages, prefix_len: int, p
     o, m, l, po, pm, pl = _outputs(q, shape, out, return_stats)
     ws, pw, nbytes = _workspace(cache, B, T, H, cache.kv_heads, f32, cache.page_size, n, prefix_len)
     _call(index, lib().dt_prefix_attn_fwd, cache._ref, q.data_ptr(), s[0], s[1], f32, po, pm, pl, pages, prefix_len, table,
-          stride, n, lens, _ints("q_lens", q_lens, index, B), B, T, H, scale, pw, nbytes)
+          stride, n, lens, _ints("q_lens", q_lens, index, B), B, T, H, float(scale), pw, nbytes)
     return FlashAttentionResult(o, m, l) if return_stats else o
 
 
@@ -261,8 +261,8 @@ def _rows(name, t):
                 break
             n *= size
         else:
-            if (ld or V) >= V:
-                return n, ld or V
+            if ld is None or ld >= V:  # (rows that share memory have a distance of zero)
+                return n, V if ld is None else ld
     raise ValueError(f"{name}: rows must be contiguous and evenly spaced")
 
 

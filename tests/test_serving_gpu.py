@@ -315,6 +315,51 @@ def test_cache_attention_long_sequence_is_split_and_joined(dt, cuda):
         ref.check_attention(got, ref.attention(q, c, table, lens, SCALE))
 
 
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("group, T", [(1, 1), (8, 1), (4, 5)])
+def test_few_long_sequences_are_shared_out_over_the_gpu(dt, cuda, fmt, dtype, group, T):
+    """Even shares of all tiles, whatever the lengths: none, one key, one tile, many, and padding queries."""
+    for lens, q_lens in (([9001], None), ([0], None), ([T], None), ([0, 8200, 33, 1000], [T, T, 0, T])):
+        B = len(lens)
+        c, _, _, seq_lens, q = attention_case(dt, cuda, 41, fmt, dtype, B, T, 1, group, 64, lens)
+        table = torch.full((B, 160), -1, dtype=torch.int32, device=cuda)
+        table[:, :-(-max(lens) // 64)] = torch.arange(B * -(-max(lens) // 64), device=cuda, dtype=torch.int32).view(B, -1)
+        ql = None if q_lens is None else ints(cuda, *q_lens)
+        poison(c, table, seq_lens)
+        got = dt.cache_attention_forward(q, c, table, seq_lens, SCALE, q_lens=ql, return_stats=True)
+        dt.check_device_error()
+        ref.check_attention(got, ref.attention(q, c, table, seq_lens, SCALE, q_lens=ql))
+
+
+def test_more_items_than_fit_take_the_longest_sequences_first(dt, cuda):
+    """40 x 16 items, a wide page table, equal and zero lengths among the sequences."""
+    B = 40
+    lens = [0, 1, 70, 70, 70, 33, 0, 140] * 5
+    c, _, _, seq_lens, q = attention_case(dt, cuda, 42, "int8", BF16, B, 1, 16, 1, 64, lens)
+    table = torch.full((B, 40), 1 << 30, dtype=torch.int32, device=cuda)
+    table[:, :3] = torch.randperm(c.num_pages, device=cuda)[: 3 * B].view(B, 3).to(torch.int32)
+    poison(c, table, seq_lens)
+    got = dt.cache_attention_forward(q, c, table, seq_lens, SCALE, return_stats=True)
+    ref.check_attention(got, ref.attention(q, c, table, seq_lens, SCALE))
+
+
+def test_an_empty_page_table_and_outputs_in_the_queries_own_memory(dt, cuda):
+    c, _, table, lens, q = attention_case(dt, cuda, 43, "int8", BF16, 2, 3, 2, 2, 16, [20, 33])
+    got = dt.cache_attention_forward(q, c, table[:, :0], lens, SCALE, return_stats=True)
+    assert all(bool((x == 0).all()) for x in got)
+    want = dt.cache_attention_forward(q, c, table, lens, SCALE)
+    q2 = q.clone()
+    assert torch.equal(dt.cache_attention_forward(q2, c, table, lens, SCALE, out=q2), want)
+    before = c.k.clone()
+    kv = torch.ones((2, 1, 2, D), dtype=BF16, device=cuda)
+    c.append(kv, kv, table[:, :0])
+    assert torch.equal(c.k, before)
+    assert bool((c.read(table[:, :0], None, 5)[0] == 0).all())
+    assert dt.cache_attention_forward(q[:0], c, table[:0], lens[:0], SCALE).shape == (0, 3, 4, D)
+    assert dt.cache_attention_forward(q[:, :0], c, table, lens, SCALE).shape == (2, 0, 4, D)
+
+
 def test_strided_queries_given_outputs_and_refusals(dt, cuda):
     c, _, table, lens, q = attention_case(dt, cuda, 7, "int8", BF16, 2, 2, 4, 1, 16, [20, 33])
     fused = torch.zeros((2, 2, 3, 4, D), dtype=BF16, device=cuda)
@@ -384,6 +429,40 @@ def test_prefix_attention_without_own_keys_with_padding_and_bad_pages(dt, cuda, 
     # a prefix whose every page is missing leaves the sequence's own keys
     got = dt.prefix_attention_forward(q, c, torch.full_like(pages, -1), 333, table, seq_lens, SCALE, return_stats=True)
     ref.check_attention(got, ref.attention(q, c, table, seq_lens.clamp_min(0), SCALE))
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("heads, group", [(1, 3), (2, 20)])
+def test_a_long_prefix_in_many_parts(dt, cuda, fmt, dtype, heads, group):
+    """More parts than the sequences' own kernel joins, with and without keys of their own."""
+    B, prefix = 3, 5003
+    c, pages, table, lens, q = attention_case(dt, cuda, 44, fmt, dtype, B, 1, heads, group, 32, [0, 40, 700], prefix)
+    poison(c, table, lens, pages, prefix)
+    p_half = 2.0 ** -8 if dtype == BF16 else 0.0
+    got = dt.prefix_attention_forward(q, c, pages, prefix, table, lens, SCALE, return_stats=True)
+    dt.check_device_error()
+    ref.check_attention(got, ref.attention(q, c, table, lens, SCALE, prefix_pages=pages, prefix_len=prefix, p_half=p_half))
+    got = dt.prefix_attention_forward(q, c, pages, prefix, None, None, -SCALE, return_stats=True)
+    ref.check_attention(got, ref.attention(q, c, None, None, -SCALE, prefix_pages=pages, prefix_len=prefix, p_half=p_half))
+
+
+def test_prefix_scales_that_grow_along_it_and_queries_far_from_one(dt, cuda):
+    """The running factor of the weights has to follow v_scale, upwards and with zeros before."""
+    for dtype in (BF16, F32):
+        c, pages, table, lens, q = attention_case(dt, cuda, 45, "int8", dtype, 4, 1, 1, 1, 64, [3, 9, 0, 64], 1500)
+        order = pages.long()
+        grow = torch.exp2(torch.linspace(-40, 12, len(order), device=cuda))
+        c.v_scale[order] *= grow[:, None, None]
+        c.v_scale[order[:4]] = 0.0
+        q = (q.float() * torch.tensor([1.0, 2.0 ** -30, 0.0, 2.0 ** 6], device=cuda)[:, None, None, None]).to(dtype)
+        p_half = 2.0 ** -8 if dtype == BF16 else 0.0
+        got = dt.prefix_attention_forward(q, c, pages, 1500, table, lens, SCALE, return_stats=True)
+        o, m, l, o_tol, m_tol, l_tol = ref.attention(q, c, table, lens, SCALE, prefix_pages=pages, prefix_len=1500, p_half=p_half)
+        # the prefix's weights are scaled by the largest v_scale, at most 2^6 above which lies 2^15: each is off by at most
+        # half of fp16's smallest step, 2^-25, so by 2^-31 of that scale, for codes of at most 127 over weights of at least 1
+        o_tol = o_tol + 2.0 ** -31 * float(c.v_scale[torch.isfinite(c.v_scale)].max()) * 127 * 1500
+        ref.check_attention(got, (o, m, l, o_tol, m_tol, l_tol))
 
 
 def test_prefix_attention_equals_the_cache_attention_of_the_whole(dt, cuda):
@@ -503,6 +582,29 @@ def test_log_probs_ties_masks_and_values_that_are_not_finite(dt, cuda, dtype):
     assert dt.token_log_probs(x, t, top=3).top_ids[6].tolist() == [0, 1, 2]
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_log_probs_of_few_long_rows_with_ties_and_values_that_are_not_finite(dt, cuda, dtype):
+    """Rows over clusters: what one CTA of them sees has to reach the row's result."""
+    V, top = 100352, 32
+    x = (torch.randn((5, V), generator=gen(cuda, 6), device=cuda) * 2).to(dtype)
+    x[0] = 1.5
+    x[1, V - 1] = math.nan
+    x[2] = -math.inf
+    x[2, 70000] = 4.0
+    x[3, 1000::7] = 50.0                       # more ties than are collected
+    x[4, :99000] = torch.finfo(dtype).min
+    t = torch.tensor([5, 0, 70000, 1000, 100000], device=cuda)
+    r = dt.token_log_probs(x, t, top=top)
+    assert r.top_ids[0].tolist() == list(range(top)) and abs(float(r.log_prob[0]) + math.log(V)) < 1e-4
+    assert math.isnan(float(r.lse[1])) and V - 1 not in r.top_ids[1].tolist()
+    for row in (1, 3, 4):
+        y = x[row].float().nan_to_num(nan=-math.inf)
+        assert r.top_ids[row].tolist() == torch.sort(y, descending=True, stable=True)[1][:top].tolist()
+    assert float(r.log_prob[2]) == 0.0 and r.top_ids[2].tolist() == [70000] + list(range(top - 1))
+    n = len(range(1000, V, 7))
+    assert abs(float(r.log_prob[3]) + math.log(n)) < 1e-4 and abs(float(r.entropy[3]) - math.log(n)) < 1e-4
+
+
 def test_log_probs_shapes_strides_and_refusals(dt, cuda):
     g = gen(cuda, 2)
     wide = torch.randn((4, 6, 1010), generator=g, device=cuda)
@@ -519,7 +621,9 @@ def test_log_probs_shapes_strides_and_refusals(dt, cuda):
     assert empty.top_ids.shape == (0, 6, 2)
     for bad in (lambda: dt.token_log_probs(wide[:, :3], t[:, :3]), lambda: dt.token_log_probs(wide, t, top=33),
                 lambda: dt.token_log_probs(wide, t.float()), lambda: dt.token_log_probs(wide, t[:3]),
-                lambda: dt.token_log_probs(wide.half(), t), lambda: dt.token_log_probs(wide.transpose(1, 2), t)):
+                lambda: dt.token_log_probs(wide.half(), t), lambda: dt.token_log_probs(wide.transpose(1, 2), t),
+                lambda: dt.token_log_probs(wide[:, :1].expand(4, 6, 1010), t),
+                lambda: dt.token_log_probs(wide[0, 0].expand(4, 6, 1010), t)):
         with pytest.raises(ValueError):
             bad()
 
