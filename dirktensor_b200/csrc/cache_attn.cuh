@@ -40,8 +40,8 @@ struct Params {
     int by_length;               // split_kernel takes the longest sequences first
     // Workspace of stream_kernel and join_kernel: partial sums of the CTAs and, of the prefix
     // kernel, of the shared keys.  Sums are relative to 2^m; statistics are (m, l, largest score, -).
-    int shares;                  // CTAs of stream_kernel (0: not launched, no keys but the prefix's)
-    int* starts;                 // [B + 1] first tile of each sequence, were each of one item
+    int shares;                  // CTAs that stream_kernel shares out (0: not launched, no keys but the prefix's)
+    int* starts;                 // [B + 1] first CTA of each sequence, were each of one item
     float* part_o;               // [shares + items][rows of an item][128]
     float4* part_s;              // [shares + items][rows of an item]
     int n_shared;                // parts of the prefix
@@ -86,7 +86,7 @@ enum : int { kFew = 0, kEight = 1, kWide = 2 };  // 4, 8, or 16 in two sets of c
 constexpr int rows_of(int form) { return form == kFew ? 4 : form == kEight ? 8 : 16; }
 
 // CTAs per SM: four where 128 registers a thread suffice; 16 rows spill at three (28 us instead of 26 for 16 x 2047 keys).
-constexpr int ctas_per_sm(bool f32, int form) { return form == kWide ? 2 : f32 ? 3 : 4; }
+constexpr int ctas_per_sm(bool f32, int form) { return form == kWide ? 2 : f32 && form != kFew ? 3 : 4; }
 
 __device__ __forceinline__ void cp16(void* dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
@@ -216,7 +216,8 @@ __device__ __forceinline__ void store_row(const Params& p, long long row, int la
 //   S^T (16 keys x 8 queries) = K (16 keys x 16 dims) Q^T,  O^T (16 dims x 8 queries) = V^T (16 dims x 16 keys) P^T
 // so that no row of an MMA is idle however few queries there are.  Codes are exact in fp16.  Queries
 // are scaled row by row by a power of two into fp16's range, where bf16 values are exact; fp32 ones
-// go in as fp16(q) and q - fp16(q), and so do their weights p * v_scale.  The weights of bf16 queries
+// go in as fp16(q) and q - fp16(q), and so do their weights p * v_scale: in two columns, where there are
+// four queries at most, else in two MMAs.  The weights of bf16 queries
 // are rounded to fp16 once, at 2^-11 well below the result's own 2^-8.  More than 8 bf16 queries of
 // a K/V head take two sets of columns (kWide), so that the keys are read and converted once.
 //
@@ -239,11 +240,17 @@ struct State {
     float l[kSets][kCols];       // this lane's share of the sums of p
     float mx[kSets][kCols];      // this lane's largest scores
     float f[kSets][kCols];       // acc holds sums of p * v_scale * f: f keeps them in fp16's range
-    // dim 16g + d of query 2t + c
-    __device__ __forceinline__ float sum(int z, int c, int d) const { return acc[z][d >> 1][2 * (d & 1) + c]; }
+    // dim 16g + d of query 2t + c (kFew: of query t, the sum of its two columns)
+    __device__ __forceinline__ float sum(int z, int c, int d) const {
+        const float* a = acc[z][d >> 1] + 2 * (d & 1);
+        return kForm == kFew ? a[0] + a[1] : a[c];
+    }
     __device__ __forceinline__ void rescale(int z, int c, float a) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc[z][j][c] *= a, acc[z][j][2 + c] *= a;
+        for (int j = 0; j < 8; ++j) {
+            acc[z][j][c] *= a, acc[z][j][2 + c] *= a;
+            if (kForm == kFew) acc[z][j][1] *= a, acc[z][j][3] *= a;
+        }
     }
 };
 
@@ -252,7 +259,8 @@ __device__ __forceinline__ void attend(const Params& p, Stage* ring, int b, int 
                                        State<kForm>& st) {
     static_assert(!(kF32 && kForm == kWide), "fp32 queries have no wide form: twice the registers");
     constexpr int kSets = kForm == kWide ? 2 : 1, kCols = kForm == kFew ? 1 : 2;
-    constexpr int kParts = kF32 ? 2 : 1;
+    constexpr bool kBeside = kF32 && kForm == kFew;  // the rest of an fp32 query in the column beside it
+    constexpr int kParts = kF32 && !kBeside ? 2 : 1;  // or in an MMA of its own
     const int lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
 
@@ -261,7 +269,7 @@ __device__ __forceinline__ void attend(const Params& p, Stage* ring, int b, int 
 #pragma unroll
     for (int z = 0; z < kSets; ++z) {
         const int r = row0 + (kCols == 1 ? g >> 1 : g) + 8 * z;
-        const bool in = r < p.T * p.group && (kCols == 2 || !(g & 1));
+        const bool in = r < p.T * p.group && (kCols == 2 || kBeside || !(g & 1));
         const int tq = in ? token_of(r, p.group) : 0;
         const int h = hk * p.group + (in ? r - tq * p.group : 0);
         const long long at = (long long)b * p.q_batch + (long long)tq * p.q_token + (long long)h * kD + 16 * t;
@@ -377,8 +385,15 @@ __device__ __forceinline__ void attend(const Params& p, Stage* ring, int b, int 
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const float a = finite ? x[2 * i] * mul : 0.f, c = finite ? x[2 * i + 1] * mul : 0.f;
-            if (kF32) split_pair(a, c, qb[z][0][i], qb[z][kParts - 1][i]);
-            else qb[z][0][i] = half_pair(a, c);
+            if (kBeside) {
+                uint32_t hi, lo;
+                split_pair(a, c, hi, lo);
+                qb[z][0][i] = g & 1 ? lo : hi;
+            } else if (kF32) {
+                split_pair(a, c, qb[z][0][i], qb[z][kParts - 1][i]);
+            } else {
+                qb[z][0][i] = half_pair(a, c);
+            }
         }
     }
 
@@ -434,8 +449,10 @@ __device__ __forceinline__ void attend(const Params& p, Stage* ring, int b, int 
                 for (int z = 0; z < kSets; ++z)
 #pragma unroll
                     for (int c = 0; c < kCols; ++c) {
-                        s[z][a][0][c] = (d[z][0][c] + d[z][1][c]) * (ks0 * factor[z][c]);
-                        s[z][a][1][c] = (d[z][0][2 + c] + d[z][1][2 + c]) * (ks1 * factor[z][c]);
+                        float s0 = d[z][0][c] + d[z][1][c], s1 = d[z][0][2 + c] + d[z][1][2 + c];
+                        if (kBeside) s0 += d[z][0][1] + d[z][1][1], s1 += d[z][0][3] + d[z][1][3];
+                        s[z][a][0][c] = s0 * (ks0 * factor[z][c]);
+                        s[z][a][1][c] = s1 * (ks1 * factor[z][c]);
                     }
             }
         }
@@ -530,7 +547,10 @@ __device__ __forceinline__ void attend(const Params& p, Stage* ring, int b, int 
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                     const float x = u[z][a][k][0] * st.f[z][0], y = kCols == 2 ? u[z][a][k][kCols - 1] * st.f[z][kCols - 1] : 0.f;
-                    if (kF32) {
+                    if (kBeside) {
+                        const uint32_t hi = half_pair(x, 0.f);
+                        pb[z][0][k] = transposed(half_pair(x, x - half_values(hi).x));
+                    } else if (kF32) {
                         uint32_t hi, lo;
                         split_pair(x, y, hi, lo);
                         pb[z][0][k] = transposed(hi);
@@ -707,50 +727,63 @@ __device__ __forceinline__ int tiles_of(const Params& p, int b) {
     return q_len > 0 && keys > 0 ? (int)((keys + kTile - 1) / kTile) : 0;
 }
 
-// CTA w of W takes the tiles [w n / W, (w + 1) n / W) of all n tiles of all items in order
-// (sequence, K/V head, rows): every CTA has the same amount of work whatever the lengths are.
-// W <= n, so that none of them has nothing (and leaves a part unwritten that join_kernel reads).
-__device__ __forceinline__ int shares_of(const Params& p, long long n) { return (int)min((long long)p.shares, n); }
-__device__ __forceinline__ long long first_tile(long long n, int w, int W) { return n * w / W; }
-// The CTA that takes tile x.
-__device__ __forceinline__ int share_of(long long n, long long x, int W) { return (int)(((x + 1) * W - 1) / n); }
+// CTAs that take an item of sequence b: its share of the GPU by its tiles, one at least.  (`all`: tiles of all
+// items.  All together that is at most p.shares + the number of items.)
+__device__ __forceinline__ int shares_of(const Params& p, int tiles, long long all) {
+    return tiles == 0 ? 0 : max(1, (int)((long long)p.shares * tiles / all));
+}
 
-// One even share of all the work per CTA, for few items of many keys; its warps take the share's tiles
-// in turn.  A share may begin and end inside items: what it has of an item goes to the workspace at
-// slot w + item (which no other pair of CTA and item has, since one of the two grows from pair
-// to pair), and join_kernel adds the parts up.  An item that lies within one share is written at once.
-constexpr int kMaxBatch = 8192;  // the first tiles of so many sequences fit into the ring's memory
+// Few items of many keys: as many CTAs for each as its keys are of all keys, whose warps take its tiles in
+// turn, so that all of them, and those of the other heads, read the same pages at about the same time.
+// What a CTA has goes to the workspace, and join_kernel adds an item's parts up; an item of one CTA is written at once.
+constexpr int kMaxBatch = 8192;  // the first CTAs of so many sequences fit into the ring's memory
 template <int kFmt, bool kF32, int kForm>
 __global__ void __launch_bounds__(kThreads, ctas_per_sm(kF32, kForm)) stream_kernel(const Params p) {
     pdl_enter();
     constexpr int kRows = rows_of(kForm);
     extern __shared__ __align__(16) uint8_t smem_raw[];
     Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
-    static_assert(sizeof(sm.ring) >= (kMaxBatch + 1) * 4, "first tiles of a batch");
+    static_assert(sizeof(sm.ring) >= (kMaxBatch + 1) * 4, "first CTAs of a batch");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int per_head = (p.T * p.group + kRows - 1) / kRows;
+    const int items = p.c.heads * per_head;  // of one sequence
 
-    // starts[b] = tiles of the sequences before b; in the ring's memory until the first tile comes
+    // starts[b] = CTAs per item of the sequences before b; in the ring's memory until the first tile comes
     int* starts = reinterpret_cast<int*>(&sm.ring);
     {
         __shared__ int totals[kWarps];
         const int per = (p.B + kThreads - 1) / kThreads;
         const int b0 = min((int)threadIdx.x * per, p.B), b1 = min(b0 + per, p.B);
-        int sum = 0;
-        for (int b = b0; b < b1; ++b) sum += tiles_of(p, b);
-        int before = sum;
+        // sum over the CTA's threads, and over those before this one
+        auto scan = [&](int mine, int& before) {
+            int upto = mine;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, before, o);
-            if (lane >= o) before += y;
-        }
-        if (lane == 31) totals[warp] = before;
-        __syncthreads();
-        before -= sum;
-        for (int w = 0; w < warp; ++w) before += totals[w];
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += y;
+            }
+            __syncthreads();
+            if (lane == 31) totals[warp] = upto;
+            __syncthreads();
+            int all = 0;
+            before = upto - mine;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                if (w < warp) before += totals[w];
+                all += totals[w];
+            }
+            return all;
+        };
+        int sum = 0, before;
+        for (int b = b0; b < b1; ++b) sum += tiles_of(p, b);
+        const long long all = (long long)scan(sum, before) * items;
+        sum = 0;
+        for (int b = b0; b < b1; ++b) sum += shares_of(p, tiles_of(p, b), all);
+        scan(sum, before);
         for (int b = b0; b < b1; ++b) {
             starts[b] = before;
             if (blockIdx.x == 0) p.starts[b] = before;
-            before += tiles_of(p, b);
+            before += shares_of(p, tiles_of(p, b), all);
         }
         if (threadIdx.x == kThreads - 1) {
             starts[p.B] = before;
@@ -758,57 +791,41 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kF32, kForm)) stream_ker
         }
         __syncthreads();
     }
-    const int per_head = (p.T * p.group + kRows - 1) / kRows;
-    const int items = p.c.heads * per_head;  // of one sequence
-    const long long n = (long long)starts[p.B] * items;
-    const int w = blockIdx.x, W = shares_of(p, n);
-    if (w >= W) return;
-    long long x = first_tile(n, w, W);
-    const long long end = first_tile(n, w + 1, W);
-    // the sequence that tile x is of: the last one that starts at or before it
+    const int w = blockIdx.x;
+    if (w >= starts[p.B] * items) return;
+    // the sequence of this CTA: the last one that starts at or before it
     int b = 0;
     for (int up = kMaxBatch / 2; up > 0; up >>= 1)
-        if (b + up < p.B && (long long)starts[b + up] * items <= x) b += up;
-    long long at = (long long)starts[b] * items;
-    while (x < end) {
-        const int tiles = tiles_of(p, b);
-        if (x >= at + (long long)tiles * items) {
-            at += (long long)tiles * items;
-            ++b;
-            continue;
+        if (b + up < p.B && starts[b + up] * items <= w) b += up;
+    const int split = starts[b + 1] - starts[b];
+    const int i = (w - starts[b] * items) / split, rank = (w - starts[b] * items) % split;
+    __syncthreads();  // the ring's memory is free
+    const int hk = i / per_head, row0 = i % per_head * kRows;
+    State<kForm> st;
+    attend<kFmt, kF32, kForm>(p, sm.ring[warp], b, hk, row0, rank * kWarps + warp, 0x7fffffff, split * kWarps, st);
+    const bool whole = split == 1 && p.n_shared == 0;
+    join_warps<kForm>(sm, st, min(kRows, p.T * p.group - row0), [&](int row, const Joined& y, float best, float big) {
+        if (whole) {
+            const int r = row0 + row;
+            store_row<kF32>(p, ((long long)b * p.T + r / p.group) * p.heads + hk * p.group + r % p.group, lane, y, best, big);
+        } else {
+            const long long at = (long long)w * kRows + row;
+            reinterpret_cast<float4*>(p.part_o + at * kD)[lane] = y.o;
+            if (lane == 0) p.part_s[at] = make_float4(best, y.l, big, 0.f);
         }
-        const int i = (int)((x - at) / tiles);
-        const int tile0 = (int)((x - at) % tiles);
-        const int tile1 = (int)min((long long)tiles, tile0 + (end - x));
-        const int hk = i / per_head, row0 = i % per_head * kRows;
-        __syncthreads();  // the ring's memory is free
-        State<kForm> st;
-        attend<kFmt, kF32, kForm>(p, sm.ring[warp], b, hk, row0, tile0 + warp, tile1, kWarps, st);
-        const bool whole = tile0 == 0 && tile1 == tiles && p.n_shared == 0;
-        const long long slot = ((long long)w + (long long)b * items + i) * kRows;
-        join_warps<kForm>(sm, st, min(kRows, p.T * p.group - row0), [&](int row, const Joined& y, float best, float big) {
-            if (whole) {
-                const int r = row0 + row;
-                store_row<kF32>(p, ((long long)b * p.T + r / p.group) * p.heads + hk * p.group + r % p.group, lane, y, best, big);
-            } else {
-                reinterpret_cast<float4*>(p.part_o + (slot + row) * kD)[lane] = y.o;
-                if (lane == 0) p.part_s[slot + row] = make_float4(best, y.l, big, 0.f);
-            }
-        });
-        x += tile1 - tile0;
-    }
+    });
 }
 
-// Joins the parts of each query row: a CTA per row, its warps taking eight parts at a time (so
-// that eight rows of 512 bytes are on their way at once), then joined themselves.
-constexpr int kJoinWarps = 4;
+// Joins the parts of each query row: a CTA per row, of as many warps as there are eights of parts, up to 16; a
+// warp takes eight parts at a time (so that eight rows of 512 bytes are on their way at once).
+constexpr int kJoinWarps = 16;
 template <bool kF32, int kForm>
 __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const Params p) {
     pdl_enter();
     constexpr int kRows = rows_of(kForm);
     const long long rows = (long long)p.B * p.T * p.heads;
     const long long row = blockIdx.x;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     const int h = (int)(row % p.heads), tq = (int)(row / p.heads % p.T), b = (int)(row / p.heads / p.T);
     const int r = tq * p.group + h % p.group;
     const int q_len = p.q_lens ? min(p.q_lens[b], p.T) : p.T;
@@ -820,16 +837,10 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const Params p) {
         const int per_head = (p.T * p.group + kRows - 1) / kRows;
         const int items = p.c.heads * per_head;
         const int i = h / p.group * per_head + r / kRows;
-        const int start = p.starts[b], tiles = p.starts[b + 1] - start;
-        const long long n = (long long)p.starts[p.B] * items;
-        if (tiles > 0) {
-            const long long x = (long long)start * items + (long long)i * tiles;
-            const int W = shares_of(p, n);
-            const int first = share_of(n, x, W);
-            parts = share_of(n, x + tiles - 1, W) - first + 1;
-            if (parts == 1 && p.n_shared == 0) return;  // written by stream_kernel
-            slot = (long long)first + (long long)b * items + i;
-        }
+        const int start = p.starts[b];
+        parts = p.starts[b + 1] - start;
+        if (parts == 1 && p.n_shared == 0) return;  // written by stream_kernel
+        slot = (long long)start * items + (long long)i * parts;
     }
     const int shared = tq < q_len ? p.n_shared : 0;
     const float4* own_s = p.part_s + slot * kRows + r % kRows;
@@ -838,7 +849,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const Params p) {
     const float4* shared_o = reinterpret_cast<const float4*>(p.shared_o + row * kD) + lane;
     float m = -INFINITY, big = -INFINITY;
     Joined y;
-    for (int i0 = 8 * warp; i0 < parts + shared; i0 += 8 * kJoinWarps) {
+    for (int i0 = 8 * warp; i0 < parts + shared; i0 += 8 * warps) {
         float4 s = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
         const int mine = i0 + (lane & 7);
         if (mine < parts) s = own_s[(long long)mine * kRows];
@@ -874,11 +885,9 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const Params p) {
     if (warp != 0) return;
     float best = -INFINITY;
     big = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) best = fmaxf(best, sm[w]), big = fmaxf(big, sx[w]);
+    for (int w = 0; w < warps; ++w) best = fmaxf(best, sm[w]), big = fmaxf(big, sx[w]);
     Joined all;
-#pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) all.add(sm[w], sl[w], best, so[w][lane]);
+    for (int w = 0; w < warps; ++w) all.add(sm[w], sl[w], best, so[w][lane]);
     store_row<kF32>(p, row, lane, all, best, big);
 }
 

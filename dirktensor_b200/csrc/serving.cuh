@@ -146,12 +146,12 @@ struct AttnPlan {
     long long items;  // (sequence, K/V head, rows)
     int split;        // CTAs per item (split_kernel), or
     bool by_length;   // longest sequences first (split_kernel)
-    int shares;       // CTAs of stream_kernel, which join_kernel follows (0: split_kernel)
+    int shares;       // CTAs that stream_kernel shares out, and one per item at least; join_kernel follows (0: split_kernel)
 };
 
 // split_kernel, with as many CTAs per item as the GPU holds at once, up to a cluster, and no more
 // than there are tiles for; stream_kernel where that leaves most of the GPU idle: few items with
-// many keys.  (8 x 131071 keys: 71 us shared by 444 CTAs, 149 us in 8 clusters of 8.)
+// many keys.  (8 x 131071 keys: 149 us in 8 clusters of 8, 70 shared out over 592 CTAs.)
 // Behind a prefix, split_kernel also joins its rows with the prefix's n_shared parts, if these are few.
 AttnPlan plan_attn(int B, int T, int heads, int kv_heads, int q_f32, int page_size, int max_pages, int n_shared) {
     namespace ca = dt::cache_attn;
@@ -240,8 +240,11 @@ int launch_stream(const dt::cache_attn::Params& p, const AttnPlan& plan, int for
     namespace ca = dt::cache_attn;
     if (plan.shares > 0)
         DT_TRY(launch_pdl(attn_kernel_of(true, format, q_f32, plan.form),
-                          dim3((unsigned)plan.shares), dim3(ca::kThreads), sizeof(ca::Smem), st, p));
-    const dim3 grid((unsigned)((long long)p.B * p.T * p.heads)), block(ca::kJoinWarps * 32);
+                          dim3((unsigned)(plan.shares + plan.items)), dim3(ca::kThreads), sizeof(ca::Smem), st, p));
+    // (an item's CTAs are its share of all keys: of as many equal ones, about this many)
+    const long long parts = (plan.items > 0 ? plan.shares / plan.items : 0) + p.n_shared;
+    const int warps = (int)std::min<long long>(ca::kJoinWarps, std::max<long long>(1, (parts + 7) / 8));
+    const dim3 grid((unsigned)((long long)p.B * p.T * p.heads)), block((unsigned)warps * 32);
     AttnKernel join = ca::join_kernel<false, ca::kWide>;
     if (plan.form == ca::kFew) join = q_f32 ? ca::join_kernel<true, ca::kFew> : ca::join_kernel<false, ca::kFew>;
     if (plan.form == ca::kEight) join = q_f32 ? ca::join_kernel<true, ca::kEight> : ca::join_kernel<false, ca::kEight>;
