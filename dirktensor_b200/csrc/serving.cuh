@@ -134,7 +134,7 @@ PrefixPlan plan_prefix(int B, int T, int heads, int kv_heads, int q_f32, int pre
     PrefixPlan s{};
     s.rows = B * T * (heads / kv_heads);
     s.pairs = q_f32 || s.rows <= 128;
-    s.blocks = (s.rows + (s.pairs ? 127 : 255)) / (s.pairs ? 128 : 256);
+    s.blocks = (s.rows - 1) / (s.pairs ? 128 : 256) + 1;
     s.tiles = (int)(((long long)prefix_len + 127) / 128);
     const long long groups = (long long)kv_heads * s.blocks;
     s.split = (int)std::max<long long>(1, std::min<long long>(s.tiles, kPlanSms / groups));
@@ -345,6 +345,19 @@ int cache_attn(const dt_kv_cache* cache, const void* q, long long q_batch_stride
     return launch_stream(p, plan, cache->format, q_f32, st);
 }
 
+// Whether N rows of V elements at b may be written while those at a are read, each thread reading what it
+// writes before it does: the rows are the same, or none of one lies in one of the other.
+bool writes_apart(const void* a, long long lda, const void* b, long long ldb, int N, int V, int elem) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    if (x == y) return lda == ldb || N == 1;
+    const auto end = [&](uintptr_t at, long long ld) { return (unsigned __int128)at + ((unsigned __int128)(N - 1) * ld + V) * elem; };
+    if (y >= end(x, lda) || x >= end(y, ldb)) return true;
+    // rows between each other's: at an even distance, so that the first two show it
+    const unsigned long long step = (unsigned long long)lda * elem, off = (x < y ? y - x : x - y) % step;
+    const unsigned long long row = (unsigned long long)V * elem;
+    return lda == ldb && off >= row && off <= step - row;
+}
+
 }  // namespace
 
 extern "C" {
@@ -440,6 +453,8 @@ int dt_token_log_probs_bwd(const void* logits, int logits_f32, long long ld, int
     if (!lse) return fail(DT_ERR_INVALID_ARGUMENT, "null lse");
     if (d_log_prob && !targets) return fail(DT_ERR_INVALID_ARGUMENT, "d_log_prob needs targets");
     if (d_entropy && !entropy) return fail(DT_ERR_INVALID_ARGUMENT, "d_entropy needs entropy");
+    if (!writes_apart(logits, ld, d_logits, d_ld, N, V, logits_f32 ? 4 : 2))
+        return fail(DT_ERR_INVALID_ARGUMENT, "d_logits may be the logits' own rows, and must not overlap them otherwise");
     int dev;
     DT_TRY(prepare_device(&dev));
     namespace lp = dt::logprobs;

@@ -20,6 +20,7 @@ from .attention import FlashAttentionResult, head_dim, n_heads
 _CODES = {"int8": (torch.int8, 0), "e4m3": (torch.float8_e4m3fn, 1)}
 _FORMAT_OF = {torch.int8: 0, torch.float8_e4m3fn: 1}
 _VALUES = (torch.bfloat16, torch.float32)
+_INT_MAX = 2**31 - 1  # counts are ints at the C ABI
 
 
 # A decoding step's calls take a few microseconds on the GPU, so the checks below look at each
@@ -49,6 +50,8 @@ def _values(name: str, t, index: int, heads: Optional[int] = None):
     if _index_of(t) != index or t.dtype not in _VALUES or t.dim() != 4 or t.shape[3] != head_dim:
         raise ValueError(f"{name} must be a bfloat16 or float32 tensor [B, T, heads, {head_dim}] on cuda:{index}")
     shape, s = t.shape, t.stride()
+    if shape[0] * shape[1] > _INT_MAX:  # (a broadcast tensor)
+        raise ValueError(f"{name} has too many tokens")
     if heads is not None and shape[2] != heads:
         raise ValueError(f"{name} must have {heads} heads")
     if ((s[3] != 1 or (s[2] != head_dim and shape[2] > 1) or (s[0] | s[1]) % (16 // t.element_size()) or s[0] < 0
@@ -114,7 +117,7 @@ class KVCache:
             if not (isinstance(t, torch.Tensor) and t.device == k.device and t.dtype == dtype and t.shape == shape
                     and t.is_contiguous()):
                 raise ValueError(f"{name} must be a contiguous {dtype} tensor {list(shape)} on {k.device}")
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self._arrays = k, v, k_scale, v_scale
         self.num_pages, self.kv_heads, self.page_size = k.shape[:3]
         if self.page_size not in (16, 32, 64, 128, 256):
             raise ValueError("page_size must be 16, 32, 64, 128 or 256")
@@ -122,6 +125,12 @@ class KVCache:
         self._c = dt_kv_cache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), self.num_pages,
                               self.page_size, self.kv_heads, _FORMAT_OF[k.dtype])
         self._ref = ctypes.byref(self._c)
+
+    # (the library keeps their addresses: they are not to be replaced)
+    k = property(lambda self: self._arrays[0])
+    v = property(lambda self: self._arrays[1])
+    k_scale = property(lambda self: self._arrays[2])
+    v_scale = property(lambda self: self._arrays[3])
 
     @property
     def format(self) -> str:
@@ -149,6 +158,8 @@ class KVCache:
         if not isinstance(page_table, torch.Tensor) or page_table.dim() != 2:
             raise ValueError("page_table must be an int32 tensor [B, pages]")
         B, T = page_table.shape[0], int(T)
+        if not 0 <= T <= _INT_MAX:
+            raise ValueError("T must be >= 0 and below 2^31")
         table, stride, n = _table(page_table, self._index, B)
         k = torch.empty((B, T, self.kv_heads, head_dim), dtype=dtype, device=self.device)
         v = torch.empty_like(k)
@@ -221,8 +232,8 @@ def prefix_attention_forward(q, cache: KVCache, prefix_pages, prefix_len: int, p
     B, T, H, _ = shape
     prefix_len = int(prefix_len)
     pages = _ints("prefix_pages", prefix_pages, index, None)
-    if prefix_len < 0 or prefix_len > (0 if prefix_pages is None else prefix_pages.shape[0] * cache.page_size):
-        raise ValueError("prefix_len must be >= 0 and within prefix_pages")
+    if not 0 <= prefix_len <= min(_INT_MAX, 0 if prefix_pages is None else prefix_pages.shape[0] * cache.page_size):
+        raise ValueError("prefix_len must be >= 0, within prefix_pages and below 2^31")
     if (page_table is None) != (seq_lens is None):
         raise ValueError("page_table and seq_lens come together")
     table, stride, n = (None, 0, 0) if page_table is None else _table(page_table, index, B)
@@ -248,6 +259,8 @@ def _rows(name, t):
     if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in _VALUES and t.dim() >= 1 and t.shape[-1] >= 1):
         raise ValueError(f"{name} must be a bfloat16 or float32 CUDA tensor [..., vocabulary]")
     V = t.shape[-1]
+    if V > 1 << 30 or t.numel() > V * _INT_MAX:
+        raise ValueError(f"{name} must have at most 2^30 entries a row and fewer than 2^31 rows")
     if t.is_contiguous():
         return (t.shape[0] if t.dim() == 2 else t.numel() // V), V
     n, ld = 1, None
@@ -305,7 +318,7 @@ def token_log_probs(logits, targets=None, top: int = 0) -> TokenLogProbs:
 def token_log_probs_backward(logits, targets, lse, entropy, d_log_prob, d_entropy=None, out=None):
     """Gradient of token_log_probs with respect to the logits, of their shape and type, from its
     lse and entropy and the upstream gradients (fp32; d_log_prob or d_entropy may be None).
-    ``out`` may be the logits themselves."""
+    ``out`` may be the logits themselves, and must not overlap them otherwise."""
     n, ld = _rows("logits", logits)
     V, shape, dev = logits.shape[-1], logits.shape[:-1], logits.device
     t, t64 = _targets(targets, shape, dev)

@@ -130,3 +130,26 @@ def test_importing_the_package_does_not_need_the_serving_module():
     code = "import sys; import dirktensor_b200; assert 'dirktensor_b200.serving' not in sys.modules; " \
            "assert 'torch' not in sys.modules; dirktensor_b200.KVCache; assert 'torch' in sys.modules"
     subprocess.run([sys.executable, "-c", code], check=True)
+
+
+def test_gradient_that_overlaps_its_logits_is_refused():
+    L = _lib.lib()
+
+    def refused(delta, N=4, V=100, ld=100, dld=100, f32=1):
+        status = L.dt_token_log_probs_bwd(FAKE, f32, ld, N, V, None, 0, FAKE, FAKE, None, None, FAKE + delta, dld, None)
+        return status == 1 and b"overlap" in L.dt_last_error()
+
+    assert refused(4) and refused(-4) and refused(396) and refused(2, f32=0)      # part of a row
+    assert refused(400) and refused(-400) and refused(1200)                       # another row's place
+    assert refused(0, ld=104) and refused(0, dld=1 << 40) and refused(400, ld=1 << 40)
+    assert refused(500, ld=250, N=2) and refused(-500, ld=250)   # rows at 500 and 900 bytes: in 1000..1399; at -100: in 0..399
+    assert not refused(404, ld=202, dld=202, V=101)              # halves of the same rows
+    assert refused(404, ld=201, dld=201, V=101) and refused(400, ld=201, dld=201, V=101)
+    assert not refused(0) and not refused(1600) and not refused(-1600) and not refused(0, N=1, ld=104)
+    assert not refused(400, N=1) and refused(396, N=1) and not refused(0, N=0)
+
+
+def test_cache_arrays_cannot_be_replaced_under_their_addresses():
+    for name in ("k", "v", "k_scale", "v_scale"):
+        with pytest.raises(AttributeError):
+            setattr(dt.KVCache.__new__(dt.KVCache), name, None)

@@ -822,3 +822,37 @@ def test_calls_on_two_streams_at_once_keep_their_results(dt, cuda):
     for out in got:
         for a, b in zip(out, want):
             assert torch.equal(a, b)
+
+
+def test_counts_past_32_bits_are_refused(dt, cuda):
+    cache = dt.KVCache(1, 16, 1, device=cuda)
+    one = torch.ones((1, 1, 1, 128), dtype=torch.bfloat16, device=cuda)
+    table = torch.zeros((1, 1), dtype=torch.int32, device=cuda)
+    many = one.expand(1, 2**32 + 1, 1, 128)  # (no memory of its own)
+    for bad in (lambda: cache.append(many, many, table), lambda: cache.read(table, None, -1),
+                lambda: cache.read(table, None, 2**32 + 1),
+                lambda: dt.cache_attention_forward(many, cache, table, table[0], 1.0),
+                lambda: dt.prefix_attention_forward(one, cache, table[0], 2**32 + 1, None, None, 1.0)):
+        with pytest.raises(ValueError):
+            bad()
+    assert float(cache.k_scale.abs().sum()) == 0.0
+    long = torch.empty(2**32 + 5, dtype=torch.bfloat16, device=cuda)  # 8.6 GB
+    for bad in (long, long[:, None]):
+        with pytest.raises(ValueError):
+            dt.token_log_probs(bad)
+
+
+def test_gradient_into_the_other_half_of_the_logits_rows(dt, cuda):
+    g = gen(cuda, 5)
+    both = torch.randn((9, 2, 333), generator=g, device=cuda)
+    x, out, t = both[:, 0], both[:, 1], torch.randint(0, 333, (9,), generator=g, device=cuda)
+    r = dt.token_log_probs(x, t)
+    up = torch.randn((9,), generator=g, device=cuda)
+    plain = dt.token_log_probs_backward(x.contiguous(), t, r.lse, r.entropy, up)
+    kept = x.clone()
+    dt.token_log_probs_backward(x, t, r.lse, r.entropy, up, out=out)
+    # the same formula in the same order whatever the alignment
+    assert torch.equal(x, kept) and torch.equal(out, plain)
+    with pytest.raises(dt.DTError, match="overlap"):
+        dt.token_log_probs_backward(both.view(18, 333)[:-1], None, r.lse.new_zeros(17), None, None,
+                                    out=both.view(18, 333)[1:])
