@@ -45,6 +45,15 @@ def _index_of(t) -> int:
     return t.get_device() if isinstance(t, torch.Tensor) else -1
 
 
+def _new(shape, dtype, device):
+    """torch.empty(shape), whose own checks take a microsecond more than empty_strided's."""
+    strides, n = [1] * len(shape), 1
+    for i in range(len(shape) - 1, -1, -1):
+        strides[i] = n
+        n *= shape[i] or 1
+    return torch.empty_strided(shape, strides, dtype=dtype, device=device)
+
+
 def _values(name: str, t, index: int, heads: Optional[int] = None):
     """Shape and strides of [B, T, heads, 128] of bf16 or fp32 whose rows start on 16-byte boundaries."""
     if _index_of(t) != index or t.dtype not in _VALUES or t.dim() != 4 or t.shape[3] != head_dim:
@@ -161,7 +170,7 @@ class KVCache:
         if not 0 <= T <= _INT_MAX:
             raise ValueError("T must be >= 0 and below 2^31")
         table, stride, n = _table(page_table, self._index, B)
-        k = torch.empty((B, T, self.kv_heads, head_dim), dtype=dtype, device=self.device)
+        k = _new((B, T, self.kv_heads, head_dim), dtype, self.device)
         v = torch.empty_like(k)
         _call(self._index, lib().dt_kv_cache_read, self._ref, k.data_ptr(), v.data_ptr(), dtype == torch.float32, table,
               stride, n, _ints("start", start, self._index, B), _ints("lens", lens, self._index, B), B, T)
@@ -171,12 +180,12 @@ class KVCache:
 def _outputs(q, shape, out, return_stats):
     """Output and statistics tensors, and their addresses."""
     if out is None:
-        out = torch.empty_like(q) if q.is_contiguous() else torch.empty(shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q) if q.is_contiguous() else _new(shape, q.dtype, q.device)
     elif not (out.device == q.device and out.dtype == q.dtype and out.shape == shape and out.is_contiguous()):
         raise ValueError("out must be a contiguous tensor of q's shape and type")
     if not return_stats:
         return out, None, None, out.data_ptr(), None, None
-    m, l = (torch.empty(shape[:3], dtype=torch.float32, device=q.device) for _ in range(2))
+    m, l = (_new(shape[:3], torch.float32, q.device) for _ in range(2))
     return out, m, l, out.data_ptr(), m.data_ptr(), l.data_ptr()
 
 
@@ -193,7 +202,7 @@ def _workspace(cache, *sizes):
         nbytes = _workspace_bytes[sizes] = (lib().dt_prefix_attn_workspace_bytes(*sizes))
     if nbytes == 0:
         return None, None, 0
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=cache.device)
+    ws = torch.empty_strided((nbytes,), (1,), dtype=torch.uint8, device=cache.device)
     return ws, ws.data_ptr(), nbytes
 
 
@@ -302,12 +311,12 @@ def token_log_probs(logits, targets=None, top: int = 0) -> TokenLogProbs:
     top = int(top)
     if not 0 <= top <= min(32, V):
         raise ValueError("top must be 0..32 and at most the vocabulary")
-    lse = torch.empty(shape, dtype=torch.float32, device=dev)
+    lse = _new(shape, torch.float32, dev)
     ent = torch.empty_like(lse)
     lp = None if targets is None else torch.empty_like(lse)
     ids = tlp = None
     if top:
-        tlp = torch.empty(shape + (top,), dtype=torch.float32, device=dev)
+        tlp = _new(shape + (top,), torch.float32, dev)
         ids = torch.empty_like(tlp, dtype=torch.int32)
     _call(logits.get_device(), lib().dt_token_log_probs, logits.data_ptr(), logits.dtype == torch.float32, ld, n, V, t, t64, top,
           None if lp is None else lp.data_ptr(), ent.data_ptr(), lse.data_ptr(), ids.data_ptr() if top else None,
@@ -333,7 +342,7 @@ def token_log_probs_backward(logits, targets, lse, entropy, d_log_prob, d_entrop
                 and x.is_contiguous()):
             raise ValueError(f"{name} must be a contiguous float32 tensor {list(shape)} on {dev}")
     if out is None:
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+        out = torch.empty_like(logits) if logits.is_contiguous() else _new(logits.shape, logits.dtype, dev)
     elif out.device != dev or out.dtype != logits.dtype or out.shape != logits.shape:
         raise ValueError("out must have the logits' shape and type")
     dn, dld = _rows("out", out)
