@@ -298,6 +298,8 @@ int cache_attn(const dt_kv_cache* cache, const void* q, long long q_batch_stride
     if (!o || !aligned16(o)) return fail(DT_ERR_INVALID_ARGUMENT, "o must be non-null and 16-byte aligned");
     if (prefix_len < 0 || (prefix_len > 0 && !prefix_pages))
         return fail(DT_ERR_INVALID_ARGUMENT, "prefix_len must be >= 0, with its pages");
+    // (positions are 32-bit, and the kernel looks up pages a few tiles past the end)
+    if (prefix_len > (1 << 30)) return fail(DT_ERR_INVALID_ARGUMENT, "prefix_len must be at most 2^30");
     if ((long long)B * T * heads > 0x7fffffffll) return fail(DT_ERR_INVALID_ARGUMENT, "B * T * heads must be below 2^31");
     p.q = q;
     p.q_batch = q_batch_stride;

@@ -241,8 +241,8 @@ def prefix_attention_forward(q, cache: KVCache, prefix_pages, prefix_len: int, p
     B, T, H, _ = shape
     prefix_len = int(prefix_len)
     pages = _ints("prefix_pages", prefix_pages, index, None)
-    if not 0 <= prefix_len <= min(_INT_MAX, 0 if prefix_pages is None else prefix_pages.shape[0] * cache.page_size):
-        raise ValueError("prefix_len must be >= 0, within prefix_pages and below 2^31")
+    if not 0 <= prefix_len <= min(1 << 30, 0 if prefix_pages is None else prefix_pages.shape[0] * cache.page_size):
+        raise ValueError("prefix_len must be >= 0, within prefix_pages and at most 2^30")
     if (page_table is None) != (seq_lens is None):
         raise ValueError("page_table and seq_lens come together")
     table, stride, n = (None, 0, 0) if page_table is None else _table(page_table, index, B)

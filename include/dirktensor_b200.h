@@ -434,7 +434,7 @@ int dt_cache_attn_fwd(const dt_kv_cache* cache, const void* q, long long q_batch
                       int heads, float scale, void* workspace, size_t workspace_bytes, void* stream);
 /* The same for a batch whose sequences share their first prefix_len tokens:
  * every query that is not padding sees all keys of the prefix (prefix_pages:
- * device int[ceil(prefix_len / page_size)]) and then its own sequence's keys
+ * device int[ceil(prefix_len / page_size)]; prefix_len at most 2^30) and then its own sequence's keys
  * as above, whose positions, page_table and seq_lens count from the prefix's
  * end.  The prefix is read once for the whole batch, not once per sequence.
  * max_pages may be 0 (no keys of their own); B is at most 8192.  workspace: at least
