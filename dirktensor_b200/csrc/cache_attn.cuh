@@ -534,7 +534,8 @@ __device__ __forceinline__ void attend(const Params& p, Stage* ring, int b, int 
                     const float best = column_max(top[z][c]);
                     if (best * st.f[z][c] > 32768.f) {
                         const float fn = pow2(min(max(8 - exponent(best), -120), 100));
-                        if (st.f[z][c] != pow2(100)) st.rescale(z, c, fn / st.f[z][c]);  // by a power of two
+                        // (a power of two, 0 below 2^-149; also from the first factor, with which small weights may have been summed)
+                        st.rescale(z, c, fn / st.f[z][c]);
                         st.f[z][c] = fn;
                     }
                 }

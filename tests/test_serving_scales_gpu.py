@@ -1,0 +1,89 @@
+"""GPU tests of the cache attention and the prefix attention where rows of V differ much in size.
+
+Every value has its bound from serving_ref.attention: the second product takes the weights p * v_scale as fp16
+numbers (fp32 queries: as two), scaled so that the largest of those summed so far is well inside fp16's range whatever
+came before it."""
+import math
+
+import pytest
+import torch
+
+import serving_ref as ref
+from serving_ref import D
+
+pytestmark = pytest.mark.gpu
+
+SCALE = 1.0 / math.sqrt(D)
+BF16, F32 = torch.bfloat16, torch.float32
+LOG2 = math.log(2.0)
+
+
+@pytest.fixture(scope="module")
+def dt(cuda):
+    import dirktensor_b200
+
+    return dirktensor_b200
+
+
+def given(dt, cuda, fmt, dtype, B, T, heads, group, scores, sizes, page=64, spare=0):
+    """A cache whose key j of every sequence and head has about the score scores[j] (in log2 units) for every query, and a V
+    row of about the size sizes[j] (0: a row of zeros).  Queries are 16 in dim 0, so K's code and scale there give the score;
+    the rest of K is noise below it.  Returns cache, page table [B, pages], lengths, queries."""
+    g = torch.Generator(device=cuda)
+    g.manual_seed(len(scores))
+    n = len(scores)
+    per = -(-n // page)
+    c = dt.KVCache.from_tensors(*ref.make_cache(g, fmt, B * per + spare, heads, page, cuda))
+    table = torch.randperm(c.num_pages, generator=g, device=cuda)[: B * per].view(B, per).to(torch.int32)
+    want = torch.tensor(scores, device=cuda, dtype=torch.float64) * LOG2  # in nats
+    rows = torch.arange(n, device=cuda)
+    at, off = table.long()[:, rows // page], rows % page                 # [B, n], [n]
+    code = torch.zeros((n, D), device=cuda)
+    code[:, 0] = torch.where(want < 0, -64.0, 64.0)
+    ks = (want.abs() / (SCALE * 16 * 64)).float()
+    vs = torch.tensor(sizes, device=cuda, dtype=torch.float64) / ref.TOP[fmt]
+    for b in range(B):
+        c.k[at[b], :, off] = code.to(c.k.dtype)[:, None].expand(n, heads, D)
+        c.k_scale[at[b], :, off] = ks[:, None].expand(n, heads)
+        c.v_scale[at[b], :, off] = vs.float()[:, None].expand(n, heads)
+    q = torch.zeros((B, T, heads * group, D), device=cuda)
+    q[..., 0] = 16.0
+    return c, table, torch.full((B,), n, dtype=torch.int32, device=cuda), q.to(dtype)
+
+
+# Which keys come first (in every warp's first tile of 32, and the tiles after it), and which after them.
+def tiny_rows(first, rest, size):
+    """Rows of V of 2^size, then ordinary ones."""
+    return [0.0] * (first + rest), [2.0 ** size] * first + [1.0] * rest
+
+
+def zero_row_at_the_peak(first, rest, below):
+    """In each tile of 32 a key with a V row of zeros leads the others by `below` log2 units; an ordinary key at
+    the peak follows in each of the tiles after them."""
+    scores = [0.0 if j % 32 == 5 else -float(below) for j in range(first)]
+    sizes = [0.0 if j % 32 == 5 else 1.0 for j in range(first)]
+    return scores + [0.0 if j % 32 == 9 else -30.0 for j in range(rest)], sizes + [1.0] * rest
+
+
+EARLY = [pytest.param(tiny_rows, (size,), id="tiny%d" % size) for size in (-100, -90, -80)] + [
+    pytest.param(zero_row_at_the_peak, (below,), id="zero_peak_%d" % below) for below in (78, 80, 84, 88, 96)]
+
+
+# A warp's second tile comes 4 * split tiles after its first.  One item of up to 128 tiles is a cluster of 8: 1024 keys on.
+# Eight items over a wide page table are shared out: 592 CTAs, 74 an item, 9472 keys on (fewer where fewer CTAs fit).
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("group", [1, 8, 20])
+@pytest.mark.parametrize("early, args", EARLY)
+def test_sums_of_the_first_factor_are_kept_in_later_units(dt, cuda, fmt, dtype, group, early, args):
+    c, table, lens, q = given(dt, cuda, fmt, dtype, 1, 1, 1, group, *early(1024, 1999, *args))
+    got = dt.cache_attention_forward(q, c, table, lens, SCALE, return_stats=True)
+    ref.check_attention(got, ref.attention(q, c, table, lens, SCALE))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("early, args", EARLY)
+def test_sums_of_the_first_factor_are_kept_where_keys_are_shared_out(dt, cuda, dtype, early, args):
+    c, table, lens, q = given(dt, cuda, "int8", dtype, 1, 1, 8, 1, *early(9472, 14000, *args))
+    got = dt.cache_attention_forward(q, c, table, lens, SCALE, return_stats=True)
+    ref.check_attention(got, ref.attention(q, c, table, lens, SCALE))
