@@ -57,6 +57,7 @@ constexpr int kStages = 3;     // pieces (K or V of a tile) of a warp: one in us
 constexpr int kMaxCluster = 8;
 constexpr float kGrow = 8.f;   // the running maximum moves when a score passes it by this much (log2)
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kFirstFactor = 118;  // log2 of the weights' factor before any: rows of 2^-100, the smallest kept, then weigh 2^8 or more
 
 // K or V of one tile of one warp.  Every lane copies the 16-byte pieces that it will read itself,
 // at [piece][lane], so that reads have no bank conflicts and need no exchange; the scales are read
@@ -172,6 +173,8 @@ __device__ __forceinline__ float warp_max(float x) {
 
 // 2^e for e in [-126, 127]
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
+// 2^e for e <= 127, 0 where that is below the normal numbers
+__device__ __forceinline__ float pow2_or_0(int e) { return e < -126 ? 0.f : pow2(e); }
 // floor(log2 |x|) of a normal number
 __device__ __forceinline__ int exponent(float x) { return ((__float_as_int(x) >> 23) & 0xff) - 127; }
 
@@ -236,10 +239,10 @@ template <int kForm>
 struct State {
     static constexpr int kSets = kForm == kWide ? 2 : 1, kCols = kForm == kFew ? 1 : 2;
     float acc[kSets][8][4];  // of step j: dims 16g + 2j (0, 1) and 16g + 2j + 1 (2, 3), queries 2t (0, 2) and 2t + 1 (1, 3)
-    float m[kSets][kCols];       // running maxima that the sums refer to (log2 units; -inf: no key seen)
+    float m[kSets][kCols];       // running maxima that the sums refer to (log2 units, whole numbers; -inf: no key seen)
     float l[kSets][kCols];       // this lane's share of the sums of p
     float mx[kSets][kCols];      // this lane's largest scores
-    float f[kSets][kCols];       // acc holds sums of p * v_scale * f: f keeps them in fp16's range
+    float f[kSets][kCols];       // acc holds sums of p * v_scale * f, f = 2^e: the largest so far lies in 2^8..2^15 (fp16)
     // dim 16g + d of query 2t + c (kFew: of query t, the sum of its two columns)
     __device__ __forceinline__ float sum(int z, int c, int d) const {
         const float* a = acc[z][d >> 1] + 2 * (d & 1);
@@ -404,7 +407,7 @@ __device__ __forceinline__ void attend(const Params& p, Stage* ring, int b, int 
 #pragma unroll
             for (int e = 0; e < 4; ++e) st.acc[z][j][e] = 0.f;
 #pragma unroll
-        for (int c = 0; c < kCols; ++c) st.m[z][c] = st.mx[z][c] = -INFINITY, st.l[z][c] = 0.f, st.f[z][c] = pow2(100);
+        for (int c = 0; c < kCols; ++c) st.m[z][c] = st.mx[z][c] = -INFINITY, st.l[z][c] = 0.f, st.f[z][c] = pow2(kFirstFactor);
     }
 
     int slot = 0;
@@ -488,12 +491,18 @@ __device__ __forceinline__ void attend(const Params& p, Stage* ring, int b, int 
                 for (int c = 0; c < kCols; ++c) {
                     const float best = column_max(top[z][c]);
                     if (best > st.m[z][c] + kGrow) {
+                        const float whole_best = ceilf(best);  // so that what it changes changes by powers of two
                         if (st.m[z][c] != -INFINITY || st.l[z][c] != 0.f) {  // (else there is nothing to scale yet)
-                            const float a = ex2_approx(st.m[z][c] - best);
-                            st.l[z][c] *= a;
-                            st.rescale(z, c, a);
+                            const int d = (int)fminf(whole_best - st.m[z][c], 1000.f);
+                            st.l[z][c] *= pow2_or_0(-d);
+                            // f grows as p shrinks, up to its first value: the largest weights summed so far stay where they
+                            // are in fp16's range, and so does acc.  (A factor that only fell would leave the weights behind
+                            // a large row of V that has vanished among fp16's subnormals.)
+                            const int was = exponent(st.f[z][c]), fe = min(was + d, kFirstFactor);
+                            if (fe != was + d) st.rescale(z, c, pow2_or_0(fe - was - d));
+                            st.f[z][c] = pow2(fe);
                         }
-                        st.m[z][c] = best;
+                        st.m[z][c] = whole_best;
                     }
                 }
         }
@@ -533,7 +542,7 @@ __device__ __forceinline__ void attend(const Params& p, Stage* ring, int b, int 
                 for (int c = 0; c < kCols; ++c) {
                     const float best = column_max(top[z][c]);
                     if (best * st.f[z][c] > 32768.f) {
-                        const float fn = pow2(min(max(8 - exponent(best), -120), 100));
+                        const float fn = pow2(min(max(8 - exponent(best), -120), kFirstFactor));
                         // (a power of two, 0 below 2^-149; also from the first factor, with which small weights may have been summed)
                         st.rescale(z, c, fn / st.f[z][c]);
                         st.f[z][c] = fn;

@@ -87,3 +87,48 @@ def test_sums_of_the_first_factor_are_kept_where_keys_are_shared_out(dt, cuda, d
     c, table, lens, q = given(dt, cuda, "int8", dtype, 1, 1, 8, 1, *early(9472, 14000, *args))
     got = dt.cache_attention_forward(q, c, table, lens, SCALE, return_stats=True)
     ref.check_attention(got, ref.attention(q, c, table, lens, SCALE))
+
+
+def large_rows_that_vanish(first, rest, ratio, below):
+    """Rows of V that are 2^ratio times as large as those that come later, whose scores are `below` log2 units higher."""
+    return [-float(below)] * first + [0.0] * rest, [2.0 ** ratio] * first + [1.0] * rest
+
+
+def large_rows_that_vanish_by_steps(first, rest, ratio, below):
+    """The same, with the scores going up through all keys after the first ones."""
+    scores, sizes = large_rows_that_vanish(first, rest, ratio, below)
+    return scores[:first] + [-below * (1 - j / (rest - 1)) for j in range(rest)], sizes
+
+
+VANISH = [pytest.param(f, (ratio, below), id="%s_%d_%d" % (name, ratio, below))
+          for name, f in (("at_once", large_rows_that_vanish), ("by_steps", large_rows_that_vanish_by_steps))
+          for ratio, below in ((24, 60), (34, 90), (34, 50), (60, 120))]
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("group", [1, 8, 20])
+@pytest.mark.parametrize("early, args", VANISH)
+def test_large_rows_that_vanish_leave_the_later_weights_their_digits(dt, cuda, fmt, dtype, group, early, args):
+    c, table, lens, q = given(dt, cuda, fmt, dtype, 1, 1, 1, group, *early(1024, 2999, *args))
+    got = dt.cache_attention_forward(q, c, table, lens, SCALE, return_stats=True)
+    ref.check_attention(got, ref.attention(q, c, table, lens, SCALE))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("early, args", VANISH)
+def test_large_rows_that_vanish_where_keys_are_shared_out(dt, cuda, dtype, early, args):
+    c, table, lens, q = given(dt, cuda, "int8", dtype, 1, 1, 8, 1, *early(9472, 30000, *args))
+    got = dt.cache_attention_forward(q, c, table, lens, SCALE, return_stats=True)
+    ref.check_attention(got, ref.attention(q, c, table, lens, SCALE))
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("n, heads", [(70, 2), (500, 1), (20000, 8)])
+def test_the_smallest_rows_that_are_kept_and_the_largest(dt, cuda, fmt, dtype, n, heads):
+    """All rows of V of 2^-100 (what is smaller is stored as zeros), of 2^100, or of both in turn."""
+    for sizes in ([2.0 ** -100] * n, [2.0 ** 100] * n, [2.0 ** (100 if j % 3 else -100) for j in range(n)]):
+        c, table, lens, q = given(dt, cuda, fmt, dtype, 1, 1, heads, 1, [0.25 * (j % 5) for j in range(n)], sizes)
+        got = dt.cache_attention_forward(q, c, table, lens, SCALE, return_stats=True)
+        ref.check_attention(got, ref.attention(q, c, table, lens, SCALE))
