@@ -462,9 +462,13 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const Params pp) {
                 by = m == -INFINITY ? 1.f : ex2_approx(m - top);
                 m = top;
             }
-            if (fn != fe && s > 0) by *= pow2(max(fn - fe, -126));
+            float by2 = 1.f;
+            if (fn != fe && s > 0) {  // (in two halves: down to 2^-220)
+                by2 = pow2((fn - fe) / 2);
+                by *= pow2(fn - fe - (fn - fe) / 2);  // (not one)
+            }
             fe = fn;
-            l *= by;
+            l = l * by * by2;
             if (s > 0 && __any_sync(0xffffffffu, by != 1.f)) {
 #pragma unroll 1
                 for (int cc = 0; cc < 8; ++cc) {
@@ -472,7 +476,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const Params pp) {
                     tmem_ld16(tO + cc * 16, o);
                     tmem_wait_ld();
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) o[e] *= by;
+                    for (int e = 0; e < 16; ++e) o[e] = o[e] * by * by2;
                     tmem_st16(tO + cc * 16, *reinterpret_cast<uint32_t(*)[16]>(o));
                 }
             }

@@ -132,3 +132,58 @@ def test_the_smallest_rows_that_are_kept_and_the_largest(dt, cuda, fmt, dtype, n
         c, table, lens, q = given(dt, cuda, fmt, dtype, 1, 1, heads, 1, [0.25 * (j % 5) for j in range(n)], sizes)
         got = dt.cache_attention_forward(q, c, table, lens, SCALE, return_stats=True)
         ref.check_attention(got, ref.attention(q, c, table, lens, SCALE))
+
+
+# ------------------------------------------------------- a shared prefix
+
+HEADS, SEEN = 75, [0, 41, 74]  # so many K/V heads that each CTA takes a whole prefix; the ones that are looked at
+
+
+def prefix_ref(dt, c, pages, n, q, group):
+    """softmax(scale q k^T) v over a prefix for the K/V heads in SEEN, with serving_ref.attention's bounds: (o, m, l and
+    the bound of each).  Here the weights p * v_scale are scaled so that a row's largest is at least 1: each is off by at
+    most 2^-25 of that, half of fp16's smallest step."""
+    o, m, l, o_tol, m_tol, l_tol = ([] for _ in range(6))
+    p_half = 2.0 ** -11 if q.dtype == BF16 else 0.0
+    for h in SEEN:
+        k, v, vs, codes, _ = ref.keys_of(c, pages, h, n)
+        x = q[:, :, h * group:(h + 1) * group].double()
+        s = torch.matmul(x, k.T) * SCALE
+        d = (132 * 2 * ref.EPS32 * torch.matmul(x.abs(), k.abs().T) * SCALE).amax(-1)
+        top = s.amax(-1)
+        w = torch.exp(s - top[..., None])
+        p = w / w.sum(-1, keepdim=True)
+        rel = 2 * d + 8 * ref.EPS32 * (1 + (p * (top[..., None] - s)).sum(-1)) + 2 * n * ref.EPS32
+        o.append(torch.matmul(p, v))
+        o_tol.append(ref.HALF[q.dtype] * o[-1].abs() + 2 * (rel + p_half)[..., None] * torch.matmul(p, v.abs()) +
+                     2.0 ** -25 * (p * vs).amax(-1, keepdim=True) * codes.sum(0))
+        m.append(top), m_tol.append(d + ref.EPS32 * top.abs())
+        l.append(w.sum(-1)), l_tol.append(rel * w.sum(-1))
+    return [torch.cat(x, dim=2) for x in (o, m, l, o_tol, m_tol, l_tol)]
+
+
+def check_prefix(dt, cuda, fmt, dtype, B, T, scores, sizes):
+    c, table, _, q = given(dt, cuda, fmt, dtype, 1, 1, HEADS, 1, scores, sizes)
+    q = q.expand(B, T, HEADS, D)
+    got = dt.prefix_attention_forward(q, c, table[0], len(scores), None, None, SCALE, return_stats=True)
+    dt.check_device_error()
+    ref.check_attention([x[:, :, SEEN] for x in got], prefix_ref(dt, c, table[0], len(scores), q, 1))
+
+
+# 128 rows at most: two warpgroups take tiles of 128 keys in turn; more: each takes 128 rows and all tiles.
+PREFIX_ROWS = [pytest.param(BF16, 3, 1, id="bf16_3"), pytest.param(BF16, 41, 4, id="bf16_164"), pytest.param(F32, 2, 1, id="fp32_2"),
+               pytest.param(F32, 45, 3, id="fp32_135")]
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype, B, T", PREFIX_ROWS)
+@pytest.mark.parametrize("size", [41, 60, 100])
+def test_prefix_rows_of_zeros_before_very_large_ones(dt, cuda, fmt, dtype, B, T, size):
+    check_prefix(dt, cuda, fmt, dtype, B, T, [0.0] * 900, [0.0] * 300 + [2.0 ** size] * 600)
+
+
+@pytest.mark.parametrize("dtype, B, T", PREFIX_ROWS)
+@pytest.mark.parametrize("step", [0, 1, 2, 3])
+def test_prefix_rows_that_grow_slowly(dt, cuda, dtype, B, T, step):
+    """Rows of V that double `step` times every two tiles: each change of the factor, the smallest too, reaches what is summed."""
+    check_prefix(dt, cuda, "int8", dtype, B, T, [0.5 * (j % 3) for j in range(1000)], [2.0 ** (step * (j // 256)) for j in range(1000)])
