@@ -18,8 +18,9 @@
 // range; fp32 queries go in as fp16(q) and the rest, as two products into one accumulator.  Scales stay out of
 // the operands: S is multiplied by k_scale (and the row's factor) in fp32, and the weights p by v_scale before they
 // are rounded to fp16 (once, at 2^-11 below a bf16 result's own 2^-8; for fp32 queries as two numbers
-// again).  f, a power of two that follows the largest v_scale so far, keeps p * v_scale * f
-// below 2^15; a change of it rescales O as a change of the running maximum does.
+// again).  f, a power of two of each row, keeps p * v_scale * f below 2^15 and the largest of them so far at 1 or
+// more, so that each is off by at most 2^-25 of that one: it falls where the row's largest weight asks for it and grows
+// as the running maximum takes older weights away.  Only where both together change the unit of O is O rescaled.
 //
 // Bound by its chain of steps rather than by a unit: per tile and warpgroup about 5000 cycles of softmax (two
 // passes over 128 TMEM columns; MUFU's share is 1024), 1400 of MMAs, and 10000 before the first tile is there (page
@@ -46,6 +47,10 @@ constexpr int kConvWarps = 4;
 constexpr int kMmaWarp = 8 + kConvWarps;
 constexpr int kThreads = (kMmaWarp + 1) * 32;
 constexpr float kGrow = 8.f;               // log2 units, as in flash_fwd.cuh
+// log2 of the weights' factor before any: rows of 2^-100, the smallest kept, weigh 2 or more, and 128 weights of 2^8 stay finite
+constexpr int kFirstFactor = 110;
+constexpr int kLowered = 7;                // a lowered factor puts the tile's largest weight below 2^kLowered (11: 86 us for 800 x 8 rows over 6143 keys and their own, 84 at 7)
+constexpr float kNear = 32.f;              // scales of a tile this near to each other need no look at its products: a bound is that near too
 
 struct Params {
     cache_attn::Params a;
@@ -62,7 +67,7 @@ struct __align__(1024) Smem {
     uint8_t v[2][kTileBytes];
     float ks[4][kBN];           // of tile t: at t & 3
     float vs[4][kBN];
-    float most[4][kConvWarps];  // largest v_scale of the 32 keys of each converting warp
+    float most[4][kConvWarps], least[4][kConvWarps];  // largest and smallest v_scale of the 32 keys of each converting warp
     uint32_t hidden[4][kConvWarps];  // keys past the prefix, or on a page that does not exist
     float factor[2][kBM];       // from S back to scores in log2 units (k_scale apart)
     float m[kBM], l[kBM], mx[kBM];  // of the second warpgroup, for the first (pairs)
@@ -220,10 +225,14 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const Params pp) {
                 if (!ok) break;
                 sm.ks[j & 3][cw * 32 + lane] = ks;
                 sm.vs[j & 3][cw * 32 + lane] = vs;
-                // (scales are not negative, so their bits order as they do; a NaN is not a largest)
+                // (scales are not negative, so their bits order as they do; a NaN is neither the largest nor the smallest)
                 const uint32_t most = __reduce_max_sync(0xffffffffu, vs > 0.f ? __float_as_uint(vs) : 0u);
+                const uint32_t least = __reduce_min_sync(0xffffffffu, see && vs == vs ? __float_as_uint(vs) : 0x7f800000u);
                 const uint32_t seen = __ballot_sync(0xffffffffu, see);
-                if (lane == 0) sm.most[j & 3][cw] = __uint_as_float(most), sm.hidden[j & 3][cw] = ~seen;
+                if (lane == 0) {
+                    sm.most[j & 3][cw] = __uint_as_float(most), sm.least[j & 3][cw] = __uint_as_float(least);
+                    sm.hidden[j & 3][cw] = ~seen;
+                }
                 put(sm.k[s], xk);
                 fence_async();
                 __syncwarp();
@@ -396,9 +405,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const Params pp) {
         const uint32_t tO = tmem + lane_off + 256 + i * 128;
         float factor = sm.factor[pp.pairs ? 0 : i][r];
         if (factor == 0.f) factor = 1e-37f;  // (no 0 * -inf; scores of 1e-37 weigh as 0 do)
-        // Weights are computed as p * f: l and O hold sums with that factor.
+        // Weights are computed as p * f, and O holds sums with that factor.
         float m = -INFINITY, l = 0.f, mx = -INFINITY;
-        int fe = 100;  // f = 2^fe
+        int fe = kFirstFactor;  // f = 2^fe
         const bool idle = row0 + (pp.pairs ? 0 : i * kBM) + (warp & 3) * 32 >= pp.rows;  // no query in this warp's rows
         bool ok = true;
         for (int s = 0; s < steps[i]; ++s) {
@@ -448,40 +457,60 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const Params pp) {
                 tmem_ld32(tS + cc * 32 + 32, xb);
                 largest(xa, cc);
                 wait_for(xb);
-                tmem_ld32(tS + ((cc * 32 + 64) & 127), xa);  // (the last: column 0 again, for the second pass)
+                if (cc == 0) tmem_ld32(tS + 64, xa);
                 largest(xb, cc + 1);
             }
             top *= factor;  // (-inf where every key is hidden; factor is not negative)
             if (top != top) top = -INFINITY;  // (a row whose query is not finite: no maximum)
             mx = fmaxf(mx, top);
-            const float4 most = *reinterpret_cast<const float4*>(sm.most[at]);
-            // p <= 2^8 (the lazy maximum), so p * v_scale * f < 2^15
-            const int fn = min(fe, min(max(6 - exponent(fmaxf(fmaxf(most.x, most.y), fmaxf(most.z, most.w))), -120), 100));
-            float by = 1.f;
+            int d = 0;  // log2 of the maximum's change: whole maxima change the sums by powers of two
             if (top > m + kGrow) {
-                by = m == -INFINITY ? 1.f : ex2_approx(m - top);
-                m = top;
+                const float whole = ceilf(top);
+                if (m != -INFINITY) d = (int)fminf(whole - m, 1000.f);
+                m = whole;
+                l *= cache_attn::pow2_or_0(-d);
             }
-            float by2 = 1.f;
-            if (fn != fe && s > 0) {  // (in two halves: down to 2^-220)
-                by2 = pow2((fn - fe) / 2);
-                by *= pow2(fn - fe - (fn - fe) / 2);  // (not one)
+            // The row's largest p * v_scale in this tile is below 2^eb.  By the largest score and the largest scale, where
+            // scales are within a factor of kNear; else from the products themselves, since the key of the largest
+            // score may have a row of V that is small, or zeros.
+            const float4 most4 = *reinterpret_cast<const float4*>(sm.most[at]), least4 = *reinterpret_cast<const float4*>(sm.least[at]);
+            const float most = fmaxf(fmaxf(most4.x, most4.y), fmaxf(most4.z, most4.w));
+            const float least = fminf(fminf(least4.x, least4.y), fminf(least4.z, least4.w));
+            int eb = (int)ceilf(fminf(fmaxf(top - m, -1000.f), 1000.f)) + exponent(most) + 1;
+            if (most > kNear * least) {  // (the same for all rows)
+                float z = -INFINITY;
+#pragma unroll 1
+                for (int cc = 0; cc < 8; ++cc) {
+                    float x[16];
+                    tmem_ld16(tS + cc * 16, x);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        z = fmaxf(z, fmaf(x[e] * sm.ks[at][cc * 16 + e], factor, __log2f(sm.vs[at][cc * 16 + e])));
+                }
+                eb = (int)ceilf(fminf(fmaxf(z - m, -1000.f), 1000.f)) + 1;
             }
+            // f grows as p shrinks, up to its first value, so that the largest weights summed so far stay where they are in
+            // fp16's range, and so does O; new ones at or above 2^15 lower it.
+            int fn = min(fe + d, kFirstFactor);
+            if (eb + fn > 15) fn = max(kLowered - eb, -120);
+            const int change = fn - fe - d;  // <= 0
             fe = fn;
-            l = l * by * by2;
-            if (s > 0 && __any_sync(0xffffffffu, by != 1.f)) {
+            if (s > 0 && __any_sync(0xffffffffu, change != 0)) {
+                const float by = cache_attn::pow2_or_0(change);
 #pragma unroll 1
                 for (int cc = 0; cc < 8; ++cc) {
                     float o[16];
                     tmem_ld16(tO + cc * 16, o);
                     tmem_wait_ld();
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) o[e] = o[e] * by * by2;
+                    for (int e = 0; e < 16; ++e) o[e] *= by;
                     tmem_st16(tO + cc * 16, *reinterpret_cast<uint32_t(*)[16]>(o));
                 }
             }
             // second pass: weights
-            const float m_safe = (m == -INFINITY ? 0.f : m) - (float)fe;
+            tmem_ld32(tS, xa);
+            const float m_safe = (m == -INFINITY ? 0.f : m) - (float)fe;  // exponents are those of p * f
             const uint64_t c2 = f2_pack(factor, factor), nm2 = f2_pack(-m_safe, -m_safe);
             uint64_t sum2[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
             auto weigh = [&](const float(&x)[32], int cc) {
@@ -522,7 +551,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const Params pp) {
             }
             float s0, s1;
             f2_unpack(f2_add(sum2[0], sum2[1]), s0, s1);
-            l += s0 + s1;
+            l = fmaf(s0 + s1, pow2(-fe), l);
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
@@ -534,7 +563,6 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const Params pp) {
         have = __all_sync(0xffffffffu, have);
         if (have) tc_fence_after();
         const float inv = pow2(-fe);
-        l *= inv;
         named_bar_sync(1, 256);  // both warpgroups' products are done: the K tiles are free
         if (pp.pairs) {
             // the second warpgroup's rows go through shared memory (64 KB: K's two tiles) to the first's

@@ -177,7 +177,7 @@ PREFIX_ROWS = [pytest.param(BF16, 3, 1, id="bf16_3"), pytest.param(BF16, 41, 4, 
 
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
 @pytest.mark.parametrize("dtype, B, T", PREFIX_ROWS)
-@pytest.mark.parametrize("size", [41, 60, 100])
+@pytest.mark.parametrize("size", [41, 60, 100, 112])
 def test_prefix_rows_of_zeros_before_very_large_ones(dt, cuda, fmt, dtype, B, T, size):
     check_prefix(dt, cuda, fmt, dtype, B, T, [0.0] * 900, [0.0] * 300 + [2.0 ** size] * 600)
 
@@ -187,3 +187,28 @@ def test_prefix_rows_of_zeros_before_very_large_ones(dt, cuda, fmt, dtype, B, T,
 def test_prefix_rows_that_grow_slowly(dt, cuda, dtype, B, T, step):
     """Rows of V that double `step` times every two tiles: each change of the factor, the smallest too, reaches what is summed."""
     check_prefix(dt, cuda, "int8", dtype, B, T, [0.5 * (j % 3) for j in range(1000)], [2.0 ** (step * (j // 256)) for j in range(1000)])
+
+
+def large_rows_beside(first, rest, ratio, below):
+    """Every other key has a row of V that is 2^ratio times as large, and a score `below` log2 units lower."""
+    n = first + rest
+    return [-float(below * (j % 2)) for j in range(n)], [2.0 ** (ratio * (j % 2)) for j in range(n)]
+
+
+def a_row_of_zeros_leads(first, rest, ratio, below):
+    """The key at the peak of every tile of 128 has a row of zeros, the others' rows are 2^ratio and far below it."""
+    n = first + rest
+    return [0.0 if j % 128 == 70 else -float(below) for j in range(n)], [0.0 if j % 128 == 70 else 2.0 ** ratio for j in range(n)]
+
+
+PREFIX_EARLY = EARLY + VANISH + [pytest.param(f, args, id="%s_%d_%d" % ((name,) + args)) for name, f, args in (
+    ("beside", large_rows_beside, (24, 70)), ("beside", large_rows_beside, (34, 90)), ("beside", large_rows_beside, (4, 30)),
+    ("beside", large_rows_beside, (60, 70)), ("zeros_lead", a_row_of_zeros_leads, (0, 40)), ("zeros_lead", a_row_of_zeros_leads, (50, 70)),
+    ("zeros_lead", a_row_of_zeros_leads, (-60, 30)))]
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype, B, T", PREFIX_ROWS)
+@pytest.mark.parametrize("early, args", PREFIX_EARLY)
+def test_prefix_rows_far_apart_in_size(dt, cuda, fmt, dtype, B, T, early, args):
+    check_prefix(dt, cuda, fmt, dtype, B, T, *early(256, 1300, *args))
