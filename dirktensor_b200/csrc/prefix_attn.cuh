@@ -93,6 +93,12 @@ __device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
+// (f2_fma flushes subnormal numbers to zero, also a factor)
+__device__ __forceinline__ uint64_t f2_fma_full(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // Waits for this thread's TMEM loads; x is valid afterwards, and the compiler uses it no earlier.
@@ -404,7 +410,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const Params pp) {
         const uint32_t tS = tmem + lane_off + i * 128;
         const uint32_t tO = tmem + lane_off + 256 + i * 128;
         float factor = sm.factor[pp.pairs ? 0 : i][r];
-        if (factor == 0.f) factor = 1e-37f;  // (no 0 * -inf; scores of 1e-37 weigh as 0 do)
+        if (factor == 0.f) factor = __uint_as_float(1u);  // 2^-149: no 0 * -inf where a key is hidden; scores of 2^-22 at most weigh as 0 do
         // Weights are computed as p * f, and O holds sums with that factor.
         float m = -INFINITY, l = 0.f, mx = -INFINITY;
         int fe = kFirstFactor;  // f = 2^fe
@@ -520,8 +526,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const Params pp) {
                     const float4 k = *reinterpret_cast<const float4*>(&sm.ks[at][cc * 32 + e]);
                     const float4 v = *reinterpret_cast<const float4*>(&sm.vs[at][cc * 32 + e]);
                     float y[4];
-                    f2_unpack(f2_fma(f2_mul(f2_pack(x[e], x[e + 1]), f2_pack(k.x, k.y)), c2, nm2), y[0], y[1]);
-                    f2_unpack(f2_fma(f2_mul(f2_pack(x[e + 2], x[e + 3]), f2_pack(k.z, k.w)), c2, nm2), y[2], y[3]);
+                    f2_unpack(f2_fma_full(f2_mul(f2_pack(x[e], x[e + 1]), f2_pack(k.x, k.y)), c2, nm2), y[0], y[1]);
+                    f2_unpack(f2_fma_full(f2_mul(f2_pack(x[e + 2], x[e + 3]), f2_pack(k.z, k.w)), c2, nm2), y[2], y[3]);
                     const uint64_t p0 = f2_pack(ex2_approx(y[0]), ex2_approx(y[1])), p1 = f2_pack(ex2_approx(y[2]), ex2_approx(y[3]));
                     sum2[0] = f2_add(sum2[0], p0);
                     sum2[1] = f2_add(sum2[1], p1);

@@ -212,3 +212,28 @@ PREFIX_EARLY = EARLY + VANISH + [pytest.param(f, args, id="%s_%d_%d" % ((name,) 
 @pytest.mark.parametrize("early, args", PREFIX_EARLY)
 def test_prefix_rows_far_apart_in_size(dt, cuda, fmt, dtype, B, T, early, args):
     check_prefix(dt, cuda, fmt, dtype, B, T, *early(256, 1300, *args))
+
+
+@pytest.mark.parametrize("dtype, B, T", PREFIX_ROWS)
+@pytest.mark.parametrize("size, scale", [(0.0, 1e-5), (0.0, -1e-5), (2.0 ** -100, 1e-5), (2.0 ** -60, 1e-30), (0.0, 1e-44), (1.0, 0.0),
+                                         (1.0, 1e-38), (2.0 ** -100, 1.0)])
+def test_prefix_of_small_queries_and_scales_with_hidden_keys(dt, cuda, dtype, B, T, size, scale):
+    """A query of zeros, or a scale so small that every score is next to none: an even average, and no NaN from keys past
+    the end or on a page that does not exist."""
+    n, heads = 400, 2
+    c, table, _, q = given(dt, cuda, "int8", dtype, 1, 1, heads, 1, [0.0] * n, [1.0] * n)
+    q = (torch.randn((B, T, heads, D), device=cuda, generator=torch.Generator(device=cuda).manual_seed(3)) * size).to(dtype)
+    c.k_scale.fill_(1.0)
+    pages = table[0].clone()
+    pages[3] = -1
+    for prefix, given_pages in ((100, table[0]), (n, pages), (n - 1, table[0])):
+        got = dt.prefix_attention_forward(q, c, given_pages, prefix, None, None, scale, return_stats=True)
+        want = list(ref.attention(q[:2], c, None, None, scale, prefix_pages=given_pages, prefix_len=prefix))
+        # The scale's product with a power of two is off by half of fp32's smallest step, 2^-150, where it is subnormal (by 2^-149
+        # where it would be zero); what it multiplies, a query of at most 2^14 times one code of 64, is at most 2^20.
+        want[4] = want[4] + 2.0 ** -129
+        ref.check_attention([x[:2] for x in got], want)
+        assert all(bool(torch.isfinite(x).all()) for x in got)
+        own = dt.cache_attention_forward(q, c, given_pages[None].expand(B, -1).contiguous(),
+                                         torch.full((B,), prefix + T - 1, dtype=torch.int32, device=cuda), scale)
+        assert bool(torch.isfinite(own).all())
