@@ -280,6 +280,22 @@ int serving_attrs() {
     return DT_OK;
 }
 
+// Whether the dense output at o may be written while queries are read: it is q's own dense memory (whoever writes a row
+// has read it), or no row of q lies in it.
+bool output_apart(const void* q, long long batch, long long token, const void* o, int B, int T, int heads, int elem) {
+    typedef unsigned __int128 Wide;
+    const Wide x = reinterpret_cast<uintptr_t>(q), y = reinterpret_cast<uintptr_t>(o);
+    const Wide row = (Wide)heads * dt::cache_attn::kD * elem, end = y + row * T * B;
+    if (x == y && (T == 1 || (Wide)token * elem == row) && (B == 1 || (Wide)batch * elem == row * T)) return true;
+    if (x >= end || x + ((Wide)(B - 1) * batch + (Wide)(T - 1) * token) * elem + row <= y) return true;
+    for (int b = 0; b < B; ++b) {  // the first row of sequence b that ends behind o's start
+        const Wide first = x + (Wide)b * batch * elem, step = (Wide)token * elem;
+        const Wide t = first + row > y ? 0 : step == 0 ? (Wide)T : (y - first - row) / step + 1;
+        if (t < (Wide)T && first + t * step < end) return false;
+    }
+    return true;
+}
+
 int cache_attn(const dt_kv_cache* cache, const void* q, long long q_batch_stride, long long q_token_stride, int q_f32,
                void* o, float* m, float* l, const int* prefix_pages, int prefix_len, const int* page_table,
                long long page_table_stride, int max_pages, const int* seq_lens, const int* q_lens, int B, int T,
@@ -301,6 +317,8 @@ int cache_attn(const dt_kv_cache* cache, const void* q, long long q_batch_stride
     // (positions are 32-bit, and the kernel looks up pages a few tiles past the end)
     if (prefix_len > (1 << 30)) return fail(DT_ERR_INVALID_ARGUMENT, "prefix_len must be at most 2^30");
     if ((long long)B * T * heads > 0x7fffffffll) return fail(DT_ERR_INVALID_ARGUMENT, "B * T * heads must be below 2^31");
+    if (!output_apart(q, q_batch_stride, q_token_stride, o, B, T, heads, q_f32 ? 4 : 2))
+        return fail(DT_ERR_INVALID_ARGUMENT, "o may be q's own dense memory, and must not overlap it otherwise");
     p.q = q;
     p.q_batch = q_batch_stride;
     p.q_token = q_token_stride;

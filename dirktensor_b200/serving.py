@@ -213,8 +213,8 @@ def cache_attention_forward(q, cache: KVCache, page_table, seq_lens, scale: floa
     q: [B, T, heads, 128] bf16 or fp32, heads a multiple of the cache's.  seq_lens (int32 [B])
     counts each sequence's tokens in the cache, the queries' own included: query t sees the keys
     j < seq_lens[b] - q_lens[b] + t + 1.  q_lens (int32 [B], default T): rows past it are padding
-    and come back as zeros, as do rows that see no key.  Returns the output [B, T, heads, 128]
-    of q's type, or with return_stats a ``FlashAttentionResult`` with softmax_m and softmax_l.
+    and come back as zeros, as do rows that see no key.  ``out`` may be a contiguous q itself, and must
+    not overlap it otherwise.  Returns the output [B, T, heads, 128] of q's type, or with return_stats a ``FlashAttentionResult`` with softmax_m and softmax_l.
     """
     index = cache._index
     shape, s = _values("q", q, index)

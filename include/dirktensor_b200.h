@@ -417,7 +417,8 @@ int dt_kv_cache_read(const dt_kv_cache* cache, void* k, void* v, int dst_f32, co
  * the keys j < seq_lens[b] - q_lens[b] + t + 1, i.e. seq_lens counts the
  * sequence's tokens in the cache, the call's own included, and the queries are
  * the last q_lens[b] of them.  q: bf16 or fp32 (q_f32 = 1) [B, T, heads, 128]
- * at the given strides (in elements); o: dense [B, T, heads, 128] of q's type;
+ * at the given strides (in elements); o: dense [B, T, heads, 128] of q's type,
+ * which may be q's own memory where q is dense, and must not overlap it otherwise;
  * softmax_m, softmax_l [B, T, heads] as dt_flash_fwd writes them, or NULL.
  * heads is a multiple of the cache's kv_heads: query head h reads K/V head
  * h / (heads / kv_heads).  q_lens: device int[B] or NULL (T).  Rows

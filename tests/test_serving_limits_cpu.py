@@ -22,3 +22,29 @@ def test_a_prefix_past_2_to_the_30_tokens_is_refused(prefix_len):
     status = L.dt_prefix_attn_fwd(cache(), 5 * FAKE, 512, 512, 0, 6 * FAKE, None, None, 7 * FAKE, prefix_len, None, 0, 0,
                                   None, None, 1, 1, 4, 0.1, 8 * FAKE, size, None)
     assert status == 1 and b"2^30" in L.dt_last_error(), L.dt_last_error()
+
+
+@pytest.mark.parametrize("prefix_len", [0, 100])
+def test_an_output_that_overlaps_its_queries_is_refused(prefix_len):
+    """One item's rows would be written while another's queries are still read.  In place is fine."""
+    L = _lib.lib()
+
+    def overlaps(delta, B=2, T=3, H=4, qb=None, qt=512, f32=0):
+        q = 64 * FAKE
+        qb = T * qt if qb is None else qb
+        args = (B, T, H, 4, f32, 64, 4, prefix_len)
+        status = L.dt_prefix_attn_fwd(cache(), q, qb, qt, f32, q + delta, None, None, 7 * FAKE, prefix_len, 9 * FAKE, 4, 4, 10 * FAKE,
+                                      None, B, T, H, 0.1, 8 * FAKE, L.dt_prefix_attn_workspace_bytes(*args) + 16, None)
+        assert status != 0
+        return status == 1 and b"overlap" in L.dt_last_error()
+
+    row = 4 * 128 * 2  # of one token
+    assert not overlaps(0) and not overlaps(0, f32=1)                       # in place
+    assert overlaps(16) and overlaps(-16) and overlaps(row) and overlaps(-row) and overlaps(5 * row) and overlaps(-5 * row)
+    assert not overlaps(6 * row) and not overlaps(-6 * row)                 # before and behind
+    assert overlaps(0, qt=1024) and overlaps(0, qb=4 * 512)                 # the same start, other rows
+    assert not overlaps(0, B=1, qb=16) and not overlaps(0, T=1, qt=16, qb=512) and not overlaps(0, B=1, T=1, qb=0, qt=0)
+    # queries of a fused projection, the output between its rows
+    assert not overlaps(row, B=1, T=2, qt=3 * 512) and overlaps(row + 16, B=1, T=2, qt=3 * 512)
+    assert overlaps(0, qb=0, qt=0) and overlaps(-16, qb=0, qt=0) and not overlaps(row, qb=0, qt=0)  # one query for all
+    assert overlaps(2 * row, B=2, T=2, qb=1 << 20, qt=512) is False and overlaps(2 << 20, B=3, T=2, qb=1 << 20, qt=512)

@@ -1,0 +1,42 @@
+"""GPU tests of what the serving operators take and refuse at the edges of their arguments."""
+import math
+
+import pytest
+import torch
+
+from serving_ref import D
+from test_serving_gpu import attention_case, ints
+
+pytestmark = pytest.mark.gpu
+
+SCALE = 1.0 / math.sqrt(D)
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+@pytest.fixture(scope="module")
+def dt(cuda):
+    import dirktensor_b200
+
+    return dirktensor_b200
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_outputs_in_place_and_outputs_that_overlap(dt, cuda, dtype):
+    B, T = 30, 5
+    c, pages, table, lens, q = attention_case(dt, cuda, 61, "int8", dtype, B, T, 2, 2, 16, [20 + i for i in range(B)], 200)
+    both = torch.empty((B + 1, T, 4, D), dtype=dtype, device=cuda)
+    for call in (lambda x, **kw: dt.cache_attention_forward(x, c, table, lens, SCALE, **kw),
+                 lambda x, **kw: dt.prefix_attention_forward(x, c, pages, 200, table, lens, SCALE, **kw),
+                 lambda x, **kw: dt.prefix_attention_forward(x, c, pages, 200, None, None, SCALE, **kw)):
+        want = call(q)
+        x = q.clone()
+        assert call(x, out=x) is x and torch.equal(x, want)
+        both[:B] = q
+        with pytest.raises(dt.DTError, match="overlap"):
+            call(both[:B], out=both[1:])
+        assert torch.equal(both[:B], q)
+        x = torch.zeros((B, T, 3, 4, D), dtype=dtype, device=cuda)
+        x[:, :, 1] = q
+        with pytest.raises(dt.DTError, match="overlap"):
+            call(x[:, :, 1], out=x.view(-1)[:q.numel()].view(q.shape))
+        assert torch.equal(call(x[:, :, 1]), want)
