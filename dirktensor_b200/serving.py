@@ -55,7 +55,8 @@ def _new(shape, dtype, device):
 
 
 def _values(name: str, t, index: int, heads: Optional[int] = None):
-    """Shape and strides of [B, T, heads, 128] of bf16 or fp32 whose rows start on 16-byte boundaries."""
+    """Shape and strides (of sequences and tokens) of [B, T, heads, 128] of bf16 or fp32 whose rows start on 16-byte
+    boundaries.  The stride of a dimension of one leads nowhere and counts as 0."""
     if _index_of(t) != index or t.dtype not in _VALUES or t.dim() != 4 or t.shape[3] != head_dim:
         raise ValueError(f"{name} must be a bfloat16 or float32 tensor [B, T, heads, {head_dim}] on cuda:{index}")
     shape, s = t.shape, t.stride()
@@ -63,10 +64,11 @@ def _values(name: str, t, index: int, heads: Optional[int] = None):
         raise ValueError(f"{name} has too many tokens")
     if heads is not None and shape[2] != heads:
         raise ValueError(f"{name} must have {heads} heads")
-    if ((s[3] != 1 or (s[2] != head_dim and shape[2] > 1) or (s[0] | s[1]) % (16 // t.element_size()) or s[0] < 0
-         or s[1] < 0 or t.data_ptr() & 15) and t.numel()):
+    batch, token = s[0] if shape[0] > 1 else 0, s[1] if shape[1] > 1 else 0
+    if ((s[3] != 1 or (s[2] != head_dim and shape[2] > 1) or (batch | token) % (16 // t.element_size())
+         or t.data_ptr() & 15) and t.numel()):
         raise ValueError(f"{name}: heads must be {head_dim} apart, and rows must start on 16-byte boundaries")
-    return shape, s
+    return shape, (batch, token)
 
 
 def _ints(name: str, t, index: int, n: Optional[int]):

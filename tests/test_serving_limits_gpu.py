@@ -40,3 +40,18 @@ def test_outputs_in_place_and_outputs_that_overlap(dt, cuda, dtype):
         with pytest.raises(dt.DTError, match="overlap"):
             call(x[:, :, 1], out=x.view(-1)[:q.numel()].view(q.shape))
         assert torch.equal(call(x[:, :, 1]), want)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("B, T", [(1, 1), (3, 1), (1, 4)])
+def test_strides_of_dimensions_of_one_do_not_matter(dt, cuda, dtype, B, T):
+    """Their strides lead nowhere: every row starts on a 16-byte boundary whatever they are."""
+    c, pages, table, lens, q = attention_case(dt, cuda, 62, "int8", dtype, B, T, 2, 1, 16, [20] * B, 40)
+    odd = q.as_strided(q.shape, (q.stride(0) if B > 1 else 7, q.stride(1) if T > 1 else 3, D, 1))
+    assert torch.equal(dt.cache_attention_forward(odd, c, table, lens, SCALE), dt.cache_attention_forward(q, c, table, lens, SCALE))
+    assert torch.equal(dt.prefix_attention_forward(odd, c, pages, 40, table, lens, SCALE),
+                       dt.prefix_attention_forward(q, c, pages, 40, table, lens, SCALE))
+    c.append(odd, odd, table)
+    k, v = c.k.clone(), c.v_scale.clone()
+    c.append(q, q, table)
+    assert torch.equal(c.k, k) and torch.equal(c.v_scale, v)
