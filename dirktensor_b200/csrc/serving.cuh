@@ -48,6 +48,19 @@ int check_strides(const char* name, const void* p, long long batch, long long to
     return DT_OK;
 }
 
+// Whether no two of a cache's arrays share memory.
+bool arrays_apart(const dt_kv_cache* c) {
+    const size_t rows = (size_t)c->num_pages * c->kv_heads * c->page_size;
+    const struct { const void* at; size_t bytes; } a[4] = {
+        {c->k, rows * dt::kv::kD}, {c->v, rows * dt::kv::kD}, {c->k_scale, rows * 4}, {c->v_scale, rows * 4}};
+    for (int i = 0; i < 4; ++i)
+        for (int j = 0; j < i; ++j) {
+            const uintptr_t x = reinterpret_cast<uintptr_t>(a[i].at), y = reinterpret_cast<uintptr_t>(a[j].at);
+            if (x < y ? y - x < a[i].bytes : x - y < a[j].bytes) return false;
+        }
+    return true;
+}
+
 }  // namespace
 
 extern "C" {
@@ -65,6 +78,7 @@ int dt_kv_cache_append(const dt_kv_cache* cache, const void* k, long long k_batc
     const int elem = src_f32 ? 4 : 2;
     DT_TRY(check_strides("k", k, k_batch_stride, k_token_stride, elem));
     DT_TRY(check_strides("v", v, v_batch_stride, v_token_stride, elem));
+    if (!arrays_apart(cache)) return fail(DT_ERR_INVALID_ARGUMENT, "cache arrays that are written must not overlap");
     p.s = {page_table, page_table_stride, max_pages, start, lens, B, T};
     p.k = k;
     p.v = v;

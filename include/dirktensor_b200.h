@@ -399,6 +399,7 @@ typedef struct dt_kv_cache {
  * or NULL (0, and T).  A token whose position is negative or past the table,
  * or whose page id is not in 0..num_pages-1, is skipped.  Where one call maps
  * several tokens to one slot, the one of the highest (b, position) is kept.
+ * The cache's four arrays must not overlap (a cache that is only read may share them).
  * Asynchronous on `stream`. */
 int dt_kv_cache_append(const dt_kv_cache* cache, const void* k, long long k_batch_stride, long long k_token_stride,
                        const void* v, long long v_batch_stride, long long v_token_stride, int src_f32,

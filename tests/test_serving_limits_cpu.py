@@ -48,3 +48,21 @@ def test_an_output_that_overlaps_its_queries_is_refused(prefix_len):
     assert not overlaps(row, B=1, T=2, qt=3 * 512) and overlaps(row + 16, B=1, T=2, qt=3 * 512)
     assert overlaps(0, qb=0, qt=0) and overlaps(-16, qb=0, qt=0) and not overlaps(row, qb=0, qt=0)  # one query for all
     assert overlaps(2 * row, B=2, T=2, qb=1 << 20, qt=512) is False and overlaps(2 << 20, B=3, T=2, qb=1 << 20, qt=512)
+
+
+def test_append_into_a_cache_whose_arrays_overlap_is_refused():
+    """K and V of a token would be written to one place at once.  Reading such a cache is fine."""
+    L = _lib.lib()
+    codes, scales = 8 * 4 * 64 * 128, 8 * 4 * 64 * 4  # bytes of cache()'s arrays
+
+    def refused(**kw):
+        status = L.dt_kv_cache_append(cache(**kw), 5 * FAKE, 512, 512, 6 * FAKE, 512, 512, 0, 7 * FAKE, 4, 4, None, None, 1, 1, None)
+        assert status != 0
+        return status == 1 and b"overlap" in L.dt_last_error()
+
+    assert not refused()
+    assert refused(v=FAKE) and refused(v_scale=3 * FAKE) and refused(v=FAKE + codes - 16) and refused(k=2 * FAKE + codes - 16)
+    assert not refused(v=FAKE + codes) and not refused(v_scale=3 * FAKE + scales) and refused(v_scale=3 * FAKE + scales - 16)
+    assert refused(k_scale=FAKE + 1024) and refused(v_scale=2 * FAKE - 16)
+    status = L.dt_kv_cache_read(cache(v=FAKE, v_scale=3 * FAKE), 5 * FAKE, 6 * FAKE, 0, 7 * FAKE, 4, 4, None, None, 1, 1, None)
+    assert status != 1
