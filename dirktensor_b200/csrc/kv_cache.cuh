@@ -85,7 +85,7 @@ __device__ __forceinline__ bool written_above(const Span& s, const Cache& c, int
         const unsigned skip = i / width;
         const int b2 = b + (int)skip;
         const int len = s.lens ? min(s.lens[b2], s.T) : s.T;
-        const long long first = s.start ? s.start[b2] : 0, last = first + len - 1;
+        const long long first = s.start ? s.start[b2] : 0, last = min(first + len - 1, 0x7fffffffll);
         if (len <= 0) continue;
         const long long j = (first >> c.page_shift) + (i - skip * width);
         if (j < 0 || j > (last >> c.page_shift) || j >= s.max_pages || (b2 == b && j <= j0)) continue;

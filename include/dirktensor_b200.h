@@ -396,8 +396,8 @@ typedef struct dt_kv_cache {
  * [B, T, kv_heads, 128], heads 128 elements apart, tokens and sequences at the
  * given strides (in elements; multiples of 16 bytes).  page_table: device
  * int[B, max_pages], rows page_table_stride apart.  start, lens: device int[B]
- * or NULL (0, and T).  A token whose position is negative or past the table,
- * or whose page id is not in 0..num_pages-1, is skipped.  Where one call maps
+ * or NULL (0, and T).  A token whose position is negative, past the table or past
+ * 2^31 - 1, or whose page id is not in 0..num_pages-1, is skipped.  Where one call maps
  * several tokens to one slot, the one of the highest (b, position) is kept.
  * The cache's four arrays must not overlap (a cache that is only read may share them).
  * Asynchronous on `stream`. */

@@ -55,3 +55,19 @@ def test_strides_of_dimensions_of_one_do_not_matter(dt, cuda, dtype, B, T):
     k, v = c.k.clone(), c.v_scale.clone()
     c.append(q, q, table)
     assert torch.equal(c.k, k) and torch.equal(c.v_scale, v)
+
+
+def test_append_past_the_last_position_takes_no_slot(dt, cuda):
+    """Positions end at 2^31 - 1: tokens past it are skipped, and give way to those that are written."""
+    page, last = 256, (1 << 31) // 256 - 1
+    c = dt.KVCache(3, page, 1)
+    table = torch.full((2, last + 3), -1, dtype=torch.int32, device=cuda)
+    table[0, 0], table[1, last], table[1, last + 1] = 0, 1, 0
+    k = torch.randn((2, 20, 1, D), generator=torch.Generator(device=cuda).manual_seed(1), device=cuda)
+    start = ints(cuda, 0, (1 << 31) - 10)
+    c.append(k, k, table, start)
+    back, _ = c.read(table, start, 20, dtype=F32)
+    dt.check_device_error()
+    assert bool((c.k_scale[0, 0, :20] > 0).all()) and bool((c.k_scale[1, 0, 246:] > 0).all())
+    assert int((c.k_scale > 0).sum()) == 30
+    assert bool((back[0] != 0).any(-1).all()) and bool((back[1, :10] != 0).any(-1).all()) and bool((back[1, 10:] == 0).all())
