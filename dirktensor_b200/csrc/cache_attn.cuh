@@ -532,7 +532,8 @@ __device__ __forceinline__ void attend(const Params& p, Stage* ring, int b, int 
         for (int z = 0; z < kSets; ++z)
 #pragma unroll
             for (int c = 0; c < kCols; ++c) {
-                top[z][c] = fmaxf(fmaxf(u[z][0][0][c], u[z][0][1][c]), fmaxf(u[z][1][0][c], u[z][1][1][c]));
+                // (scales of a caller's own codes may be below zero)
+                top[z][c] = fmaxf(fmaxf(fabsf(u[z][0][0][c]), fabsf(u[z][0][1][c])), fmaxf(fabsf(u[z][1][0][c]), fabsf(u[z][1][1][c])));
                 grows |= top[z][c] * st.f[z][c] > 32768.f;
             }
         if (__any_sync(0xffffffffu, grows)) {

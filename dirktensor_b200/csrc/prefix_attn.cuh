@@ -67,7 +67,7 @@ struct __align__(1024) Smem {
     uint8_t v[2][kTileBytes];
     float ks[4][kBN];           // of tile t: at t & 3
     float vs[4][kBN];
-    float most[4][kConvWarps], least[4][kConvWarps];  // largest and smallest v_scale of the 32 keys of each converting warp
+    float most[4][kConvWarps], least[4][kConvWarps];  // largest and smallest |v_scale| of the 32 keys of each converting warp
     uint32_t hidden[4][kConvWarps];  // keys past the prefix, or on a page that does not exist
     float factor[2][kBM];       // from S back to scores in log2 units (k_scale apart)
     float m[kBM], l[kBM], mx[kBM];  // of the second warpgroup, for the first (pairs)
@@ -231,9 +231,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const Params pp) {
                 if (!ok) break;
                 sm.ks[j & 3][cw * 32 + lane] = ks;
                 sm.vs[j & 3][cw * 32 + lane] = vs;
-                // (scales are not negative, so their bits order as they do; a NaN is neither the largest nor the smallest)
-                const uint32_t most = __reduce_max_sync(0xffffffffu, vs > 0.f ? __float_as_uint(vs) : 0u);
-                const uint32_t least = __reduce_min_sync(0xffffffffu, see && vs == vs ? __float_as_uint(vs) : 0x7f800000u);
+                // (sizes: their bits order as they do; a NaN is neither the largest nor the smallest)
+                const uint32_t size = __float_as_uint(fabsf(vs));
+                const uint32_t most = __reduce_max_sync(0xffffffffu, vs == vs ? size : 0u);
+                const uint32_t least = __reduce_min_sync(0xffffffffu, see && vs == vs ? size : 0x7f800000u);
                 const uint32_t seen = __ballot_sync(0xffffffffu, see);
                 if (lane == 0) {
                     sm.most[j & 3][cw] = __uint_as_float(most), sm.least[j & 3][cw] = __uint_as_float(least);
@@ -492,7 +493,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const Params pp) {
                     tmem_wait_ld();
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
-                        z = fmaxf(z, fmaf(x[e] * sm.ks[at][cc * 16 + e], factor, __log2f(sm.vs[at][cc * 16 + e])));
+                        z = fmaxf(z, fmaf(x[e] * sm.ks[at][cc * 16 + e], factor, __log2f(fabsf(sm.vs[at][cc * 16 + e]))));
                 }
                 eb = (int)ceilf(fminf(fmaxf(z - m, -1000.f), 1000.f)) + 1;
             }

@@ -156,7 +156,7 @@ def prefix_ref(dt, c, pages, n, q, group):
         rel = 2 * d + 8 * ref.EPS32 * (1 + (p * (top[..., None] - s)).sum(-1)) + 2 * n * ref.EPS32
         o.append(torch.matmul(p, v))
         o_tol.append(ref.HALF[q.dtype] * o[-1].abs() + 2 * (rel + p_half)[..., None] * torch.matmul(p, v.abs()) +
-                     2.0 ** -25 * (p * vs).amax(-1, keepdim=True) * codes.sum(0))
+                     2.0 ** -25 * (p * vs.abs()).amax(-1, keepdim=True) * codes.sum(0))
         m.append(top), m_tol.append(d + ref.EPS32 * top.abs())
         l.append(w.sum(-1)), l_tol.append(rel * w.sum(-1))
     return [torch.cat(x, dim=2) for x in (o, m, l, o_tol, m_tol, l_tol)]
@@ -237,3 +237,20 @@ def test_prefix_of_small_queries_and_scales_with_hidden_keys(dt, cuda, dtype, B,
         own = dt.cache_attention_forward(q, c, given_pages[None].expand(B, -1).contiguous(),
                                          torch.full((B,), prefix + T - 1, dtype=torch.int32, device=cuda), scale)
         assert bool(torch.isfinite(own).all())
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype, B, T", PREFIX_ROWS)
+@pytest.mark.parametrize("sizes", [(1.0, 1.0), (2.0 ** 40, 1.0), (2.0 ** -40, 2.0 ** 20)])
+def test_scales_of_either_sign(dt, cuda, fmt, dtype, B, T, sizes):
+    """A caller's own codes may have scales below zero (append writes none): their size is what the weights' factor goes by."""
+    n = 1300
+    c, table, lens, q = given(dt, cuda, fmt, dtype, 1, 1, HEADS, 1, [0.2 * (j % 7) for j in range(n)],
+                              [sizes[j % 2] for j in range(n)])
+    c.v_scale[:, :, ::2] *= -1
+    c.k_scale[:, :, 1::3] *= -1
+    q = q.expand(B, T, HEADS, D)
+    got = dt.prefix_attention_forward(q, c, table[0], n, None, None, SCALE, return_stats=True)
+    ref.check_attention([x[:, :, SEEN] for x in got], prefix_ref(dt, c, table[0], n, q, 1))
+    got = dt.cache_attention_forward(q[:1, :1], c, table, lens, SCALE, return_stats=True)
+    ref.check_attention([x[:, :, SEEN] for x in got], prefix_ref(dt, c, table[0], n, q[:1, :1], 1))
