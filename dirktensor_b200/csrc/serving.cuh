@@ -86,8 +86,6 @@ int dt_kv_cache_append(const dt_kv_cache* cache, const void* k, long long k_batc
     p.k_token = k_token_stride;
     p.v_batch = v_batch_stride;
     p.v_token = v_token_stride;
-    int dev;
-    DT_TRY(prepare_device(&dev));
     // A CTA takes 32 rows at a time: as many tokens as that are, or up to four times so many where there are more CTAs than
     // the GPU holds (8 per SM); at most 16, the smallest page.
     const long long rows = 2ll * B * T * p.c.heads;
@@ -97,6 +95,8 @@ int dt_kv_cache_append(const dt_kv_cache* cache, const void* k, long long k_batc
     p.tiles = (T + p.tile - 1) / p.tile;
     if ((long long)p.tiles * B > 0x7fffffffll || (T / cache->page_size + 2ll) * B > 0x7fffffffll)
         return fail(DT_ERR_INVALID_ARGUMENT, "B * T is too large");
+    int dev;
+    DT_TRY(prepare_device(&dev));
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     const dim3 grid((unsigned)(p.tiles * B)), block(dt::kv::kThreads);
     if (cache->format == DT_KV_INT8)
@@ -353,9 +353,10 @@ int cache_attn(const dt_kv_cache* cache, const void* q, long long q_batch_stride
     p.scale = scale;
     const PrefixPlan prefix = prefix_len > 0 ? plan_prefix(B, T, heads, cache->kv_heads, q_f32, prefix_len) : PrefixPlan{};
     const AttnPlan plan = plan_attn(B, T, heads, cache->kv_heads, q_f32, cache->page_size, max_pages, prefix.split);
+    // (so many parts of a prefix go with at most 8 blocks of 256 query rows, well below kMaxBatch sequences: what is left
+    // is the batch's count of tiles)
     if (plan.shares < 0)
-        return fail(DT_ERR_INVALID_ARGUMENT, "behind a prefix, B must be at most %d and the page table below 2^31 tokens",
-                    dt::cache_attn::kMaxBatch);
+        return fail(DT_ERR_INVALID_ARGUMENT, "behind a prefix in more than 16 parts, B * max_pages * page_size must be below 2^36");
     if (plan.items * std::max(plan.split, 1) > 0x7fffffffll)
         return fail(DT_ERR_INVALID_ARGUMENT, "B * kv_heads * query rows is too large");
     const AttnSpace space = attn_space(plan, B, T, heads, prefix.split);

@@ -439,7 +439,9 @@ int dt_cache_attn_fwd(const dt_kv_cache* cache, const void* q, long long q_batch
  * device int[ceil(prefix_len / page_size)]; prefix_len at most 2^30) and then its own sequence's keys
  * as above, whose positions, page_table and seq_lens count from the prefix's
  * end.  The prefix is read once for the whole batch, not once per sequence.
- * max_pages may be 0 (no keys of their own); B is at most 8192.  workspace: at least
+ * max_pages may be 0 (no keys of their own).  Where few query rows leave the
+ * prefix in more than 16 parts (B * T * heads of at most 2048 rows), B * max_pages *
+ * page_size must be below 2^36.  workspace: at least
  * dt_prefix_attn_workspace_bytes, 16-byte aligned (NULL when that is 0); calls
  * that may overlap on the GPU need one each. */
 size_t dt_prefix_attn_workspace_bytes(int B, int T, int heads, int kv_heads, int q_f32, int page_size, int max_pages,

@@ -1,11 +1,12 @@
-"""CPU tests of the serving operators' limits at the C ABI: what is refused before a device is touched."""
+"""CPU tests of the serving operators' limits at the C ABI: what is refused before a device is touched.  A call that
+passes the check in question is refused by a later one, so that none reaches a device, whether or not there is one."""
 import ctypes
 
 import pytest
 
 from dirktensor_b200 import _lib
 
-FAKE = 1 << 20  # 16-byte aligned, never dereferenced: every case is refused, or fails where no device is
+FAKE = 1 << 20  # 16-byte aligned, never dereferenced: every case is refused
 
 
 def cache(**kw):
@@ -32,11 +33,12 @@ def test_an_output_that_overlaps_its_queries_is_refused(prefix_len):
     def overlaps(delta, B=2, T=3, H=4, qb=None, qt=512, f32=0):
         q = 64 * FAKE
         qb = T * qt if qb is None else qb
-        args = (B, T, H, 4, f32, 64, 4, prefix_len)
-        status = L.dt_prefix_attn_fwd(cache(), q, qb, qt, f32, q + delta, None, None, 7 * FAKE, prefix_len, 9 * FAKE, 4, 4, 10 * FAKE,
-                                      None, B, T, H, 0.1, 8 * FAKE, L.dt_prefix_attn_workspace_bytes(*args) + 16, None)
-        assert status != 0
-        return status == 1 and b"overlap" in L.dt_last_error()
+        # a prefix, or few items of many keys, need a workspace, and get none
+        assert L.dt_prefix_attn_workspace_bytes(B, T, H, 4, f32, 64, 4096, prefix_len) > 0
+        status = L.dt_prefix_attn_fwd(cache(), q, qb, qt, f32, q + delta, None, None, 7 * FAKE, prefix_len, 9 * FAKE, 4096, 4096,
+                                      10 * FAKE, None, B, T, H, 0.1, None, 0, None)
+        assert status == 1 and (b"overlap" in L.dt_last_error()) != (b"workspace" in L.dt_last_error())
+        return b"overlap" in L.dt_last_error()
 
     row = 4 * 128 * 2  # of one token
     assert not overlaps(0) and not overlaps(0, f32=1)                       # in place
@@ -56,13 +58,27 @@ def test_append_into_a_cache_whose_arrays_overlap_is_refused():
     codes, scales = 8 * 4 * 64 * 128, 8 * 4 * 64 * 4  # bytes of cache()'s arrays
 
     def refused(**kw):
-        status = L.dt_kv_cache_append(cache(**kw), 5 * FAKE, 512, 512, 6 * FAKE, 512, 512, 0, 7 * FAKE, 4, 4, None, None, 1, 1, None)
-        assert status != 0
-        return status == 1 and b"overlap" in L.dt_last_error()
+        status = L.dt_kv_cache_append(cache(**kw), 5 * FAKE, 512, 512, 6 * FAKE, 512, 512, 0, 7 * FAKE, 4, 4, None, None, 1 << 20,
+                                      1 << 20, None)
+        assert status == 1 and (b"overlap" in L.dt_last_error()) != (b"too large" in L.dt_last_error())
+        return b"overlap" in L.dt_last_error()
 
     assert not refused()
     assert refused(v=FAKE) and refused(v_scale=3 * FAKE) and refused(v=FAKE + codes - 16) and refused(k=2 * FAKE + codes - 16)
     assert not refused(v=FAKE + codes) and not refused(v_scale=3 * FAKE + scales) and refused(v_scale=3 * FAKE + scales - 16)
     assert refused(k_scale=FAKE + 1024) and refused(v_scale=2 * FAKE - 16)
-    status = L.dt_kv_cache_read(cache(v=FAKE, v_scale=3 * FAKE), 5 * FAKE, 6 * FAKE, 0, 7 * FAKE, 4, 4, None, None, 1, 1, None)
-    assert status != 1
+
+
+def test_a_prefix_in_many_parts_before_a_very_wide_page_table_is_refused():
+    """Few query rows over a long prefix: what every sequence has of its own is counted in 32-bit tiles over the batch."""
+    L = _lib.lib()
+
+    def refused(B, pages):
+        status = L.dt_prefix_attn_fwd(cache(page_size=256, kv_heads=1), 5 * FAKE, 128, 128, 0, 1 << 40, None, None, 7 * FAKE,
+                                      1 << 20, 9 * FAKE, pages, pages, 10 * FAKE, None, B, 1, 1, 0.1, None, 0, None)
+        assert status == 1 and (b"2^36" in L.dt_last_error()) != (b"workspace" in L.dt_last_error()), L.dt_last_error()
+        return b"2^36" in L.dt_last_error()
+
+    assert refused(64, 1 << 22) and refused(2048, 1 << 18)
+    assert not refused(63, 1 << 22) and not refused(64, (1 << 22) - 1)
+    assert not refused(10000, 4) and not refused(1 << 20, 4)  # no limit on the batch itself

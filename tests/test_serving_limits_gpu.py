@@ -71,3 +71,28 @@ def test_append_past_the_last_position_takes_no_slot(dt, cuda):
     assert bool((c.k_scale[0, 0, :20] > 0).all()) and bool((c.k_scale[1, 0, 246:] > 0).all())
     assert int((c.k_scale > 0).sum()) == 30
     assert bool((back[0] != 0).any(-1).all()) and bool((back[1, :10] != 0).any(-1).all()) and bool((back[1, 10:] == 0).all())
+
+
+def test_a_large_batch_behind_a_prefix(dt, cuda):
+    """More than 8192 sequences: what some of them get is what they get alone, within the bounds."""
+    import serving_ref as ref
+
+    B, some = 9001, [0, 1, 127, 128, 255, 256, 4500, 8191, 8192, 8999, 9000]
+    c, pages, table, lens, q = attention_case(dt, cuda, 63, "int8", BF16, B, 1, 1, 1, 16, [i % 31 for i in range(B)], 300)
+    got = dt.prefix_attention_forward(q, c, pages, 300, table, lens, SCALE, return_stats=True)
+    dt.check_device_error()
+    want = ref.attention(q[some], c, table[some], lens[some], SCALE, prefix_pages=pages, prefix_len=300)
+    ref.check_attention([x[some] for x in got], want)
+
+
+def test_a_cache_that_shares_its_arrays_is_read_and_not_written(dt, cuda):
+    c, _, table, lens, q = attention_case(dt, cuda, 64, "int8", BF16, 2, 1, 2, 1, 16, [20, 7])
+    same = dt.KVCache.from_tensors(c.k, c.k, c.k_scale, c.k_scale)
+    k, v = same.read(table, None, 20)
+    assert torch.equal(k, v)
+    other = dt.KVCache.from_tensors(c.k, c.k.clone(), c.k_scale, c.k_scale.clone())
+    assert torch.equal(dt.cache_attention_forward(q, same, table, lens, SCALE), dt.cache_attention_forward(q, other, table, lens, SCALE))
+    before = c.k.clone()
+    with pytest.raises(dt.DTError, match="overlap"):
+        same.append(q, q, table)
+    assert torch.equal(c.k, before)
