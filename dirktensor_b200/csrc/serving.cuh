@@ -490,8 +490,6 @@ int dt_token_log_probs_bwd(const void* logits, int logits_f32, long long ld, int
     if (d_entropy && !entropy) return fail(DT_ERR_INVALID_ARGUMENT, "d_entropy needs entropy");
     if (!writes_apart(logits, ld, d_logits, d_ld, N, V, logits_f32 ? 4 : 2))
         return fail(DT_ERR_INVALID_ARGUMENT, "d_logits may be the logits' own rows, and must not overlap them otherwise");
-    int dev;
-    DT_TRY(prepare_device(&dev));
     namespace lp = dt::logprobs;
     dt::logprobs::GradParams p{logits, ld, N, V, targets, targets_int64 ? 1 : 0, lse, entropy, d_log_prob, d_entropy,
                                d_logits, d_ld, 1};
@@ -500,6 +498,8 @@ int dt_token_log_probs_bwd(const void* logits, int logits_f32, long long ld, int
     const long long vectors = ((long long)V * elem + 15) / 16 + 1;
     p.chunks = (int)((vectors + lp::kGradThreads * lp::kGradVectors - 1) / (lp::kGradThreads * lp::kGradVectors));
     if ((long long)N * p.chunks > 0x7fffffffll) return fail(DT_ERR_INVALID_ARGUMENT, "N * V is too large");
+    int dev;
+    DT_TRY(prepare_device(&dev));
     const bool aligned = ((reinterpret_cast<uintptr_t>(logits) ^ reinterpret_cast<uintptr_t>(d_logits)) & 15) == 0 &&
                          ((ld - d_ld) * elem) % 16 == 0;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);

@@ -82,3 +82,20 @@ def test_a_prefix_in_many_parts_before_a_very_wide_page_table_is_refused():
     assert refused(64, 1 << 22) and refused(2048, 1 << 18)
     assert not refused(63, 1 << 22) and not refused(64, (1 << 22) - 1)
     assert not refused(10000, 4) and not refused(1 << 20, 4)  # no limit on the batch itself
+
+
+def test_overlapping_gradients_are_refused_and_others_pass_that_check():
+    """As for the outputs above: rows of logits and of their gradient, with a device or without (N * V ends it)."""
+    L = _lib.lib()
+
+    def refused(delta, N=1 << 20, V=1 << 30, ld=1 << 30, dld=1 << 30, elem=4):
+        x = 1 << 56
+        status = L.dt_token_log_probs_bwd(x, int(elem == 4), ld, N, V, None, 0, 5 * FAKE, 6 * FAKE, None, None, x + delta, dld, None)
+        assert status == 1 and (b"overlap" in L.dt_last_error()) != (b"too large" in L.dt_last_error())
+        return b"overlap" in L.dt_last_error()
+
+    row = 4 << 30
+    assert refused(4) and refused(-4) and refused(row - 4) and refused(row) and refused(-row) and refused(3 * row)
+    assert refused(0, ld=(1 << 30) + 4) and refused(0, dld=1 << 40) and refused(2, elem=2)
+    assert not refused(0) and not refused(row << 20) and not refused(-(row << 20))
+    assert not refused(row, ld=2 << 30, dld=2 << 30) and refused(row - 4, ld=2 << 30, dld=2 << 30)
