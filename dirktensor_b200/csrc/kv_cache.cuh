@@ -29,6 +29,7 @@ constexpr int kD = 128;
 constexpr int kThreads = 256;
 constexpr int kRowLanes = 8;                      // lanes per row of 128 values, 16 values each
 constexpr int kRows = kThreads / kRowLanes;       // rows a CTA handles at once
+constexpr int kEntries = 2048;                    // page entries of a launch that writes
 constexpr float kTiny = 7.888609052210118e-31f;   // 2^-100
 constexpr float kHuge = 1.2676506002282294e30f;   // 2^100
 
@@ -51,7 +52,16 @@ struct Span {                 // which tokens of which sequences a call touches
     const int* start;         // [B] position of the first token (null: 0)
     const int* lens;          // [B] tokens of each sequence, at most T (null: T)
     int B, T;
+    int first;                // tokens of each sequence before the T ones of this launch
 };
+
+// Tokens of sequence b among the launch's T (none: 0 or less).  kLater: the launch has tokens before its own; known at
+// compile time, since the append kernel has no register to spare (4 x 4096 tokens of fp32, written and read back: 101 us, 107 with seven more).
+template <bool kLater>
+__device__ __forceinline__ int length_of(const Span& s, int b) {
+    if (!s.lens) return s.T;
+    return min(kLater ? max(s.lens[b], 0) - s.first : s.lens[b], s.T);
+}
 
 // Page of position pos of sequence b, or -1 where the table has none.
 __device__ __forceinline__ int page_of(const Span& s, const Cache& c, int b, int pos) {
@@ -73,19 +83,22 @@ __device__ __forceinline__ int position(int start, int t) {
 }
 
 // Where a page table gives one slot to several tokens of a call, the token of the highest
-// (sequence, position) is kept.  True if one above (b, pos) writes page `page` at the same
+// (sequence, position) is kept: within a launch by looking through its page entries, and by the order of launches
+// where a call has more than kEntries of them (each CTA looks through all that follow its own, so the time would
+// grow with their square: 163 ms for 4 million tokens of one sequence in pages of 16, 2.9 in stretches).  True if one above (b, pos) writes page `page` at the same
 // offset (pos >= 0), or any offset (pos < 0: above sequence b's page index j0).  The calling
 // lanes share the entries: lane `part` of `parts`.
+template <bool kLater>
 __device__ __forceinline__ bool written_above(const Span& s, const Cache& c, int b, int j0, int pos, int page, int part,
                                               int parts) {
-    const unsigned width = (unsigned)(s.T >> c.page_shift) + 2u;  // pages that one sequence's T tokens can touch
-    const unsigned n = (unsigned)(s.B - b) * width;               // (below 2^31: B * T is)
+    const unsigned width = (unsigned)(s.T >> c.page_shift) + 2u;  // pages that one sequence's tokens can touch
+    const unsigned n = (unsigned)(s.B - b) * width;  // (at most kEntries)
     const int off = pos & ((1 << c.page_shift) - 1);
     for (unsigned i = part; i < n; i += parts) {
         const unsigned skip = i / width;
         const int b2 = b + (int)skip;
-        const int len = s.lens ? min(s.lens[b2], s.T) : s.T;
-        const long long first = s.start ? s.start[b2] : 0, last = min(first + len - 1, 0x7fffffffll);
+        const int len = length_of<kLater>(s, b2);
+        const long long first = (s.start ? s.start[b2] : 0) + (kLater ? (long long)s.first : 0ll), last = min(first + len - 1, 0x7fffffffll);
         if (len <= 0) continue;
         const long long j = (first >> c.page_shift) + (i - skip * width);
         if (j < 0 || j > (last >> c.page_shift) || j >= s.max_pages || (b2 == b && j <= j0)) continue;
@@ -161,15 +174,19 @@ struct AppendParams {
 // Quantises and stores the new tokens.  A CTA takes `tile` tokens of one sequence, 8 lanes
 // per row; lane l holds the row's 16-byte source chunks l, l + 8, ..., so that loads and
 // stores of a row are contiguous over its lanes.
-template <int kFmt, bool kF32>
+template <int kFmt, bool kF32, bool kLater>
 __global__ void __launch_bounds__(kThreads) append_kernel(const AppendParams p) {
     pdl_enter();
     const int b = (int)(blockIdx.x / (unsigned)p.tiles);
     const int t0 = (int)(blockIdx.x % (unsigned)p.tiles) * p.tile;
-    const int len = p.s.lens ? min(p.s.lens[b], p.s.T) : p.s.T;
-    const int t1 = min(t0 + p.tile, len);
+    const int t1 = min(t0 + p.tile, length_of<kLater>(p.s, b));
     if (t0 >= t1) return;
-    const int start = p.s.start ? p.s.start[b] : 0;
+    int start = p.s.start ? p.s.start[b] : 0;
+    if (kLater) {
+        const long long from = (long long)start + p.s.first;
+        if (from > 0x7fffffffll) return;  // past the last position
+        start = (int)from;
+    }
     const int lane = threadIdx.x & (kRowLanes - 1);
     const int per_token = 2 * p.c.heads;
     const int rows = (t1 - t0) * per_token;
@@ -181,8 +198,8 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendParams p) 
         const int pa = page_of(p.s, p.c, b, first), pb = page_of(p.s, p.c, b, last);
         const int ja = first >> p.c.page_shift, jb = last >> p.c.page_shift;
         bool contested = false;
-        if (pa >= 0) contested = written_above(p.s, p.c, b, ja, -1, pa, threadIdx.x, kThreads);
-        if (pb >= 0 && jb != ja) contested |= written_above(p.s, p.c, b, jb, -1, pb, threadIdx.x, kThreads);
+        if (pa >= 0) contested = written_above<kLater>(p.s, p.c, b, ja, -1, pa, threadIdx.x, kThreads);
+        if (pb >= 0 && jb != ja) contested |= written_above<kLater>(p.s, p.c, b, jb, -1, pb, threadIdx.x, kThreads);
         return __syncthreads_or(contested) != 0;
     };
     // A row of 8 lanes: K or V of head h of a token; the next one is 32 rows on.
@@ -222,7 +239,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendParams p) 
         if (rest >= per_token) rest -= per_token, ++t;
         if (r0 + kRows < rows) load(ahead);  // the next rows are on their way while these are coded
         if (contested) {
-            const bool lost = page >= 0 && written_above(p.s, p.c, b, pos >> p.c.page_shift, pos, page, lane, kRowLanes);
+            const bool lost = page >= 0 && written_above<kLater>(p.s, p.c, b, pos >> p.c.page_shift, pos, page, lane, kRowLanes);
             const uint32_t votes = __ballot_sync(0xffffffffu, lost);
             if ((votes >> (threadIdx.x & 24)) & 0xffu) page = -1;
         }

@@ -79,31 +79,43 @@ int dt_kv_cache_append(const dt_kv_cache* cache, const void* k, long long k_batc
     DT_TRY(check_strides("k", k, k_batch_stride, k_token_stride, elem));
     DT_TRY(check_strides("v", v, v_batch_stride, v_token_stride, elem));
     if (!arrays_apart(cache)) return fail(DT_ERR_INVALID_ARGUMENT, "cache arrays that are written must not overlap");
-    p.s = {page_table, page_table_stride, max_pages, start, lens, B, T};
-    p.k = k;
-    p.v = v;
     p.k_batch = k_batch_stride;
     p.k_token = k_token_stride;
     p.v_batch = v_batch_stride;
     p.v_token = v_token_stride;
+    // Page entries of a sequence's tokens, and how many sequences, and tokens of one, a launch takes: later ones write
+    // after it, as the highest (b, position) is to.
+    const int width = T / cache->page_size + 2;
+    if ((long long)width * B > 0x7fffffffll) return fail(DT_ERR_INVALID_ARGUMENT, "B * T is too large");
+    const int seqs = std::max(1, dt::kv::kEntries / width);
+    const int tokens = width <= dt::kv::kEntries ? T : (dt::kv::kEntries - 2) * cache->page_size;
     // A CTA takes 32 rows at a time: as many tokens as that are, or up to four times so many where there are more CTAs than
     // the GPU holds (8 per SM); at most 16, the smallest page.
-    const long long rows = 2ll * B * T * p.c.heads;
+    const long long rows = 2ll * std::min(B, seqs) * std::min(T, tokens) * p.c.heads;
     const int once = std::max(1, dt::kv::kRows / (2 * p.c.heads));
     const int times = (int)std::min<long long>(4, std::max<long long>(1, rows / (dt::kv::kRows * 8ll * kPlanSms)));
     p.tile = std::min(16, once * times);
-    p.tiles = (T + p.tile - 1) / p.tile;
-    if ((long long)p.tiles * B > 0x7fffffffll || (T / cache->page_size + 2ll) * B > 0x7fffffffll)
-        return fail(DT_ERR_INVALID_ARGUMENT, "B * T is too large");
     int dev;
     DT_TRY(prepare_device(&dev));
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    const dim3 grid((unsigned)(p.tiles * B)), block(dt::kv::kThreads);
-    if (cache->format == DT_KV_INT8)
-        return src_f32 ? launch_pdl(dt::kv::append_kernel<0, true>, grid, block, 0, st, p)
-                       : launch_pdl(dt::kv::append_kernel<0, false>, grid, block, 0, st, p);
-    return src_f32 ? launch_pdl(dt::kv::append_kernel<1, true>, grid, block, 0, st, p)
-                   : launch_pdl(dt::kv::append_kernel<1, false>, grid, block, 0, st, p);
+    typedef void (*AppendKernel)(dt::kv::AppendParams);
+    const bool e4m3 = cache->format == DT_KV_E4M3;
+    const AppendKernel from_first = e4m3 ? (src_f32 ? dt::kv::append_kernel<1, true, false> : dt::kv::append_kernel<1, false, false>)
+                                         : (src_f32 ? dt::kv::append_kernel<0, true, false> : dt::kv::append_kernel<0, false, false>);
+    const AppendKernel later = e4m3 ? (src_f32 ? dt::kv::append_kernel<1, true, true> : dt::kv::append_kernel<1, false, true>)
+                                    : (src_f32 ? dt::kv::append_kernel<0, true, true> : dt::kv::append_kernel<0, false, true>);
+    for (int b = 0; b < B; b += std::min(seqs, B - b))
+        for (int t = 0; t < T; t += std::min(tokens, T - t)) {
+            const int n = std::min(seqs, B - b), len = std::min(tokens, T - t);
+            p.s = {page_table ? page_table + b * page_table_stride : nullptr, page_table_stride, max_pages,
+                   start ? start + b : nullptr, lens ? lens + b : nullptr, n, len, t};
+            p.k = static_cast<const char*>(k) + (b * k_batch_stride + t * k_token_stride) * elem;
+            p.v = static_cast<const char*>(v) + (b * v_batch_stride + t * v_token_stride) * elem;
+            p.tiles = (len + p.tile - 1) / p.tile;
+            // (a launch has at most kEntries pages of at most 256 tokens)
+            DT_TRY(launch_pdl(t > 0 ? later : from_first, dim3((unsigned)(p.tiles * n)), dim3(dt::kv::kThreads), 0, st, p));
+        }
+    return DT_OK;
 }
 
 int dt_kv_cache_read(const dt_kv_cache* cache, void* k, void* v, int dst_f32, const int* page_table,
@@ -117,7 +129,7 @@ int dt_kv_cache_read(const dt_kv_cache* cache, void* k, void* v, int dst_f32, co
     DT_TRY(check_table(page_table, page_table_stride, max_pages, B));
     if (!k || !v || !aligned16(k) || !aligned16(v))
         return fail(DT_ERR_INVALID_ARGUMENT, "k and v must be non-null and 16-byte aligned");
-    p.s = {page_table, page_table_stride, max_pages, start, lens, B, T};
+    p.s = {page_table, page_table_stride, max_pages, start, lens, B, T, 0};
     p.k = k;
     p.v = v;
     p.rows = (long long)B * T * 2 * p.c.heads;

@@ -96,3 +96,96 @@ def test_a_cache_that_shares_its_arrays_is_read_and_not_written(dt, cuda):
     with pytest.raises(dt.DTError, match="overlap"):
         same.append(q, q, table)
     assert torch.equal(c.k, before)
+
+
+def winners(table, start, lens, page, T):
+    """Slot (page * page size + offset) and token number b * T + t of each token that stays, in 64-bit indexes."""
+    B = table.shape[0]
+    t = torch.arange(T, device=table.device)
+    pos = start.long()[:, None] + t
+    at = torch.gather(table.long(), 1, (pos // page).clamp(max=table.shape[1] - 1))
+    live = (t < lens.long()[:, None]) & (pos // page < table.shape[1]) & (at >= 0)
+    slot = (at * page + pos % page)[live]
+    token = (torch.arange(B, device=table.device)[:, None] * T + t)[live]
+    best = torch.full((int(slot.max()) + 1,), -1, dtype=torch.int64, device=table.device)
+    best.scatter_reduce_(0, slot, token, "amax")
+    used = best >= 0
+    return torch.nonzero(used)[:, 0], best[used]
+
+
+@pytest.mark.parametrize("B, T, page, pool", [(9000, 1, 16, 700), (9000, 1, 64, 20000), (300, 600, 16, 4000), (2, 150000, 16, 9000),
+                                              (1, 140000, 16, 9000), (5, 70001, 64, 3000)])
+def test_appends_of_many_pages_keep_the_last_token_of_a_slot(dt, cuda, B, T, page, pool):
+    """More page entries than one launch looks through: pages that are named twice, near and far apart, short and long lengths."""
+    g = torch.Generator(device=cuda).manual_seed(B + T)
+    heads, per = 1, -(-(T + 40) // page)
+    c = dt.KVCache(pool, page, heads)
+    table = torch.randint(-1, pool, (B, per), generator=g, device=cuda).to(torch.int32)
+    start = torch.randint(0, 40, (B,), generator=g, device=cuda).to(torch.int32)
+    lens = torch.randint(0, T + 3, (B,), generator=g, device=cuda).to(torch.int32)
+    lens[-1] = T
+    k = torch.randn((B, T, heads, D), generator=g, device=cuda).to(BF16)
+    c.append(k, k.flip(1), table, start, lens)
+    dt.check_device_error()
+    slot, token = winners(table, start, lens.clamp(max=T), page, T)
+    for x, scales, codes in ((k, c.k_scale, c.k), (k.flip(1), c.v_scale, c.v)):
+        y = x.reshape(-1, D)[token].float()
+        amax = y.abs().amax(-1)
+        assert torch.equal(scales.view(-1)[slot], amax / torch.full_like(amax, 127.0))
+        assert torch.equal(codes.view(-1, D)[slot], (y * 127 / amax[:, None]).round().to(torch.int8))
+        assert int((scales > 0).sum()) == len(slot)
+
+
+def test_the_time_of_an_append_grows_with_its_tokens(dt, cuda):
+    """4 million tokens on pages of their own: the search for tokens that share a slot took 163 ms, by the square of the
+    tokens; in stretches it is some 3 ms."""
+    T, page = 1 << 22, 16
+    c = dt.KVCache(T // page, page, 1)
+    table = torch.randperm(T // page, device=cuda).to(torch.int32)[None]
+    k = torch.ones((1, 1, 1, D), dtype=BF16, device=cuda).expand(1, T, 1, D)
+    times = []
+    for _ in range(4):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        c.append(k, k, table)
+        b.record()
+        torch.cuda.synchronize()
+        times.append(a.elapsed_time(b))
+    assert bool((c.k_scale > 0).all()) and min(times) < 60.0, times
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_a_long_append_in_every_type(dt, cuda, fmt, dtype):
+    """Tokens of a sequence that a later launch writes, on pages that earlier ones name too, and past the last position."""
+    from serving_ref import TOP
+
+    g = torch.Generator(device=cuda).manual_seed(7)
+    T, page, heads, pool = 100003, 16, 2, 5000
+    c = dt.KVCache(pool, page, heads, fmt)
+    table = torch.randint(0, pool, (1, 6300), generator=g, device=cuda).to(torch.int32)
+    start, lens = ints(cuda, 9), ints(cuda, 99990)
+    k, v = (torch.randn((1, T, heads, D), generator=g, device=cuda).to(dtype) for _ in range(2))
+    c.append(k, v, table, start, lens)
+    dt.check_device_error()
+    slot, token = winners(table, start, lens, page, T)
+    for x, scales, codes in ((k, c.k_scale, c.k), (v, c.v_scale, c.v)):
+        y = x[0, token].float()
+        amax = y.abs().amax(-1)
+        assert torch.equal(scales[slot // page, :, slot % page], amax / torch.full_like(amax, TOP[fmt]))
+        want = y * TOP[fmt] / amax[..., None]
+        got = codes.view(torch.int8)[slot // page, :, slot % page]
+        assert torch.equal(got, (want.round() if fmt == "int8" else want).to(codes.dtype).view(torch.int8))
+    before = c.k.clone(), c.k_scale.clone()
+    c.append(k, v, torch.zeros((1, (1 << 27) + 10), dtype=torch.int32, device=cuda), ints(cuda, (1 << 31) - 40000), ints(cuda, 39990))
+    used = torch.zeros(pool, dtype=torch.bool, device=cuda)
+    used[0] = True
+    assert torch.equal(before[0].view(torch.int8)[~used], c.k.view(torch.int8)[~used])
+    where = ((1 << 31) - 40000 + torch.arange(39990, device=cuda)) % page
+    for off in range(page):
+        last = int(torch.nonzero(where == off)[-1])
+        amax = k[0, last].float().abs().amax(-1)
+        assert torch.equal(c.k_scale[0, :, off], amax / torch.full_like(amax, TOP[fmt]))
+    c.append(k, v, torch.zeros((1, (1 << 27) + 10), dtype=torch.int32, device=cuda), ints(cuda, (1 << 31) - 5), None)
+    first = k[0, :5].float().abs().amax(-1)
+    assert torch.equal(c.k_scale[0, :, 11:], (first / torch.full_like(first, TOP[fmt])).T)
