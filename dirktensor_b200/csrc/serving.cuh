@@ -177,7 +177,8 @@ struct AttnPlan {
 
 // split_kernel, with as many CTAs per item as the GPU holds at once, up to a cluster, and no more
 // than there are tiles for; stream_kernel where that leaves most of the GPU idle: few items with
-// many keys.  (8 x 131071 keys: 149 us in 8 clusters of 8, 70 shared out over 592 CTAs.)
+// many keys.  (8 x 131071 keys: 149 us in 8 clusters of 8, 70 shared out over 592 CTAs.  The rule knows the items and the
+// table's width, not the lengths: of 128 items, 8 of 131071 keys and 120 of 200, split_kernel's even split takes 398 us.)
 // Behind a prefix, split_kernel also joins its rows with the prefix's n_shared parts, if these are few.
 AttnPlan plan_attn(int B, int T, int heads, int kv_heads, int q_f32, int page_size, int max_pages, int n_shared) {
     namespace ca = dt::cache_attn;

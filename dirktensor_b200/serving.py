@@ -4,7 +4,7 @@ given tokens with their gradient.
 
 Arguments are CUDA torch tensors; calls run on the current stream of the tensors' device, do not
 synchronise, and raise ``ValueError`` for arguments they cannot take and ``DTError`` for
-what the library refuses.  The reference has no counterpart: it recomputes every prefix, and its
+what the library refuses.  None records autograd history.  The reference has no counterpart: it recomputes every prefix, and its
 CrossEntropyLoss.cpp:8-43 reduces the loss to one number.
 """
 from __future__ import annotations
@@ -113,7 +113,7 @@ class KVCache:
 
     @classmethod
     def from_tensors(cls, k, v, k_scale, v_scale) -> "KVCache":
-        """A cache over the caller's own arrays, in the layout above."""
+        """A cache over the caller's own arrays, in the layout above.  ``append`` needs four that do not overlap."""
         self = cls.__new__(cls)
         self._take(k, v, k_scale, v_scale)
         return self
@@ -305,7 +305,8 @@ def token_log_probs(logits, targets=None, top: int = 0) -> TokenLogProbs:
 
     logits: [..., V] fp32 or bf16 (rows may be spaced apart); targets: int32 or int64 [...].
     A target outside 0..V-1, such as an ignored label's -100, gives 0.  Ties among the
-    alternatives go to the lower id.  Logits of -inf have probability 0.
+    alternatives go to the lower id.  Logits of -inf have probability 0.  The results have no
+    autograd history, also where the logits have one: token_log_probs_backward is the gradient.
     """
     n, ld = _rows("logits", logits)
     V, shape, dev = logits.shape[-1], logits.shape[:-1], logits.device

@@ -406,8 +406,8 @@ int dt_kv_cache_append(const dt_kv_cache* cache, const void* k, long long k_batc
                        const int* page_table, long long page_table_stride, int max_pages, const int* start,
                        const int* lens, int B, int T, void* stream);
 /* Reads the values of positions start[b] .. start[b] + T - 1 back into dense
- * k, v [B, T, kv_heads, 128], fp32 (dst_f32 = 1) or bf16: code * scale, rounded
- * once.  Rows t >= lens[b], and rows whose position has no valid page, are
+ * k, v [B, T, kv_heads, 128], fp32 (dst_f32 = 1) or bf16: code * scale in fp32, and
+ * then rounded to bf16.  Rows t >= lens[b], and rows whose position has no valid page, are
  * written as zeros. */
 int dt_kv_cache_read(const dt_kv_cache* cache, void* k, void* v, int dst_f32, const int* page_table,
                      long long page_table_stride, int max_pages, const int* start, const int* lens, int B, int T,
@@ -426,7 +426,9 @@ int dt_kv_cache_read(const dt_kv_cache* cache, void* k, void* v, int dst_f32, co
  * t >= q_lens[b] and rows that see no key are written as zeros (m = l = 0).
  * Lengths past the page table are cut to it; keys on a page whose id is not in
  * 0..num_pages-1 are not seen.  Codes are exact in the products, which are
- * summed in fp32.  max_pages * page_size is at most 2^30.  workspace: at least dt_cache_attn_workspace_bytes (which
+ * summed in fp32; the weights of bf16 queries are rounded to fp16 numbers, in a
+ * range that follows each row's largest p * |v| (rows of V may differ in size from
+ * 2^-100 to 2^100).  max_pages * page_size is at most 2^30.  workspace: at least dt_cache_attn_workspace_bytes (which
  * may be 0: then NULL), 16-byte aligned; calls that may overlap on the GPU
  * need one each.  Asynchronous on `stream`. */
 size_t dt_cache_attn_workspace_bytes(int B, int T, int heads, int kv_heads, int q_f32, int page_size, int max_pages);
