@@ -462,9 +462,15 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kF32)) row_kernel(const 
 
 constexpr int kGradThreads = 256;
 constexpr int kGradVectors = 4;  // 16-byte vectors per thread
+// lse in fp32 is off by up to |lse| 2^-24, and so is each p = e^(x - lse), relatively: 2^-12 at this size
+constexpr float kFarLse = 4096.f;
 
 // One pass: a CTA takes a stretch of a row.  kAligned: the rows of both arrays start equally far from a
 // 16-byte boundary, so vectors of one are vectors of the other; else element by element.
+// Where lse is far from zero (at the worst in a row masked whole with the type's lowest value, where it has no digit left
+// for log V) the row's first CTA takes all of it, adds up e^(x - lse) before it writes, and divides by that sum: alone,
+// since the gradient may go where the logits are.  (One such row of 100352 fp32 logits takes 69 us a call, where one near
+// zero takes 16; 1023 of them 297 against 119.)
 template <bool kF32, bool kAligned>
 __global__ void __launch_bounds__(kGradThreads) grad_kernel(const GradParams p) {
     pdl_enter();
@@ -476,8 +482,8 @@ __global__ void __launch_bounds__(kGradThreads) grad_kernel(const GradParams p) 
     const float h = p.d_entropy ? p.d_entropy[row] : 0.f;
     const float lse = p.lse[row], ent = p.entropy ? p.entropy[row] : 0.f;
     const bool empty = lse == -INFINITY;
-    auto grad = [&](float x, int j) {
-        const float lp = max_nan(x - lse, kFar);  // (at -inf too: no weight, and no inf * 0)
+    auto grad = [&](float x, int j, float rest) {  // rest: the log of the sum of e^(x - lse), 0 to lse's digits
+        const float lp = max_nan((x - lse) - rest, kFar);  // (at -inf too: no weight, and no inf * 0)
         float d = -ex2_approx(lp * kLog2e) * fmaf(h, lp + ent, g);
         if (j == t) d += g;
         return empty ? 0.f : d;
@@ -488,21 +494,47 @@ __global__ void __launch_bounds__(kGradThreads) grad_kernel(const GradParams p) 
     };
     constexpr int kN = Vec<kF32>::kN;
     constexpr int kPer = kGradThreads * kGradVectors;  // vectors per CTA
-    if (!kAligned) {
-        const int j0 = chunk * kPer * kN, j1 = min(p.V, j0 + kPer * kN);
-        for (int j = j0 + threadIdx.x; j < j1; j += kGradThreads) put(j, grad(logit<kF32>(p.x, base + j), j));
-        return;
-    }
     const Row<kF32> r(p.x, base, p.V);
-    char* out = static_cast<char*>(p.dx) + (dbase - r.skip) * (kF32 ? 4 : 2);
     const int vectors = r.vectors();
     uint4 y[kGradVectors];
+    if (kAligned) {  // (asked for before anything waits for lse)
 #pragma unroll
-    for (int i = 0; i < kGradVectors; ++i) {
-        const int v = chunk * kPer + i * kGradThreads + threadIdx.x;
-        // (not __ldg: the gradient may go where the logits are)
-        if (v < vectors && r.inside(v)) y[i] = *(reinterpret_cast<const uint4*>(r.base) + v);
+        for (int i = 0; i < kGradVectors; ++i) {
+            const int v = chunk * kPer + i * kGradThreads + threadIdx.x;
+            // (not __ldg: the gradient may go where the logits are)
+            if (v < vectors && r.inside(v)) y[i] = *(reinterpret_cast<const uint4*>(r.base) + v);
+        }
     }
+    if (fabsf(lse) > kFarLse && !isinf(lse)) {
+        if (chunk != 0) return;
+        __shared__ float sums[kGradThreads / 32];
+        float s = 0.f;
+#pragma unroll 4
+        for (int j = threadIdx.x; j < p.V; j += kGradThreads)
+            s += ex2_approx(max_nan(logit<kF32>(p.x, base + j) - lse, kFar) * kLog2e);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = s;
+        __syncthreads();
+        s = 0.f;
+        for (int w = 0; w < kGradThreads / 32; ++w) s += sums[w];
+        const float rest = s > 0.f ? logf(s) : 0.f;  // (0: an lse that is not of these logits)
+        for (int j0 = threadIdx.x; j0 < p.V; j0 += 4 * kGradThreads) {
+            float x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = j0 + i * kGradThreads < p.V ? logit<kF32>(p.x, base + j0 + i * kGradThreads) : 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (j0 + i * kGradThreads < p.V) put(j0 + i * kGradThreads, grad(x[i], j0 + i * kGradThreads, rest));
+        }
+        return;
+    }
+    if (!kAligned) {
+        const int j0 = chunk * kPer * kN, j1 = min(p.V, j0 + kPer * kN);
+        for (int j = j0 + threadIdx.x; j < j1; j += kGradThreads) put(j, grad(logit<kF32>(p.x, base + j), j, 0.f));
+        return;
+    }
+    char* out = static_cast<char*>(p.dx) + (dbase - r.skip) * (kF32 ? 4 : 2);
 #pragma unroll
     for (int i = 0; i < kGradVectors; ++i) {
         const int v = chunk * kPer + i * kGradThreads + threadIdx.x;
@@ -511,7 +543,7 @@ __global__ void __launch_bounds__(kGradThreads) grad_kernel(const GradParams p) 
             const Vec<kF32> z = Row<kF32>::unpack(y[i]);
             float d[kN];
 #pragma unroll
-            for (int e = 0; e < kN; ++e) d[e] = grad(z.x[e], r.id(v, e));
+            for (int e = 0; e < kN; ++e) d[e] = grad(z.x[e], r.id(v, e), 0.f);
             uint32_t w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) w[e] = kF32 ? __float_as_uint(d[e % kN]) : pack_bf16x2(d[2 * e % kN], d[(2 * e + 1) % kN]);
@@ -519,7 +551,7 @@ __global__ void __launch_bounds__(kGradThreads) grad_kernel(const GradParams p) 
         } else {
             for (int e = 0; e < kN; ++e) {
                 const int j = r.id(v, e);
-                if (j >= 0 && j < p.V) put(j, grad(logit<kF32>(p.x, base + j), j));
+                if (j >= 0 && j < p.V) put(j, grad(logit<kF32>(p.x, base + j), j, 0.f));
             }
         }
     }

@@ -472,7 +472,8 @@ int dt_token_log_probs(const void* logits, int logits_f32, long long ld, int N, 
  * apart, from lse and entropy as written there and the upstream gradients
  * d_log_prob and d_entropy (fp32 [N]; either may be NULL for zero):
  *   d_logits[j] = d_log_prob (1[j = target] - p_j) - d_entropy p_j (log p_j + entropy)
- * Rows whose lse is -inf get zeros; d_log_prob of an ignored target is not
+ * p_j = e^(x_j - lse), divided by their sum where |lse| is above 4096, whose fp32 form
+ * has too few digits for it.  Rows whose lse is -inf get zeros; d_log_prob of an ignored target is not
  * used.  d_logits may be the logits' own rows (with d_ld = ld), or lie between them
  * (with d_ld = ld); it is refused where it overlaps them otherwise. */
 int dt_token_log_probs_bwd(const void* logits, int logits_f32, long long ld, int N, int V, const void* targets,
